@@ -244,7 +244,7 @@ def prepare(case, seed):
         zero = torch.zeros(seqs, dtype=torch.int32, device="cuda")
         cache.append(None, dev(k), dev(v), vb.CacheRows(dev(table), dev(every), dev(zero), seqs * longest))
         backend.synchronize()
-        s["attention"] = vb.CacheAttention(backend, cache, case["heads"], max_seqs=seqs, max_rows=seqs * n)
+        s["attention"] = vb.CacheAttention(backend, cache, case["heads"], max_seqs=seqs)
         s["out"], s["mask"] = torch.empty_like(s["q"]), None
         if case["tree"] != "chain":
             words = -(-n // 32)
