@@ -174,6 +174,85 @@ VX_API vx_status vx_gemv_q_rows(vx_context* ctx, const vx_qweights* w, size_t ro
 VX_API vx_status vx_gemv_q_multi(vx_context* ctx, const vx_qweights* const* ws, size_t n_matrices, const float* x,
                                  size_t x_stride, float* const* ys, size_t y_stride, size_t batch);
 
+/* ------------------------------------------------- a quantised cache of keys and values ---- */
+/* No reference counterpart.  Keys and values of the tokens that a decoder has seen, kept as blocks of 32 along the
+ * head dimension in the weights' own formats (Q8_0 / Q4_0, chosen for keys and values separately) and quantised as
+ * they are written: 34 or 18 bytes per 32 values, with vx_quantize's scales and codes.  A block that holds a NaN or an
+ * infinity, or whose scale passes f16, reads back as NaN throughout (its scale is NaN).
+ * The cache is `pages` pages of `page_tokens` tokens (a multiple of 32); which page holds which tokens of a sequence
+ * is the caller's page table.  The device form is tiles of 32 tokens of one head in the order in which the
+ * attention kernel reads them.  Zero at creation.  Any context of the cache's device may use it. */
+typedef struct vx_kv_cache vx_kv_cache;
+VX_API vx_status vx_kv_cache_create(vx_context* ctx, vx_qtype k_type, vx_qtype v_type, size_t heads, size_t head_dim,
+                                    size_t pages, size_t page_tokens, vx_kv_cache** out);
+VX_API vx_status vx_kv_cache_free(vx_context* ctx, vx_kv_cache* cache);
+VX_API vx_status vx_kv_cache_info(const vx_kv_cache* cache, int32_t* k_type, int32_t* v_type, size_t* heads,
+                                  size_t* head_dim, size_t* pages, size_t* page_tokens, size_t* device_bytes);
+/* Which tokens the rows of a call are.  Row begin[s] + i (i < begin[s + 1] - begin[s]) is token start[s] + i of
+ * sequence s, and token p of sequence s lies in page table[s * max_pages + p / page_tokens].  The three arrays are
+ * int32 on the device and are read there when the call's kernels run (a recorded call follows their contents);
+ * `rows` is the number of rows that the call's tensors have.  Whatever the arrays hold, nothing outside the tensors
+ * and the cache is touched: rows that no sequence names, tokens behind the page table's end and tokens whose page
+ * number is negative or too large have no place (they are not written, read back as zeros, and are not attended to);
+ * a sequence whose start is negative has no rows.  The places of two rows of a call must differ: sequences that share
+ * a page may both read it, and what is kept of a block that two rows write at once is not defined. */
+typedef struct {
+    const int32_t* table; /* [seqs][max_pages] */
+    size_t max_pages;
+    const int32_t* begin; /* [seqs + 1], not decreasing */
+    const int32_t* start; /* [seqs] */
+    size_t seqs;
+    size_t rows;
+} vx_kv_rows;
+/* Quantises rows of k and v (heads * head_dim floats each, k_stride / v_stride floats apart) into their places. */
+VX_API vx_status vx_kv_append(vx_context* ctx, vx_kv_cache* cache, const vx_kv_rows* rows, const float* k, size_t k_stride,
+                              const float* v, size_t v_stride);
+/* The reverse: rows of k and v receive the values that the cache's codes stand for.  k or v may be NULL. */
+VX_API vx_status vx_kv_read(vx_context* ctx, const vx_kv_cache* cache, const vx_kv_rows* rows, float* k, size_t k_stride,
+                            float* v, size_t v_stride);
+/* Attention of the rows of a call over the cache.  The call's tokens are in the cache already (vx_kv_append of the same
+ * vx_kv_rows): row i of sequence s attends to the start[s] tokens before them and, among the call's own tokens of
+ * its sequence, to token j if bit j % 32 of mask[(begin[s] + i) * mask_words + j / 32] is set (a tree of drafted tokens: a
+ * row's ancestors and itself; tokens from 32 * mask_words on are not attended to).  With mask NULL, to its tokens
+ * j <= i: one new token per sequence, or a piece of a prompt.
+ *   out[r, h, :] = sum_p softmax_p(scale * q[r, h, :] . k[p, h / group, :]) v[p, h / group, :],   group = heads / cache heads
+ * q and out are rows of heads * head_dim floats, q_stride / out_stride apart; a row that attends to nothing is zeros; rows
+ * of no sequence are left as they were.  Scores, softmax and sums are f32; q and the weights of the softmax enter the
+ * tensor cores as two f16 parts (22 bits, csrc/vx_decode.cuh).  head_dim is 64, 96, 128 or 256 (VX_ERR_UNSUPPORTED
+ * otherwise).  What lies in masked places, NaN included, does not reach the result.
+ * A vx_kv_attention is the workspace of such calls (partial results of sequences that are split over the GPU's SMs),
+ * made once for up to max_seqs sequences; calls with it follow each other on its context's stream.  A
+ * recorded call keeps using it: graphs that may run at the same time need a vx_kv_attention each. */
+typedef struct vx_kv_attention vx_kv_attention;
+VX_API vx_status vx_kv_attention_create(vx_context* ctx, const vx_kv_cache* cache, size_t heads, size_t max_seqs,
+                                        vx_kv_attention** out);
+VX_API vx_status vx_kv_attention_free(vx_context* ctx, vx_kv_attention* attention);
+VX_API vx_status vx_kv_attention_run(vx_context* ctx, const vx_kv_attention* attention, const vx_kv_rows* rows, const float* q,
+                                     size_t q_stride, float* out, size_t out_stride, float scale, const uint32_t* mask,
+                                     size_t mask_words);
+
+/* ------------------------------------------------- a mixture-of-experts layer ---- */
+/* No reference counterpart.  `experts` gated experts on block-quantised weights for a few tokens:
+ *   l = router x;  the top_k largest l (ties to the lowest index, NaN last) choose the experts, with weights softmax(l)
+ *   over all experts, or over the chosen ones if `normalise`;
+ *   y = sum_e weight_e * down_e (silu(gate_e x) * (up_e x)),   silu(a) = a / (1 + exp(-a))
+ * router is f32 on the device, [experts][hidden] (its pointer is kept).  gate and up hold the experts' matrices one
+ * below the other (experts * inner rows, hidden columns, one type), down likewise (experts * hidden rows, inner columns,
+ * its own type): the order of a weight file's three-dimensional expert tensors.  The handles are kept, not copied.
+ * Only the weights of experts that get a token are read, each once per 16 of its tokens.  Three launches.
+ * Sums are f32; x and the inner vector enter the tensor cores as two f16 parts per block (csrc/vx_decode.cuh).
+ * experts <= 256, top_k <= 16 and <= experts, max_tokens <= 64.  The layer owns the workspace of its calls, with the same rule
+ * as vx_kv_attention for calls that overlap.
+ * run: x is `tokens` rows of `hidden` floats, x_stride apart; y likewise.  ids / weights (device, [tokens][top_k], may be
+ * NULL) receive the chosen experts, best first, and their weights.  y must not overlap x. */
+typedef struct vx_moe vx_moe;
+VX_API vx_status vx_moe_create(vx_context* ctx, const float* router, size_t experts, const vx_qweights* gate,
+                               const vx_qweights* up, const vx_qweights* down, size_t top_k, int32_t normalise,
+                               size_t max_tokens, vx_moe** out);
+VX_API vx_status vx_moe_free(vx_context* ctx, vx_moe* moe);
+VX_API vx_status vx_moe_run(vx_context* ctx, const vx_moe* moe, const float* x, size_t x_stride, float* y, size_t y_stride,
+                            size_t tokens, int32_t* ids, float* weights);
+
 /* ------------------------------------------------- several GPUs, one process each ---- */
 /* No reference counterpart (vortx knows one device ordinal, src/linalg/gemm.rs:353).
  * A row-sharded GEMV needs every rank's slab of y on every GPU.  Instead of a collective after

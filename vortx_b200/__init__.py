@@ -11,11 +11,13 @@ from .tensor import Tensor, TensorBuilder, TensorMut, TensorRef
 from .weights_file import WeightFile, write_gguf
 from .linalg import (Contiguous, Gemm, Gemv, GemvBatch, HostStages, MatrixMode, N, OpAssign, OpAssignVariant, Q4_0, Q8_0, QuantizedMatrix,
                      Reduce, ReduceVariant, Repeat, T, dequantize_host, quantize)
+from .decode import CacheAttention, CacheRows, MoeLayer, QuantizedCache, tree_mask
 
 __all__ = [
     "Backend", "BufferUsages", "GpuBuffer", "GpuBufferSlice", "GpuEncoder", "GpuPass",
     "GGML_IDS", "TensorLayout", "TensorLayoutBuffers", "Tensor", "TensorBuilder", "TensorMut",
     "TensorRef", "Gemm", "Gemv", "GemvBatch", "HostStages", "Reduce", "ReduceVariant", "OpAssign", "OpAssignVariant", "Contiguous", "Repeat",
     "MatrixMode", "N", "T", "Q4_0", "Q8_0", "QuantizedMatrix",
+    "QuantizedCache", "CacheRows", "CacheAttention", "MoeLayer", "tree_mask",
     "quantize", "dequantize_host", "WeightFile", "write_gguf", "LayoutError", "ShapeMismatch", "VortxError", "load", "LIB_PATH",
 ]

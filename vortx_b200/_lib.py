@@ -67,6 +67,13 @@ class VxHostStage(C.Structure):
                 ("barrier_flags", C.POINTER(C.c_void_p)), ("world", C.c_size_t), ("rank", C.c_size_t)]
 
 
+class VxKvRows(C.Structure):
+    """vx_kv_rows: which tokens the rows of a cache call are."""
+
+    _fields_ = [("table", C.c_void_p), ("max_pages", C.c_size_t), ("begin", C.c_void_p), ("start", C.c_void_p),
+                ("seqs", C.c_size_t), ("rows", C.c_size_t)]
+
+
 class VortxError(RuntimeError):
     """A non-zero vx_status; `.status` holds the code."""
 
@@ -124,6 +131,17 @@ SIGNATURES = {
     "vx_gemv_q_rows": (C.c_int32, [_P, _P, C.c_size_t, C.c_size_t, _P, C.c_size_t, _P,
                                    C.c_size_t, C.c_size_t]),
     "vx_gemv_q_multi": (C.c_int32, [_P, C.POINTER(_P), C.c_size_t, _P, C.c_size_t, C.POINTER(_P), C.c_size_t, C.c_size_t]),
+    "vx_kv_cache_create": (C.c_int32, [_P, C.c_int, C.c_int, C.c_size_t, C.c_size_t, C.c_size_t, C.c_size_t, C.POINTER(_P)]),
+    "vx_kv_cache_free": (C.c_int32, [_P, _P]),
+    "vx_kv_cache_info": (C.c_int32, [_P, C.POINTER(C.c_int32), C.POINTER(C.c_int32)] + [C.POINTER(C.c_size_t)] * 5),
+    "vx_kv_append": (C.c_int32, [_P, _P, C.POINTER(VxKvRows), _P, C.c_size_t, _P, C.c_size_t]),
+    "vx_kv_read": (C.c_int32, [_P, _P, C.POINTER(VxKvRows), _P, C.c_size_t, _P, C.c_size_t]),
+    "vx_kv_attention_create": (C.c_int32, [_P, _P, C.c_size_t, C.c_size_t, C.POINTER(_P)]),
+    "vx_kv_attention_free": (C.c_int32, [_P, _P]),
+    "vx_kv_attention_run": (C.c_int32, [_P, _P, C.POINTER(VxKvRows), _P, C.c_size_t, _P, C.c_size_t, C.c_float, _P, C.c_size_t]),
+    "vx_moe_create": (C.c_int32, [_P, _P, C.c_size_t, _P, _P, _P, C.c_size_t, C.c_int32, C.c_size_t, C.POINTER(_P)]),
+    "vx_moe_free": (C.c_int32, [_P, _P]),
+    "vx_moe_run": (C.c_int32, [_P, _P, _P, C.c_size_t, _P, C.c_size_t, C.c_size_t, _P, _P]),
     "vx_ipc_export": (C.c_int32, [_P, _P, _P]),
     "vx_ipc_import": (C.c_int32, [_P, _P, C.POINTER(_P)]),
     "vx_ipc_release": (C.c_int32, [_P, _P]),

@@ -1,0 +1,218 @@
+// Attention over the quantised cache: entry points and the kernel that joins the parts of a sequence that was split.
+#include <algorithm>
+#include <memory>
+#include <new>
+#include <type_traits>
+
+#include "vx_kv_attention.cuh"
+
+struct vx_kv_attention {
+    const vx_context* ctx = nullptr;
+    const vx_kv_cache* cache = nullptr;
+    size_t heads = 0, max_seqs = 0;
+    uint32_t grid[5] = {};  // thread blocks by groups of eight rows (1, 2, 4), 0 where there is no such kernel
+    uint8_t* workspace = nullptr;
+    size_t ml_offset = 0, plan_offset = 0;
+};
+
+namespace vx {
+
+// One block per row and query head: the maximum over the parts, then the parts' outputs in turn over four warps.
+// A few parts of D floats each: bound by the latency of two dependent loads.
+__global__ void __launch_bounds__(128) kv_merge_kernel(const AttnParams p, uint32_t R) {
+    __shared__ __align__(16) float parts[3][256];
+    const uint32_t row = blockIdx.x, hq = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, dim = p.g.blocks * 32;
+    const uint32_t seq = warp_search(p.r.seqs, row, [&](uint32_t s) { return (uint32_t)max(p.r.begin[s], 0); });
+    const KvSeq sq = kv_seq(p.r, p.g, seq);
+    if (row < sq.row0 || row - sq.row0 >= sq.n || sq.end == 0) return;
+    const uint64_t total = p.plan[0], blocks = p.plan[1];
+    const uint32_t tiles = (sq.end + kTileTokens - 1) / kTileTokens;
+    const uint32_t groups = (uint32_t)(((uint64_t)sq.n * p.group + R - 1) / R);
+    const uint32_t head = hq / p.group, rr = (row - sq.row0) * p.group + (hq - head * p.group);
+    const uint64_t first = p.plan[2 + seq] + ((uint64_t)head * groups + rr / R) * tiles;
+    const uint64_t c0 = share_of(total, blocks, first), c1 = share_of(total, blocks, first + tiles - 1);
+    if (c0 == c1) return;
+    auto slot = [&](uint64_t c) { return (size_t)c * 2 + (c == c0 && share_begin(total, blocks, c) <= first ? 1 : 0); };
+    float m = -INFINITY, l = 0.0f;
+    for (uint64_t c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, p.part_ml[slot(c) * R + rr % R].x);
+    m = warp_max(m);
+    auto weight = [&](float x) { return x == -INFINITY ? 1.0f : exp2f(x - m); };  // a part that saw nothing is zeros
+    for (uint64_t c = c0 + lane; c <= c1; c += 32) {
+        const float2 f = p.part_ml[slot(c) * R + rr % R];
+        l += f.y * weight(f.x);
+    }
+    l = warp_add(l);
+    const float n = l == 0.0f ? 0.0f : 1.0f / l;
+    float4 o[2] = {make_float4(0.0f, 0.0f, 0.0f, 0.0f), make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
+#pragma unroll 4
+    for (uint64_t c = c0 + warp; c <= c1; c += 4) {
+        const size_t at = slot(c) * R + rr % R;
+        const float w = weight(p.part_ml[at].x);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const uint32_t col = lane * 4 + x * 128;
+            if (col < dim) {
+                const float4 f = *reinterpret_cast<const float4*>(p.part_o + at * dim + col);
+                o[x].x = fmaf(w, f.x, o[x].x);
+                o[x].y = fmaf(w, f.y, o[x].y);
+                o[x].z = fmaf(w, f.z, o[x].z);
+                o[x].w = fmaf(w, f.w, o[x].w);
+            }
+        }
+    }
+    if (warp > 0) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+            if (lane * 4 + x * 128 < dim) *reinterpret_cast<float4*>(&parts[warp - 1][lane * 4 + x * 128]) = o[x];
+    }
+    __syncthreads();
+    if (warp > 0) return;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+        const uint32_t col = lane * 4 + x * 128;
+        if (col >= dim) continue;
+#pragma unroll
+        for (int w = 0; w < 3; ++w) {
+            const float4 f = *reinterpret_cast<const float4*>(&parts[w][col]);
+            o[x].x += f.x;
+            o[x].y += f.y;
+            o[x].z += f.z;
+            o[x].w += f.w;
+        }
+        float* dst = p.out + (size_t)row * p.out_stride + (size_t)hq * dim + col;
+        dst[0] = o[x].x * n;
+        dst[1] = o[x].y * n;
+        dst[2] = o[x].z * n;
+        dst[3] = o[x].w * n;
+    }
+}
+
+extern template vx_status kv_attention_setup<false, false>(uint32_t, uint32_t, int*, uint32_t*);
+extern template vx_status kv_attention_setup<false, true>(uint32_t, uint32_t, int*, uint32_t*);
+extern template vx_status kv_attention_setup<true, false>(uint32_t, uint32_t, int*, uint32_t*);
+extern template vx_status kv_attention_setup<true, true>(uint32_t, uint32_t, int*, uint32_t*);
+extern template vx_status kv_attention_launch<false, false>(uint32_t, uint32_t, uint32_t, cudaStream_t, const AttnParams&);
+extern template vx_status kv_attention_launch<false, true>(uint32_t, uint32_t, uint32_t, cudaStream_t, const AttnParams&);
+extern template vx_status kv_attention_launch<true, false>(uint32_t, uint32_t, uint32_t, cudaStream_t, const AttnParams&);
+extern template vx_status kv_attention_launch<true, true>(uint32_t, uint32_t, uint32_t, cudaStream_t, const AttnParams&);
+
+}  // namespace vx
+
+namespace {
+
+using namespace vx;
+
+bool attn_dim(size_t d) { return d == 64 || d == 96 || d == 128 || d == 256; }
+// Groups of eight rows that the kernels of a head size exist for: four keep their output in 128 registers of a thread
+// at 128 values a head, two at 256.
+uint32_t most_groups(size_t d) { return d == 64 || d == 128 ? 4 : 2; }
+
+vx_status setup(const vx_kv_cache* c, uint32_t nt, int* per_sm, uint32_t* smem) {
+    const bool k4 = c->g.k4, v4 = c->g.v4;
+    if (k4) return v4 ? kv_attention_setup<true, true>(c->g.blocks, nt, per_sm, smem) : kv_attention_setup<true, false>(c->g.blocks, nt, per_sm, smem);
+    return v4 ? kv_attention_setup<false, true>(c->g.blocks, nt, per_sm, smem) : kv_attention_setup<false, false>(c->g.blocks, nt, per_sm, smem);
+}
+
+vx_status launch(const vx_kv_cache* c, uint32_t nt, uint32_t grid, cudaStream_t s, const AttnParams& p) {
+    const bool k4 = c->g.k4, v4 = c->g.v4;
+    if (k4) return v4 ? kv_attention_launch<true, true>(c->g.blocks, nt, grid, s, p) : kv_attention_launch<true, false>(c->g.blocks, nt, grid, s, p);
+    return v4 ? kv_attention_launch<false, true>(c->g.blocks, nt, grid, s, p) : kv_attention_launch<false, false>(c->g.blocks, nt, grid, s, p);
+}
+
+}  // namespace
+
+extern "C" {
+
+vx_status vx_kv_attention_create(vx_context* ctx, const vx_kv_cache* cache, size_t heads, size_t max_seqs, vx_kv_attention** out) {
+    VX_REQUIRE(ctx && cache && out, VX_ERR_INVALID_ARGUMENT, "vx_kv_attention_create: null argument");
+    *out = nullptr;
+    VX_REQUIRE(ctx->device == cache->device, VX_ERR_INVALID_ARGUMENT, "vx_kv_attention_create: the cache is on device %d, the context on %d",
+               cache->device, ctx->device);
+    VX_REQUIRE(heads > 0 && heads % cache->g.heads == 0, VX_ERR_SHAPE, "vx_kv_attention_create: %zu query heads over %u heads of keys", heads,
+               cache->g.heads);
+    VX_REQUIRE(max_seqs > 0, VX_ERR_INVALID_ARGUMENT, "vx_kv_attention_create: max_seqs is 0");
+    VX_REQUIRE(attn_dim(cache->head_dim), VX_ERR_UNSUPPORTED, "vx_kv_attention_create: heads of %zu values (64, 96, 128 and 256 are supported)",
+               cache->head_dim);
+    VX_REQUIRE(heads <= 65535 && max_seqs <= 0x0fffffffull, VX_ERR_UNSUPPORTED, "vx_kv_attention_create: too many heads or sequences");
+    DeviceGuard guard(ctx->device);
+    std::unique_ptr<vx_kv_attention> a(new (std::nothrow) vx_kv_attention());
+    VX_REQUIRE(a, VX_ERR_OUT_OF_MEMORY, "host allocation failed");
+    a->ctx = ctx;
+    a->cache = cache;
+    a->heads = heads;
+    a->max_seqs = max_seqs;
+    size_t rows = 0;
+    for (uint32_t nt = 1; nt <= most_groups(cache->head_dim); nt *= 2) {
+        int per_sm = 0;
+        uint32_t smem = 0;
+        const vx_status st = setup(cache, nt, &per_sm, &smem);
+        if (st != VX_OK) return st;
+        VX_REQUIRE(per_sm > 0, VX_ERR_UNSUPPORTED, "vx_kv_attention_create: the kernel does not fit an SM");
+        a->grid[nt] = (uint32_t)(ctx->sm_count * per_sm);
+        rows = std::max(rows, (size_t)2 * a->grid[nt] * 8 * nt);
+    }
+    a->ml_offset = rows * cache->head_dim * sizeof(float);
+    a->plan_offset = a->ml_offset + rows * sizeof(float2);
+    const size_t bytes = a->plan_offset + (2 + max_seqs) * sizeof(uint64_t);
+    const cudaError_t e = device_malloc(ctx, reinterpret_cast<void**>(&a->workspace), bytes);
+    if (e != cudaSuccess) {
+        (void)cudaGetLastError();
+        return fail(VX_ERR_OUT_OF_MEMORY, "allocating %zu bytes of attention workspace failed: %s", bytes, cudaGetErrorString(e));
+    }
+    *out = a.release();
+    return VX_OK;
+}
+
+vx_status vx_kv_attention_free(vx_context* ctx, vx_kv_attention* a) {
+    VX_REQUIRE(ctx, VX_ERR_INVALID_ARGUMENT, "vx_kv_attention_free: null context");
+    if (!a) return VX_OK;
+    VX_REQUIRE(ctx == a->ctx, VX_ERR_INVALID_ARGUMENT, "vx_kv_attention_free: made with another context");
+    DeviceGuard guard(ctx->device);
+    VX_CUDA(cudaStreamSynchronize(ctx->stream));
+    VX_CUDA(cudaFree(a->workspace));
+    delete a;
+    return VX_OK;
+}
+
+vx_status vx_kv_attention_run(vx_context* ctx, const vx_kv_attention* a, const vx_kv_rows* rows, const float* q, size_t q_stride, float* out,
+                              size_t out_stride, float scale, const uint32_t* mask, size_t mask_words) {
+    VX_REQUIRE(ctx && a, VX_ERR_INVALID_ARGUMENT, "vx_kv_attention_run: null argument");
+    VX_REQUIRE(ctx == a->ctx, VX_ERR_INVALID_ARGUMENT, "vx_kv_attention_run: the workspace was made with another context");
+    AttnParams p{};
+    const vx_status st = kv_rows_check("vx_kv_attention_run", rows, &p.r);
+    if (st != VX_OK || p.r.rows == 0) return st;
+    VX_REQUIRE(rows->seqs <= a->max_seqs, VX_ERR_INVALID_ARGUMENT, "vx_kv_attention_run: %zu sequences, made for %zu", rows->seqs, a->max_seqs);
+    VX_REQUIRE(q && out, VX_ERR_INVALID_ARGUMENT, "vx_kv_attention_run: null q or out");
+    const size_t width = a->heads * a->cache->head_dim;
+    VX_REQUIRE(p.r.rows == 1 || (q_stride >= width && out_stride >= width), VX_ERR_INVALID_ARGUMENT,
+               "vx_kv_attention_run: rows %zu and %zu elements apart, a row has %zu", q_stride, out_stride, width);
+    VX_REQUIRE(!mask || (mask_words > 0 && mask_words <= 0x7ffffffull), VX_ERR_INVALID_ARGUMENT, "vx_kv_attention_run: a mask of %zu words a row", mask_words);
+    const uint32_t group = (uint32_t)(a->heads / a->cache->g.heads);
+    VX_REQUIRE((uint64_t)p.r.rows * group <= 0x7fffffffull, VX_ERR_UNSUPPORTED, "vx_kv_attention_run: too many rows (%u)", p.r.rows);
+    p.g = a->cache->g;
+    p.q = q;
+    p.out = out;
+    p.q_stride = q_stride;
+    p.out_stride = out_stride;
+    p.heads = (uint32_t)a->heads;
+    p.group = group;
+    p.scale_log2 = scale * 1.4426950408889634f;
+    p.mask = mask;
+    p.mask_words = (uint32_t)mask_words;
+    p.part_o = reinterpret_cast<float*>(a->workspace);
+    p.part_ml = reinterpret_cast<float2*>(a->workspace + a->ml_offset);
+    p.plan = reinterpret_cast<uint64_t*>(a->workspace + a->plan_offset);
+    // Rows of a sequence that share a head of keys, as the host can know them: the average.
+    const uint64_t each = ((uint64_t)p.r.rows + p.r.seqs - 1) / p.r.seqs * group;
+    uint32_t nt = each <= 8 ? 1 : each <= 16 ? 2 : 4;
+    nt = std::min(nt, most_groups(a->cache->head_dim));
+    DeviceGuard guard(ctx->device);
+    const vx_status ls = launch(a->cache, nt, a->grid[nt], ctx->stream, p);
+    if (ls != VX_OK) return ls;
+    kv_merge_kernel<<<dim3(p.r.rows, (unsigned)a->heads), 128, 0, ctx->stream>>>(p, 8 * nt);
+    VX_CUDA(cudaGetLastError());
+    ctx->launches += 2;
+    return VX_OK;
+}
+
+}  // extern "C"
