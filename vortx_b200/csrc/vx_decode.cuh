@@ -22,10 +22,16 @@ using sm100::smem_addr;
 
 // D = A B + D, A 16 x 16 (rows of codes), B 16 x 8, f16 in, f32 sums.
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// D = A B.
+__device__ __forceinline__ void mma_f16_new(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
 }
 
 // Four 8 x 16-byte matrices; lane l passes the row address of row l % 8 of matrix l / 8 and receives, of each matrix,
@@ -101,6 +107,25 @@ __device__ __forceinline__ float lift(float largest) {
     return __uint_as_float((uint32_t)(min(126, max(-113, want)) + 127) << 23);
 }
 
+// 2^v to 2^-22 relative; results below the smallest normal number are 0.
+__device__ __forceinline__ float ex2(float v) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+
+// Whether this block is the last of `count` that get here with this counter; what the others wrote before is then
+// visible.  The counter is zero again afterwards.
+__device__ __forceinline__ bool last_of(uint32_t* counter, uint32_t count, uint32_t* shared) {
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) *shared = atomicInc(counter, count - 1);
+    __syncthreads();
+    const bool last = *shared == count - 1;
+    if (last) __threadfence();
+    return last;
+}
+
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
@@ -166,10 +191,11 @@ __host__ __device__ constexpr uint32_t k_word(bool four_bit, uint32_t block, uin
 }
 __host__ __device__ constexpr uint32_t k_scale(uint32_t block, uint32_t token) { return block * 64 + ((token % 8) * 4 + token / 8) * 2; }
 // Values, codes: token = t + 4 i + 16 s; lane 4 j + t of a warp takes values 4 j .. 4 j + 3 of its tokens.
-// Q8_0: 4 bytes (codes + 128); Q4_0: 2 bytes (four nibbles, code + 8).
+// Q4_0: two bytes (four nibbles, code + 8) of a token; Q8_0: value 4 j is this byte (code + 128), the next three follow four
+// bytes apart, so a word has one value of four tokens.
 __host__ __device__ constexpr uint32_t v_word(bool four_bit, uint32_t block, uint32_t token, uint32_t j) {
     const uint32_t t = token % 4, i = (token / 4) % 4, s = token / 16;
-    return four_bit ? block * 512 + (j * 4 + t) * 16 + s * 8 + i * 2 : block * 1024 + s * 512 + (j * 4 + t) * 16 + i * 4;
+    return four_bit ? block * 512 + (j * 4 + t) * 16 + s * 8 + i * 2 : block * 1024 + s * 512 + (j * 4 + t) * 16 + i;
 }
 __host__ __device__ constexpr uint32_t v_scale(uint32_t block, uint32_t token) {
     return block * 64 + ((token % 4) * 8 + (token / 16) * 4 + (token / 4) % 4) * 2;
@@ -239,6 +265,29 @@ struct vx_kv_cache {
 };
 
 namespace vx {
+// Launches a kernel whose blocks may be scheduled while the stream's previous kernel ends (it calls pdl_wait first).
+template <class P>
+cudaError_t launch_after(void (*kernel)(P), dim3 grid, uint32_t threads, uint32_t smem, cudaStream_t stream, const P& p, dim3 cluster = dim3(1)) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2]{};
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = 1;
+    if (cluster.x * cluster.y * cluster.z > 1) {
+        attr[1].id = cudaLaunchAttributeClusterDimension;
+        attr[1].val.clusterDim.x = cluster.x;
+        attr[1].val.clusterDim.y = cluster.y;
+        attr[1].val.clusterDim.z = cluster.z;
+        cfg.numAttrs = 2;
+    }
+    cfg.attrs = attr;
+    return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
 // The host's checks of a vx_kv_rows and what the kernels get of it.
 vx_status kv_rows_check(const char* who, const vx_kv_rows* rows, KvRows* out);
 }  // namespace vx

@@ -1,4 +1,4 @@
-// Attention over the quantised cache: entry points and the kernel that joins the parts of a sequence that was split.
+// Attention over the quantised cache: entry points.
 #include <algorithm>
 #include <memory>
 #include <new>
@@ -12,80 +12,10 @@ struct vx_kv_attention {
     size_t heads = 0, max_seqs = 0;
     uint32_t grid[5] = {};  // thread blocks by groups of eight rows (1, 2, 4), 0 where there is no such kernel
     uint8_t* workspace = nullptr;
-    size_t ml_offset = 0, plan_offset = 0;
+    size_t ml_offset = 0, counters_offset = 0;
 };
 
 namespace vx {
-
-// One block per row and query head: the maximum over the parts, then the parts' outputs in turn over four warps.
-// A few parts of D floats each: bound by the latency of two dependent loads.
-__global__ void __launch_bounds__(128) kv_merge_kernel(const AttnParams p, uint32_t R) {
-    __shared__ __align__(16) float parts[3][256];
-    const uint32_t row = blockIdx.x, hq = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, dim = p.g.blocks * 32;
-    const uint32_t seq = warp_search(p.r.seqs, row, [&](uint32_t s) { return (uint32_t)max(p.r.begin[s], 0); });
-    const KvSeq sq = kv_seq(p.r, p.g, seq);
-    if (row < sq.row0 || row - sq.row0 >= sq.n || sq.end == 0) return;
-    const uint64_t total = p.plan[0], blocks = p.plan[1];
-    const uint32_t tiles = (sq.end + kTileTokens - 1) / kTileTokens;
-    const uint32_t groups = (uint32_t)(((uint64_t)sq.n * p.group + R - 1) / R);
-    const uint32_t head = hq / p.group, rr = (row - sq.row0) * p.group + (hq - head * p.group);
-    const uint64_t first = p.plan[2 + seq] + ((uint64_t)head * groups + rr / R) * tiles;
-    const uint64_t c0 = share_of(total, blocks, first), c1 = share_of(total, blocks, first + tiles - 1);
-    if (c0 == c1) return;
-    auto slot = [&](uint64_t c) { return (size_t)c * 2 + (c == c0 && share_begin(total, blocks, c) <= first ? 1 : 0); };
-    float m = -INFINITY, l = 0.0f;
-    for (uint64_t c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, p.part_ml[slot(c) * R + rr % R].x);
-    m = warp_max(m);
-    auto weight = [&](float x) { return x == -INFINITY ? 1.0f : exp2f(x - m); };  // a part that saw nothing is zeros
-    for (uint64_t c = c0 + lane; c <= c1; c += 32) {
-        const float2 f = p.part_ml[slot(c) * R + rr % R];
-        l += f.y * weight(f.x);
-    }
-    l = warp_add(l);
-    const float n = l == 0.0f ? 0.0f : 1.0f / l;
-    float4 o[2] = {make_float4(0.0f, 0.0f, 0.0f, 0.0f), make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
-#pragma unroll 4
-    for (uint64_t c = c0 + warp; c <= c1; c += 4) {
-        const size_t at = slot(c) * R + rr % R;
-        const float w = weight(p.part_ml[at].x);
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            const uint32_t col = lane * 4 + x * 128;
-            if (col < dim) {
-                const float4 f = *reinterpret_cast<const float4*>(p.part_o + at * dim + col);
-                o[x].x = fmaf(w, f.x, o[x].x);
-                o[x].y = fmaf(w, f.y, o[x].y);
-                o[x].z = fmaf(w, f.z, o[x].z);
-                o[x].w = fmaf(w, f.w, o[x].w);
-            }
-        }
-    }
-    if (warp > 0) {
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-            if (lane * 4 + x * 128 < dim) *reinterpret_cast<float4*>(&parts[warp - 1][lane * 4 + x * 128]) = o[x];
-    }
-    __syncthreads();
-    if (warp > 0) return;
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-        const uint32_t col = lane * 4 + x * 128;
-        if (col >= dim) continue;
-#pragma unroll
-        for (int w = 0; w < 3; ++w) {
-            const float4 f = *reinterpret_cast<const float4*>(&parts[w][col]);
-            o[x].x += f.x;
-            o[x].y += f.y;
-            o[x].z += f.z;
-            o[x].w += f.w;
-        }
-        float* dst = p.out + (size_t)row * p.out_stride + (size_t)hq * dim + col;
-        dst[0] = o[x].x * n;
-        dst[1] = o[x].y * n;
-        dst[2] = o[x].z * n;
-        dst[3] = o[x].w * n;
-    }
-}
 
 extern template vx_status kv_attention_setup<false, false>(uint32_t, uint32_t, int*, uint32_t*);
 extern template vx_status kv_attention_setup<false, true>(uint32_t, uint32_t, int*, uint32_t*);
@@ -141,7 +71,7 @@ vx_status vx_kv_attention_create(vx_context* ctx, const vx_kv_cache* cache, size
     a->cache = cache;
     a->heads = heads;
     a->max_seqs = max_seqs;
-    size_t rows = 0;
+    size_t rows = 0, blocks = 0;
     for (uint32_t nt = 1; nt <= most_groups(cache->head_dim); nt *= 2) {
         int per_sm = 0;
         uint32_t smem = 0;
@@ -150,14 +80,21 @@ vx_status vx_kv_attention_create(vx_context* ctx, const vx_kv_cache* cache, size
         VX_REQUIRE(per_sm > 0, VX_ERR_UNSUPPORTED, "vx_kv_attention_create: the kernel does not fit an SM");
         a->grid[nt] = (uint32_t)(ctx->sm_count * per_sm);
         rows = std::max(rows, (size_t)2 * a->grid[nt] * 8 * nt);
+        blocks = std::max(blocks, (size_t)a->grid[nt]);
     }
     a->ml_offset = rows * cache->head_dim * sizeof(float);
-    a->plan_offset = a->ml_offset + rows * sizeof(float2);
-    const size_t bytes = a->plan_offset + (2 + max_seqs) * sizeof(uint64_t);
-    const cudaError_t e = device_malloc(ctx, reinterpret_cast<void**>(&a->workspace), bytes);
+    a->counters_offset = a->ml_offset + rows * sizeof(float2);
+    const size_t bytes = a->counters_offset + blocks * sizeof(uint32_t);
+    cudaError_t e = device_malloc(ctx, reinterpret_cast<void**>(&a->workspace), bytes);
     if (e != cudaSuccess) {
         (void)cudaGetLastError();
         return fail(VX_ERR_OUT_OF_MEMORY, "allocating %zu bytes of attention workspace failed: %s", bytes, cudaGetErrorString(e));
+    }
+    e = cudaMemsetAsync(a->workspace + a->counters_offset, 0, blocks * sizeof(uint32_t), ctx->stream);
+    if (e != cudaSuccess) {
+        (void)cudaGetLastError();
+        cudaFree(a->workspace);
+        return fail(VX_ERR_CUDA, "clearing the attention counters failed: %s", cudaGetErrorString(e));
     }
     *out = a.release();
     return VX_OK;
@@ -201,7 +138,7 @@ vx_status vx_kv_attention_run(vx_context* ctx, const vx_kv_attention* a, const v
     p.mask_words = (uint32_t)mask_words;
     p.part_o = reinterpret_cast<float*>(a->workspace);
     p.part_ml = reinterpret_cast<float2*>(a->workspace + a->ml_offset);
-    p.plan = reinterpret_cast<uint64_t*>(a->workspace + a->plan_offset);
+    p.counters = reinterpret_cast<uint32_t*>(a->workspace + a->counters_offset);
     // Rows of a sequence that share a head of keys, as the host can know them: the average.
     const uint64_t each = ((uint64_t)p.r.rows + p.r.seqs - 1) / p.r.seqs * group;
     uint32_t nt = each <= 8 ? 1 : each <= 16 ? 2 : 4;
@@ -209,9 +146,7 @@ vx_status vx_kv_attention_run(vx_context* ctx, const vx_kv_attention* a, const v
     DeviceGuard guard(ctx->device);
     const vx_status ls = launch(a->cache, nt, a->grid[nt], ctx->stream, p);
     if (ls != VX_OK) return ls;
-    kv_merge_kernel<<<dim3(p.r.rows, (unsigned)a->heads), 128, 0, ctx->stream>>>(p, 8 * nt);
-    VX_CUDA(cudaGetLastError());
-    ctx->launches += 2;
+    ctx->launches++;
     return VX_OK;
 }
 

@@ -8,19 +8,25 @@
 // cache, no synchronisation between tiles), two tiles in flight per warp (cp.async, a record is contiguous).
 //   scores   per block of 32 values: sum of code * (q hi + q lo) on the tensor cores, times the block's scale, in f32
 //   softmax  base 2 (log2 e is multiplied into q), running maximum per row, weights p <= 1
-//   output   the value blocks' scales are per token, so they go into the weights: w = p * d * c with c a power of two
-//            that keeps the largest |d| c in [2^14, 2^15), w split into two f16 parts, times the codes
-// The runs are equal shares of all tiles of all (sequence, head, group of rows): whatever the lengths, every block of
-// the grid has the same number of tiles.  A share that covers the tiles of a (sequence, head, rows) only in part leaves maximum, sum
-// and unnormalised output in the workspace, at most two per block, and kv_merge_kernel joins them in a fixed order.
+//   output   the value blocks' scales d are per token, so they go into the weights.  With 2^e the power of two below a
+//            token's largest |d|, p 2^e is lifted so that the tile's largest lies in [2^12, 2^13) and split into two f16
+//            parts, once per tile; the f16 scales become d 2^(1 - e), in [2, 4) for the largest, exact; and the two parts of
+//            the product, hi = p hi * d and lo = p lo * d + (p hi * d - hi), are three f16 operations per pair of
+//            tokens and block (the difference is exact).  A token of no weight, however large, costs the others nothing
+// The runs are shares of all tiles of all (sequence, head, group of rows), see Schedule.  A share that covers the tiles of a (sequence, head, rows) only in part leaves
+// maximum, sum and unnormalised output in the workspace, at most two per block, and the last block to finish a part
+// joins them all, in their order.
 #pragma once
+
+#include <type_traits>
 
 #include "vx_decode.cuh"
 
 namespace vx {
 
 constexpr int kAttnWarps = 4;
-constexpr uint32_t kAttnMinTiles = kAttnWarps;  // tiles per block below which fewer blocks work
+constexpr uint32_t kAttnMinTiles = 4;   // tiles per block below which fewer blocks work
+constexpr uint32_t kAttnJoin = 32;       // parts whose weights are in shared memory at a time
 
 struct AttnParams {
     KvGeometry g;
@@ -34,16 +40,28 @@ struct AttnParams {
     uint32_t mask_words;
     float* part_o;           // [2 * grid][8 NT][D]
     float2* part_ml;         // [2 * grid][8 NT] maximum (base 2), sum
-    uint64_t* plan;          // [0] all tiles, [1] blocks that work, [2 + s] tiles before sequence s
+    uint32_t* counters;      // [grid] parts that are done, of what begins in this block; zero between calls
 };
 
-// Tiles of sequence s over all its (head, group of rows).
-__device__ __forceinline__ uint64_t seq_work(const KvSeq& q, const KvGeometry& g, uint32_t group, uint32_t rows_per_item) {
-    const uint64_t items = (uint64_t)g.heads * (((uint64_t)q.n * group + rows_per_item - 1) / rows_per_item);
-    return items * ((q.end + kTileTokens - 1) / kTileTokens);
+// The (head, group of rows) of a sequence, and its tiles.
+__device__ __forceinline__ uint64_t seq_items(const KvSeq& q, const KvGeometry& g, uint32_t group, uint32_t rows_per_item) {
+    return (uint64_t)g.heads * (((uint64_t)q.n * group + rows_per_item - 1) / rows_per_item);
 }
-__device__ __forceinline__ uint64_t share_begin(uint64_t total, uint64_t blocks, uint64_t c) { return c * total / blocks; }
-__device__ __forceinline__ uint64_t share_of(uint64_t total, uint64_t blocks, uint64_t x) { return ((x + 1) * blocks - 1) / total; }
+__device__ __forceinline__ uint32_t seq_tiles_of(const KvSeq& q) { return (q.end + kTileTokens - 1) / kTileTokens; }
+// a / b; most often both fit 32 bits, and a 64-bit division is a call.
+__device__ __forceinline__ uint64_t quotient(uint64_t a, uint64_t b) {
+    return ((a | b) >> 32) == 0 ? (uint32_t)a / (uint32_t)b : a / b;
+}
+// Shares of `total` tiles: the first `more` blocks have `each` + 1, the others `each`.
+struct Shares {
+    uint64_t each, more;
+    __device__ Shares(uint64_t total, uint64_t blocks) : each(quotient(total, blocks)), more(total - each * blocks) {}
+    __device__ uint64_t begin(uint64_t block) const { return block * each + (block < more ? block : more); }
+    __device__ uint32_t block_of(uint64_t tile) const {  // every block has a tile
+        const uint64_t large = more * (each + 1);
+        return (uint32_t)(tile < large ? quotient(tile, each + 1) : more + quotient(tile - large, each));
+    }
+};
 
 template <bool K4, bool V4, int NB, int NT>
 struct AttnShape {
@@ -53,8 +71,11 @@ struct AttnShape {
     static constexpr uint32_t joined = 2 * rows * dim * 4;  // outputs of two warps, after the loop
     static constexpr uint32_t tiles = ring > joined ? ring : joined;
     static constexpr uint32_t q_bytes = NB * NT * 2 * 512;
-    static constexpr uint32_t p_bytes = kAttnWarps * rows * 32 * 4;
-    static constexpr uint32_t smem = tiles + q_bytes + p_bytes + rows * 4 + kAttnWarps * rows * 8 + 64;
+    // the weights' transposition buffer lies over the keys' codes, which have been read by then, where it fits
+    static constexpr uint32_t p_warp = rows * 32 * 4;
+    static constexpr bool p_over = p_warp <= kv_code_bytes(K4, NB);
+    static constexpr uint32_t p_bytes = p_over ? 0 : kAttnWarps * p_warp;
+    static constexpr uint32_t smem = tiles + q_bytes + p_bytes + rows * 4 + kAttnWarps * rows * 8 + 128;
 };
 
 // 16-byte slot of the weights' transposition buffer: rows of eight slots, spread so that the writes (one float per
@@ -63,33 +84,71 @@ __device__ __forceinline__ uint32_t p_slot(uint32_t row, uint32_t slot) { return
 
 template <bool K4, bool V4, int NB, int NT>
 __global__ void __launch_bounds__(kAttnWarps * 32, NT == 1 ? (NB <= 4 ? 3 : 2) : (NT * NB <= 8 ? 3 : 2))
-kv_attention_kernel(const AttnParams p) {
+kv_attention_kernel(AttnParams p) {
     using Shape = AttnShape<K4, V4, NB, NT>;
     constexpr uint32_t R = Shape::rows;
     constexpr float kNone = -INFINITY;
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t* qf = smem + Shape::tiles;
     float* pbuf = reinterpret_cast<float*>(qf + Shape::q_bytes);
-    float* inv_lift = pbuf + kAttnWarps * R * 32;
+    float* inv_lift = pbuf + Shape::p_bytes / 4;
     float2* ml = reinterpret_cast<float2*>(inv_lift + R);
     uint64_t* shared64 = reinterpret_cast<uint64_t*>(ml + kAttnWarps * R);
 
+    pdl_wait();
+    pdl_launch();
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
 
-    // ---- this block's share -----------------------------------------------------------------------------------
-    uint32_t seq;
-    uint64_t pos, hi;   // position within the sequence's tiles, end of the share (in the same count)
+    // ---- this block's share: of units of `step` tiles of an item (sequence, head, group of rows) -------------------
+    // One unit per block where that leaves the blocks nearly equal (few items next to the grid), else the same number
+    // of tiles, whichever items they are of.
+    uint32_t seq, step = 1;
+    uint64_t pos, hi;      // units of the sequence: where the block is, where its share ends
+    uint64_t origin;       // units before the sequence
+    Shares shares(0, 1);
     {
         const uint32_t per = (p.r.seqs + kAttnWarps * 32 - 1) / (kAttnWarps * 32);
         const uint32_t s0 = min(p.r.seqs, tid * per), s1 = min(p.r.seqs, s0 + per);
+        uint64_t tiles = 0, items = 0;
+        for (uint32_t s = s0; s < s1; ++s) {
+            const KvSeq q = kv_seq(p.r, p.g, s);
+            const uint64_t i = seq_items(q, p.g, p.group, R);
+            items += i;
+            tiles += i * seq_tiles_of(q);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o /= 2) {
+            tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
+            items += __shfl_xor_sync(0xffffffffu, items, o);
+        }
+        if (lane == 0) {
+            shared64[warp] = tiles;
+            shared64[kAttnWarps + warp] = items;
+        }
+        __syncthreads();
+        tiles = items = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < kAttnWarps; ++w) {
+            tiles += shared64[w];
+            items += shared64[kAttnWarps + w];
+        }
+        if (tiles == 0) return;
+        const uint64_t even = quotient(tiles + gridDim.x - 1, gridDim.x);
+        const uint64_t apart = items < gridDim.x ? quotient(tiles, gridDim.x - items) + 1 : ~0ull;  // sum ceil(tiles / apart) <= grid
+        if (apart <= even + even / 4 + kAttnMinTiles) step = max((uint32_t)apart, kAttnMinTiles);
+        auto units_of = [&](uint32_t s) {
+            const KvSeq q = kv_seq(p.r, p.g, s);
+            return seq_items(q, p.g, p.group, R) * ((seq_tiles_of(q) + step - 1) / step);
+        };
         uint64_t mine = 0;
-        for (uint32_t s = s0; s < s1; ++s) mine += seq_work(kv_seq(p.r, p.g, s), p.g, p.group, R);
+        for (uint32_t s = s0; s < s1; ++s) mine += units_of(s);
         uint64_t before = mine;
 #pragma unroll
         for (int o = 1; o < 32; o *= 2) {
             const uint64_t v = __shfl_up_sync(0xffffffffu, before, o);
             if (lane >= (uint32_t)o) before += v;
         }
+        __syncthreads();
         if (lane == 31) shared64[warp] = before;
         __syncthreads();
         uint64_t total = 0;
@@ -98,29 +157,18 @@ kv_attention_kernel(const AttnParams p) {
             if (w < warp) before += shared64[w];
             total += shared64[w];
         }
-        uint64_t blocks = (total + kAttnMinTiles - 1) / kAttnMinTiles;
+        uint64_t blocks = step > 1 ? total : quotient(total + kAttnMinTiles - 1, kAttnMinTiles);
         if (blocks > gridDim.x) blocks = gridDim.x;
-        if (blocks < 1) blocks = 1;
-        if (blockIdx.x == 0) {  // for the kernel that joins the parts
-            if (tid == 0) {
-                p.plan[0] = total;
-                p.plan[1] = blocks;
-            }
-            uint64_t at = before;
-            for (uint32_t s = s0; s < s1; ++s) {
-                p.plan[2 + s] = at;
-                at += seq_work(kv_seq(p.r, p.g, s), p.g, p.group, R);
-            }
-        }
-        if (blockIdx.x >= blocks || total == 0) return;
-        const uint64_t lo = share_begin(total, blocks, blockIdx.x);
-        hi = share_begin(total, blocks, blockIdx.x + 1);
+        if (blockIdx.x >= blocks) return;
+        shares = Shares(total, blocks);
+        const uint64_t lo = shares.begin(blockIdx.x);
+        hi = shares.begin(blockIdx.x + 1);
         __syncthreads();
         if (before <= lo && lo < before + mine) {  // one thread of the block
             uint64_t at = before;
             uint32_t s = s0;
             for (;; ++s) {
-                const uint64_t w = seq_work(kv_seq(p.r, p.g, s), p.g, p.group, R);
+                const uint64_t w = units_of(s);
                 if (lo < at + w) break;
                 at += w;
             }
@@ -129,37 +177,47 @@ kv_attention_kernel(const AttnParams p) {
         }
         __syncthreads();
         seq = (uint32_t)shared64[0];
-        pos = lo - shared64[1];
-        hi -= shared64[1];
+        origin = shared64[1];
+        pos = lo - origin;
+        hi -= origin;
     }
 
     const uint32_t ring = smem_addr(smem) + warp * 2 * Shape::record;
-    const uint32_t pw = smem_addr(pbuf) + warp * R * 32 * 4;
-    float* pwf = pbuf + warp * R * 32;
 
     while (pos < hi) {
         const KvSeq sq = kv_seq(p.r, p.g, seq);
-        const uint64_t work = seq_work(sq, p.g, p.group, R);
+        const uint32_t seq_tiles = seq_tiles_of(sq), units = (seq_tiles + step - 1) / step;
+        const uint64_t work = seq_items(sq, p.g, p.group, R) * units;
         if (pos >= work) {  // on to the next sequence
             pos -= work;
             hi -= work;
+            origin += work;
             ++seq;
             continue;
         }
-        const uint32_t seq_tiles = (sq.end + kTileTokens - 1) / kTileTokens;
         const uint32_t groups = (uint32_t)(((uint64_t)sq.n * p.group + R - 1) / R);
-        const uint32_t item = (uint32_t)(pos / seq_tiles), tile0 = (uint32_t)(pos - (uint64_t)item * seq_tiles);
+        const uint32_t item = (uint32_t)quotient(pos, units), unit0 = (uint32_t)(pos - (uint64_t)item * units);
         const uint32_t head = item / groups, rt = item - head * groups;
-        uint32_t tile1 = seq_tiles;
-        if (hi - pos < seq_tiles - tile0) tile1 = tile0 + (uint32_t)(hi - pos);
-        pos += tile1 - tile0;
+        const uint32_t count = hi - pos < units - unit0 ? (uint32_t)(hi - pos) : units - unit0;
+        const uint32_t tile0 = unit0 * step, tile1 = min(seq_tiles, (unit0 + count) * step);
+        const bool whole = count == units;
+        pos += count;
         const uint32_t row_first = rt * R, row_count = min(R, sq.n * p.group - row_first);
         // with no mask, nothing is attended to behind the last row's own token
         uint32_t last_tile = tile1;
         if (p.mask == nullptr) last_tile = min(last_tile, (sq.start + (row_first + row_count - 1) / p.group) / kTileTokens + 1);
 
-        // ---- the first two tiles of every warp, while q is laid out -----------------------------------------------
+        // ---- q's rows (2 NT a warp) and the first two tiles of every warp come in together -----------------------------
+        float qv[2 * NT][NB];
+#pragma unroll
+        for (int x = 0; x < 2 * NT; ++x) {
+            const uint32_t r = warp + x * kAttnWarps, rr = row_first + r, i = rr / p.group, hq = head * p.group + (rr - i * p.group);
+            const float* src = p.q + (size_t)(sq.row0 + i) * p.q_stride + (size_t)hq * Shape::dim + lane;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) qv[x][b] = r < row_count ? src[b * 32] : 0.0f;
+        }
         const uint32_t mine0 = tile0 + warp;
+        uint32_t have = 0;           // bit k & 1: tile number k has a page
         uint64_t ahead = 0;          // record of this lane's tile of the next 32 of this warp, 0 if it has no page
         auto look_ahead = [&](uint32_t tile) {
             const uint32_t x = tile + lane * kAttnWarps;
@@ -175,30 +233,29 @@ kv_attention_kernel(const AttnParams p) {
                     if (o + 512 <= Shape::record || o + lane * 16 < Shape::record) cp_async16(dst + o, from + o);
             }
             cp_async_commit();
-            return src != 0;
+            have = src ? have | 1u << (k & 1) : have & ~(1u << (k & 1));
         };
         const uint32_t mine = mine0 < last_tile ? (last_tile - mine0 + kAttnWarps - 1) / kAttnWarps : 0;
         look_ahead(mine0);
-        bool have[2];
-        have[0] = fetch(0);
-        have[1] = fetch(1);
+        fetch(0);
+        fetch(1);
 
         // ---- q: scaled, lifted by a power of two per row, split into two f16 parts in B-operand order ----------------
-        for (uint32_t r = warp; r < R; r += kAttnWarps) {
-            float v[NB], top = 0.0f;
-            const uint32_t rr = row_first + r, i = rr / p.group, hq = head * p.group + (rr - i * p.group);
-            const float* src = p.q + (size_t)(sq.row0 + i) * p.q_stride + (size_t)hq * Shape::dim;
+#pragma unroll
+        for (int x = 0; x < 2 * NT; ++x) {
+            const uint32_t r = warp + x * kAttnWarps;
+            float most = 0.0f;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                v[b] = r < row_count ? src[b * 32 + lane] * p.scale_log2 : 0.0f;
-                top = fmaxf(top, fabsf(v[b]));
+                qv[x][b] *= p.scale_log2;
+                most = fmaxf(most, fabsf(qv[x][b]));
             }
-            const float up = lift(warp_max(top));
+            const float up = lift(warp_max(most));
             if (lane == 0) inv_lift[r] = 1.0f / up;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                const float x = v[b] * up;
-                const __half h = __float2half_rn(x), l = __float2half_rn(x - __half2float(h));
+                const float v = qv[x][b] * up;
+                const __half h = __float2half_rn(v), l = __float2half_rn(v - __half2float(h));
                 uint8_t* dst = qf + ((b * NT + r / 8) * 2) * 512 + ((r % 8) * 4 + frag_lane(lane)) * 16 + frag_half(K4, lane) * 2;
                 *reinterpret_cast<__half*>(dst) = h;
                 *reinterpret_cast<__half*>(dst + 512) = l;
@@ -213,7 +270,7 @@ kv_attention_kernel(const AttnParams p) {
             inv[n][1] = inv_lift[n * 8 + 2 * t + 1];
         }
 
-        float top[NT][2], sum[NT][2], acc[2 * NB][NT][4], lifted = __uint_as_float((28u + 127u) << 23);
+        float top[NT][2], sum[NT][2], acc[2 * NB][NT][4], unit = 1.0f;  // acc counts 1 / (2 unit)
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             top[n][0] = top[n][1] = kNone;
@@ -228,8 +285,36 @@ kv_attention_kernel(const AttnParams p) {
             const uint32_t tile = mine0 + k * kAttnWarps;
             cp_async_wait<1>();
             __syncwarp();
-            if (have[k & 1]) {
-                const uint32_t rec = ring + (k & 1) * Shape::record;
+            if (have >> (k & 1) & 1) {
+                const uint32_t rec = ring + (k & 1) * Shape::record, base = tile * kTileTokens;
+                float* pwf = Shape::p_over ? reinterpret_cast<float*>(smem + (warp * 2 + (k & 1)) * Shape::record) : pbuf + warp * R * 32;
+                const uint32_t pw = smem_addr(pwf);
+                // ---- which of the tile's tokens each of the thread's rows attends to, if not to all -------------------------
+                const bool masked = base + kTileTokens > sq.start;
+                uint32_t may[NT][2];
+                if (masked) {
+                    const uint32_t before = base < sq.start ? (1u << (sq.start - base)) - 1u : 0u;  // context
+                    const uint32_t there = sq.end - base >= 32 ? 0xffffffffu : (1u << (sq.end - base)) - 1u;
+                    const uint32_t j0 = base < sq.start ? 0u : base - sq.start, up = base < sq.start ? sq.start - base : 0u;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const uint32_t rr = row_first + n * 8 + 2 * t + e, i = rr / p.group;
+                            uint32_t bits = 0;  // of the call's tokens j0 ..
+                            if (rr < sq.n * p.group) {
+                                if (p.mask == nullptr) {
+                                    bits = i < j0 ? 0u : i - j0 >= 31 ? 0xffffffffu : (2u << (i - j0)) - 1u;
+                                } else {
+                                    const uint32_t* row = p.mask + (size_t)(sq.row0 + i) * p.mask_words;
+                                    const uint32_t w = j0 / 32;
+                                    const uint32_t lo_ = w < p.mask_words ? row[w] : 0u, hi_ = w + 1 < p.mask_words ? row[w + 1] : 0u;
+                                    bits = __funnelshift_r(lo_, hi_, j0 % 32);
+                                }
+                            }
+                            may[n][e] = (before | bits << up) & there;
+                        }
+                }
                 // ---- scores of 32 tokens: s[m][n] = tokens 16 m + g (c 0, 1) and 16 m + g + 8 (c 2, 3), rows 8 n + 2 t, + 1
                 float s[2][NT][4];
 #pragma unroll
@@ -261,8 +346,8 @@ kv_attention_kernel(const AttnParams p) {
                         const uint4 qh = lds128(qs + ((b * NT + n) * 2) * 512), ql = lds128(qs + ((b * NT + n) * 2 + 1) * 512);
 #pragma unroll
                         for (int m = 0; m < 2; ++m) {
-                            float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                            mma_f16(c, a[m][0], ql.x, ql.y);
+                            float c[4];
+                            mma_f16_new(c, a[m][0], ql.x, ql.y);
                             mma_f16(c, a[m][1], ql.z, ql.w);
                             mma_f16(c, a[m][0], qh.x, qh.y);
                             mma_f16(c, a[m][1], qh.z, qh.w);
@@ -274,33 +359,25 @@ kv_attention_kernel(const AttnParams p) {
                         }
                     }
                 }
-                const uint32_t base = tile * kTileTokens;
-                const bool masked = base + kTileTokens > sq.start;
 #pragma unroll
                 for (int m = 0; m < 2; ++m)
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            s[m][n][c] *= inv[n][c & 1];
-                            if (masked) {
-                                const uint32_t token = base + m * 16 + (c >> 1) * 8 + g;
-                                if (token >= sq.start) {
-                                    const uint32_t j = token - sq.start, rr = row_first + n * 8 + 2 * t + (c & 1);
-                                    bool may = token < sq.end && rr < sq.n * p.group;
-                                    if (may) {
-                                        const uint32_t i = rr / p.group;
-                                        if (p.mask == nullptr) may = j <= i;
-                                        else may = j / 32 < p.mask_words &&
-                                                   ((p.mask[(size_t)(sq.row0 + i) * p.mask_words + j / 32] >> (j & 31)) & 1u);
-                                    }
-                                    if (!may) s[m][n][c] = kNone;
-                                }
-                            }
-                        }
+                        for (int c = 0; c < 4; ++c) s[m][n][c] *= inv[n][c & 1];
+                if (masked) {
+                    __syncwarp();  // keeps this a branch that other tiles jump over
+#pragma unroll
+                    for (int m = 0; m < 2; ++m)
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int c = 0; c < 4; ++c)
+                                if (!(may[n][c & 1] >> (m * 16 + (c >> 1) * 8 + g) & 1)) s[m][n][c] = kNone;
+                }
+                __syncwarp();  // the keys' codes have been read
                 // ---- running maximum and sum; the weights change sides through shared memory -----------------------------
                 float fall[NT][2];
-                bool rescale = false;
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -310,15 +387,14 @@ kv_attention_kernel(const AttnParams p) {
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
                         const float now = fmaxf(top[n][e], mx), ref = now == kNone ? 0.0f : now;
-                        fall[n][e] = exp2f(top[n][e] - ref);
-                        rescale |= fall[n][e] != 1.0f;
+                        fall[n][e] = ex2(top[n][e] - ref);
                         top[n][e] = now;
                         float add = 0.0f;
 #pragma unroll
                         for (int m = 0; m < 2; ++m)
 #pragma unroll
                             for (int h = 0; h < 2; ++h) {
-                                const float w = exp2f(s[m][n][e + 2 * h] - ref);
+                                const float w = ex2(s[m][n][e + 2 * h] - ref);
                                 add += w;
                                 const uint32_t row = n * 8 + 2 * t + e, lo = g + 8 * h;  // token lo + 16 m
                                 pwf[p_slot(row, (lo & 3) * 2 + m) * 4 + (lo >> 2)] = w;
@@ -329,124 +405,138 @@ kv_attention_kernel(const AttnParams p) {
                 // ---- the value blocks' scales: tokens t + 4 i + 16 s of every lane, and the power of two that they allow
                 const uint32_t vrec = rec + Shape::k_bytes, vscales = vrec + kv_code_bytes(V4, NB) + t * 16;
                 uint4 dv[NB];
-                __half2 big = __float2half2_rn(0.0f);
+                __half2 most[4];
+#pragma unroll
+                for (int x = 0; x < 4; ++x) most[x] = bits_h2(0x04000400u);  // 2^-14: smaller scales keep their own size
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
                     dv[b] = lds128(vscales + b * 64);
-                    if (masked) {  // behind the sequence's end lies whatever the page held before
-                        uint32_t* w = &dv[b].x;
-#pragma unroll
-                        for (int x = 0; x < 8; ++x)
-                            if (base + t + 4 * (x & 3) + 16 * (x >> 2) >= sq.end) w[x / 2] &= x & 1 ? 0x0000ffffu : 0xffff0000u;
-                    }
-                    big = __hmax2(big, __hmax2(__hmax2(__habs2(bits_h2(dv[b].x)), __habs2(bits_h2(dv[b].y))),
-                                               __hmax2(__habs2(bits_h2(dv[b].z)), __habs2(bits_h2(dv[b].w)))));
+                    most[0] = __hmax2(most[0], __habs2(bits_h2(dv[b].x)));  // of NaN and a number, the number
+                    most[1] = __hmax2(most[1], __habs2(bits_h2(dv[b].y)));
+                    most[2] = __hmax2(most[2], __habs2(bits_h2(dv[b].z)));
+                    most[3] = __hmax2(most[3], __habs2(bits_h2(dv[b].w)));
                 }
-                float largest = fmaxf(__low2float(big), __high2float(big));
-                largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
-                largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
-                if (largest > 0.0f) {
-                    const float up = fminf(lift(largest), lifted);
-                    if (up < lifted) {
-                        const float ratio = up / lifted;  // powers of two
-                        rescale = true;
-                        lifted = up;
+                __half2 back[4];  // 2^(1 - e)
+                float pe[NT][8], largest = 0.0f;
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) {
-                            fall[n][0] *= ratio;
-                            fall[n][1] *= ratio;
-                        }
-                    }
+                for (int x = 0; x < 4; ++x) {
+                    const uint32_t e = h2_bits(most[x]) & 0x7c007c00u;
+                    back[x] = bits_h2(0x7c007c00u - e);
+                    const float2 f = __half22float2(bits_h2(e));
+                    pe[0][2 * x] = f.x;
+                    pe[0][2 * x + 1] = f.y;
                 }
-                if (__any_sync(0xffffffffu, rescale)) {
 #pragma unroll
-                    for (int d = 0; d < 2 * NB; ++d)
-#pragma unroll
-                        for (int n = 0; n < NT; ++n)
-#pragma unroll
-                            for (int c = 0; c < 4; ++c) acc[d][n][c] *= fall[n][c & 1];
-                }
-                float w8[NT][8];
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
+                for (int n = NT - 1; n >= 0; --n)
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
                         const uint4 f = lds128(pw + p_slot(n * 8 + g, t * 2 + x) * 16);
-                        w8[n][4 * x] = __uint_as_float(f.x);
-                        w8[n][4 * x + 1] = __uint_as_float(f.y);
-                        w8[n][4 * x + 2] = __uint_as_float(f.z);
-                        w8[n][4 * x + 3] = __uint_as_float(f.w);
-                    }
-                // ---- output ------------------------------------------------------------------------------------------
+                        const uint32_t w[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    float d8[8];
-                    const uint32_t raw[4] = {dv[b].x, dv[b].y, dv[b].z, dv[b].w};
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        const float2 f = __half22float2(bits_h2(raw[x]));
-                        d8[2 * x] = f.x * lifted;
-                        d8[2 * x + 1] = f.y * lifted;
-                    }
-                    uint32_t a[2][2][4];  // [k-step][16 values][...]
-                    if (V4) {
-                        const uint4 w4 = lds128(vrec + b * 512 + lane * 16);
-                        const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-#pragma unroll
-                        for (int x = 0; x < 2; ++x)
-#pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                const uint32_t u = w[2 * x + h], v = u >> 8;
-                                a[x][0][2 * h] = f16_of_low_nibbles(u);
-                                a[x][0][2 * h + 1] = f16_of_high_nibbles(u);
-                                a[x][1][2 * h] = f16_of_low_nibbles(v);
-                                a[x][1][2 * h + 1] = f16_of_high_nibbles(v);
-                            }
-                    } else {
-#pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            const uint4 w4 = lds128(vrec + b * 1024 + x * 512 + lane * 16);
-                            const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-#pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                const uint32_t u = __byte_perm(w[2 * h], w[2 * h + 1], 0x5140), v = __byte_perm(w[2 * h], w[2 * h + 1], 0x7362);
-                                a[x][0][2 * h] = f16_of_bytes(u, 0x4140);
-                                a[x][0][2 * h + 1] = f16_of_bytes(u, 0x4342);
-                                a[x][1][2 * h] = f16_of_bytes(v, 0x4140);
-                                a[x][1][2 * h + 1] = f16_of_bytes(v, 0x4342);
-                            }
+                        for (int i = 0; i < 4; ++i) {
+                            pe[n][4 * x + i] = __uint_as_float(w[i]) * pe[0][4 * x + i];
+                            largest = fmaxf(largest, pe[n][4 * x + i]);
                         }
                     }
+                largest = warp_max(largest);
+                if (largest > 0.0f) {
+                    const float now = fminf(lift(largest) * 0.25f, __uint_as_float((40u + 127u) << 23));
+                    const float ratio = now * __uint_as_float(0x7f000000u - __float_as_uint(unit));  // powers of two
+                    unit = now;
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        uint32_t hi_[4], lo_[4];
+                        fall[n][0] *= ratio;
+                        fall[n][1] *= ratio;
+                    }
+                }
+                uint32_t ph[NT][4], pl[NT][4];  // pairs of tokens
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            float u = w8[n][2 * x] * d8[2 * x], v = w8[n][2 * x + 1] * d8[2 * x + 1];
-                            if (masked) {  // a NaN in a masked place stays there
-                                if (w8[n][2 * x] == 0.0f) u = 0.0f;
-                                if (w8[n][2 * x + 1] == 0.0f) v = 0.0f;
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) split_f16(pe[n][2 * x] * unit, pe[n][2 * x + 1] * unit, &ph[n][x], &pl[n][x]);
+                // ---- output ------------------------------------------------------------------------------------------
+                auto output = [&](auto some_masked) {
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+                        const __half2 d[4] = {__hmul2(bits_h2(dv[b].x), back[0]), __hmul2(bits_h2(dv[b].y), back[1]),
+                                              __hmul2(bits_h2(dv[b].z), back[2]), __hmul2(bits_h2(dv[b].w), back[3])};
+                        uint32_t a[2][2][4];  // [k-step][16 values][...]
+                        if (V4) {
+                            const uint4 w4 = lds128(vrec + b * 512 + lane * 16);
+                            const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+                            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                                for (int h = 0; h < 2; ++h) {
+                                    const uint32_t u = w[2 * x + h], v = u >> 8;
+                                    a[x][0][2 * h] = f16_of_low_nibbles(u);
+                                    a[x][0][2 * h + 1] = f16_of_high_nibbles(u);
+                                    a[x][1][2 * h] = f16_of_low_nibbles(v);
+                                    a[x][1][2 * h + 1] = f16_of_high_nibbles(v);
+                                }
+                        } else {
+#pragma unroll
+                            for (int x = 0; x < 2; ++x) {
+                                const uint4 w4 = lds128(vrec + b * 1024 + x * 512 + lane * 16);
+                                a[x][0][0] = f16_of_bytes(w4.x, 0x4140);
+                                a[x][0][1] = f16_of_bytes(w4.y, 0x4140);
+                                a[x][0][2] = f16_of_bytes(w4.x, 0x4342);
+                                a[x][0][3] = f16_of_bytes(w4.y, 0x4342);
+                                a[x][1][0] = f16_of_bytes(w4.z, 0x4140);
+                                a[x][1][1] = f16_of_bytes(w4.w, 0x4140);
+                                a[x][1][2] = f16_of_bytes(w4.z, 0x4342);
+                                a[x][1][3] = f16_of_bytes(w4.w, 0x4342);
                             }
-                            split_f16(u, v, &hi_[x], &lo_[x]);
                         }
 #pragma unroll
-                        for (int x = 0; x < 2; ++x)
+                        for (int n = 0; n < NT; ++n) {
+                            uint32_t hi_[4], lo_[4];
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) {
+                                const __half2 h = __hmul2(bits_h2(ph[n][x]), d[x]);
+                                const __half2 l = __hfma2(bits_h2(pl[n][x]), d[x], __hfma2(bits_h2(ph[n][x]), d[x], __hneg2(h)));
+                                hi_[x] = h2_bits(h);
+                                lo_[x] = h2_bits(l);
+                                if (decltype(some_masked)::value) {  // what is no number in a masked place stays there
+                                    const uint32_t on = (ph[n][x] & 0x7fffu ? 0xffffu : 0u) | (ph[n][x] & 0x7fff0000u ? 0xffff0000u : 0u);
+                                    hi_[x] &= on;
+                                    lo_[x] &= on;
+                                }
+                            }
+                            // The tensor cores cut their f32 sums off instead of rounding them: a tile's sum is taken from
+                            // zero and added to the output here, or the loss would grow with the number of tiles.
+                            float o[2][4];
 #pragma unroll
                             for (int m = 0; m < 2; ++m) {
-                                mma_f16(acc[2 * b + m][n], a[x][m], lo_[2 * x], lo_[2 * x + 1]);
-                                mma_f16(acc[2 * b + m][n], a[x][m], hi_[2 * x], hi_[2 * x + 1]);
+                                mma_f16_new(o[m], a[0][m], lo_[0], lo_[1]);
+                                mma_f16(o[m], a[1][m], lo_[2], lo_[3]);
                             }
+#pragma unroll
+                            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                                for (int m = 0; m < 2; ++m) mma_f16(o[m], a[x][m], hi_[2 * x], hi_[2 * x + 1]);
+#pragma unroll
+                            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                                for (int c = 0; c < 4; ++c) acc[2 * b + m][n][c] = fmaf(acc[2 * b + m][n][c], fall[n][c & 1], o[m][c]);
+                        }
                     }
+                };
+                if (masked) {
+                    __syncwarp();
+                    output(std::true_type());
+                } else {
+                    output(std::false_type());
                 }
             }
             __syncwarp();  // the tile and the weights have been read
             if (((k + 2) & 31) == 0) look_ahead(mine0 + (k + 2) * kAttnWarps);
-            have[k & 1] = fetch(k + 2);
+            fetch(k + 2);
         }
         cp_async_wait<0>();
 
         // ---- the four warps' parts become one ------------------------------------------------------------------------
-        const float down = 1.0f / lifted;
+        const float down = 0.5f / unit;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -467,7 +557,7 @@ kv_attention_kernel(const AttnParams p) {
                 float m = kNone;
 #pragma unroll
                 for (int w = 0; w < kAttnWarps; ++w) m = fmaxf(m, ml[w * R + row].x);
-                const float f = top[n][e] == kNone ? 0.0f : exp2f(top[n][e] - m) * down;
+                const float f = top[n][e] == kNone ? 0.0f : ex2(top[n][e] - m) * down;
 #pragma unroll
                 for (int d = 0; d < 2 * NB; ++d) {
                     acc[d][n][e] *= f;
@@ -501,32 +591,95 @@ kv_attention_kernel(const AttnParams p) {
             store(warp);
         }
         __syncthreads();
-        const bool whole = tile0 == 0 && tile1 == seq_tiles;
         const uint32_t slot = blockIdx.x * 2 + (tile0 == 0 ? 1 : 0);
+        auto put = [&](uint32_t row, uint32_t col, float4 o, float n) {
+            const uint32_t rr = row_first + row, i = rr / p.group;
+            float* dst = p.out + (size_t)(sq.row0 + i) * p.out_stride + (size_t)(head * p.group + (rr - i * p.group)) * Shape::dim + col;
+            dst[0] = o.x * n;
+            dst[1] = o.y * n;
+            dst[2] = o.z * n;
+            dst[3] = o.w * n;
+        };
+        // a part that saw nothing is zeros, and NaN where a NaN was seen; neither is weighted
+        auto weight = [&](float m, float most) { return m == kNone ? 1.0f : ex2(m - most); };
         for (uint32_t x = tid; x < R * Shape::dim / 4; x += kAttnWarps * 32) {
             const uint32_t row = x / (Shape::dim / 4), col = (x % (Shape::dim / 4)) * 4;
             float m = kNone, l = 0.0f;
 #pragma unroll
             for (int w = 0; w < kAttnWarps; ++w) m = fmaxf(m, ml[w * R + row].x);
 #pragma unroll
-            for (int w = 0; w < kAttnWarps; ++w)
-                if (ml[w * R + row].x != kNone || ml[w * R + row].y != 0.0f) l += ml[w * R + row].y * (ml[w * R + row].x == kNone ? 1.0f : exp2f(ml[w * R + row].x - m));
+            for (int w = 0; w < kAttnWarps; ++w) l += ml[w * R + row].y * weight(ml[w * R + row].x, m);
             const float4 u = *reinterpret_cast<const float4*>(joined + row * Shape::dim + col);
             const float4 v = *reinterpret_cast<const float4*>(joined + (R + row) * Shape::dim + col);
-            float4 o = make_float4(u.x + v.x, u.y + v.y, u.z + v.z, u.w + v.w);
+            const float4 o = make_float4(u.x + v.x, u.y + v.y, u.z + v.z, u.w + v.w);
             if (whole) {
-                if (row < row_count) {
-                    const float n = l == 0.0f ? 0.0f : 1.0f / l;
-                    const uint32_t rr = row_first + row, i = rr / p.group;
-                    float* dst = p.out + (size_t)(sq.row0 + i) * p.out_stride + (size_t)(head * p.group + (rr - i * p.group)) * Shape::dim + col;
-                    dst[0] = o.x * n;
-                    dst[1] = o.y * n;
-                    dst[2] = o.z * n;
-                    dst[3] = o.w * n;
-                }
+                if (row < row_count) put(row, col, o, l == 0.0f ? 0.0f : 1.0f / l);
             } else {
                 *reinterpret_cast<float4*>(p.part_o + ((size_t)slot * R + row) * Shape::dim + col) = o;
                 if (col == 0) p.part_ml[(size_t)slot * R + row] = make_float2(m, l);
+            }
+        }
+        if (!whole) {
+            // ---- the parts of the (sequence, head, rows): blocks c0 .. c1, the first one's second slot, the others' first
+            const uint64_t first = origin + (uint64_t)item * units;
+            const uint32_t c0 = shares.block_of(first), parts = shares.block_of(first + units - 1) - c0 + 1;
+            if (last_of(p.counters + c0, parts, reinterpret_cast<uint32_t*>(shared64))) {
+                // shared: per row the maximum and 1 / sum, then the weights of kAttnJoin parts
+                float2* of_row = ml;
+                float* weights = reinterpret_cast<float*>(smem);
+                auto slot_of = [&](uint32_t c) { return (size_t)(c0 + c) * 2 + (c == 0 ? 1 : 0); };
+                constexpr uint32_t kLanes = kAttnWarps * 32 / R;  // that share a row: 4, 8 or 16 neighbours
+                {
+                    const uint32_t row = tid / kLanes, at = tid % kLanes;
+                    float m = kNone, l = 0.0f;
+#pragma unroll 4
+                    for (uint32_t c = at; c < parts; c += kLanes) {
+                        const float2 f = __ldcg(&p.part_ml[slot_of(c) * R + row]);
+                        const float now = fmaxf(m, f.x);
+                        l = (m == kNone ? l : l * ex2(m - now)) + f.y * weight(f.x, now);
+                        m = now;
+                    }
+#pragma unroll
+                    for (uint32_t o = 1; o < kLanes; o *= 2) {
+                        const float m2 = __shfl_xor_sync(0xffffffffu, m, o), l2 = __shfl_xor_sync(0xffffffffu, l, o);
+                        const float now = fmaxf(m, m2);
+                        l = l * weight(m, now) + l2 * weight(m2, now);
+                        m = now;
+                    }
+                    if (at == 0) of_row[row] = make_float2(m, l == 0.0f ? 0.0f : 1.0f / l);
+                }
+                constexpr uint32_t kEach = (R * Shape::dim / 4 + kAttnWarps * 32 - 1) / (kAttnWarps * 32);
+                float4 o[kEach];
+#pragma unroll
+                for (uint32_t x = 0; x < kEach; ++x) o[x] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                for (uint32_t from = 0; from < parts; from += kAttnJoin) {
+                    const uint32_t count = min(kAttnJoin, parts - from);
+                    __syncthreads();
+                    for (uint32_t x = tid; x < count * R; x += kAttnWarps * 32)
+                        weights[x] = weight(__ldcg(&p.part_ml[slot_of(from + x / R) * R + x % R]).x, of_row[x % R].x);
+                    __syncthreads();
+#pragma unroll 8
+                    for (uint32_t c = 0; c < count; ++c) {
+                        const float4* src = reinterpret_cast<const float4*>(p.part_o + slot_of(from + c) * R * Shape::dim);
+#pragma unroll
+                        for (uint32_t x = 0; x < kEach; ++x) {
+                            const uint32_t at = tid + x * kAttnWarps * 32;
+                            if (at < R * Shape::dim / 4) {
+                                const float4 f = __ldcg(src + at);
+                                const float w = weights[c * R + at / (Shape::dim / 4)];
+                                o[x].x = fmaf(w, f.x, o[x].x);
+                                o[x].y = fmaf(w, f.y, o[x].y);
+                                o[x].z = fmaf(w, f.z, o[x].z);
+                                o[x].w = fmaf(w, f.w, o[x].w);
+                            }
+                        }
+                    }
+                }
+#pragma unroll
+                for (uint32_t x = 0; x < kEach; ++x) {
+                    const uint32_t at = tid + x * kAttnWarps * 32, row = at / (Shape::dim / 4);
+                    if (at < R * Shape::dim / 4 && row < row_count) put(row, at % (Shape::dim / 4) * 4, o[x], of_row[row].y);
+                }
             }
         }
         __syncthreads();
@@ -579,8 +732,9 @@ bool attn_pick(uint32_t nb, uint32_t nt, F f) {
     }                                                                                                                     \
     template <>                                                                                                           \
     vx_status kv_attention_launch<K4, V4>(uint32_t nb, uint32_t nt, uint32_t grid, cudaStream_t stream, const AttnParams& p) { \
-        attn_pick<K4, V4>(nb, nt, [&](auto kernel, uint32_t bytes) { kernel<<<grid, kAttnWarps * 32, bytes, stream>>>(p); }); \
-        VX_CUDA(cudaGetLastError());                                                                                      \
+        cudaError_t e = cudaSuccess;                                                                                      \
+        attn_pick<K4, V4>(nb, nt, [&](auto kernel, uint32_t bytes) { e = launch_after(kernel, dim3(grid), kAttnWarps * 32, bytes, stream, p); }); \
+        VX_CUDA(e);                                                                                                       \
         return VX_OK;                                                                                                     \
     }
 

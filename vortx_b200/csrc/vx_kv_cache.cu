@@ -102,7 +102,8 @@ __device__ void append_part(const KvRows& r, const KvGeometry& g, const TileOf& 
             if (FOUR)
                 *reinterpret_cast<uint16_t*>(to + v_word(true, block, token, j)) = (uint16_t)(c[0] | c[1] << 4 | c[2] << 8 | c[3] << 12);
             else
-                *reinterpret_cast<uint32_t*>(to + v_word(false, block, token, j)) = c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;
+#pragma unroll
+                for (int n = 0; n < 4; ++n) to[v_word(false, block, token, j) + 4 * n] = (uint8_t)c[n];
         } else {
             uint32_t w = c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;
             if (FOUR) w |= __shfl_xor_sync(mask, w, 4) << 4;  // byte i of a Q4_0 block: values i and i + 16
@@ -153,11 +154,14 @@ __device__ void read_part(const KvGeometry& g, const TileOf& o, const uint8_t* s
             const uint16_t dh = *reinterpret_cast<const uint16_t*>(src + scales + (VALUES ? v_scale(block, token) : k_scale(block, token)));
             const float d = __half2float(__ushort_as_half(dh));
             uint32_t w;
-            if (VALUES)
-                w = FOUR ? *reinterpret_cast<const uint16_t*>(src + v_word(true, block, token, j))
-                         : *reinterpret_cast<const uint32_t*>(src + v_word(false, block, token, j));
-            else
+            if (VALUES && FOUR) {
+                w = *reinterpret_cast<const uint16_t*>(src + v_word(true, block, token, j));
+            } else if (VALUES) {
+                const uint8_t* at = src + v_word(false, block, token, j);
+                w = at[0] | (uint32_t)at[4] << 8 | (uint32_t)at[8] << 16 | (uint32_t)at[12] << 24;
+            } else {
                 w = *reinterpret_cast<const uint32_t*>(src + k_word(FOUR, block, token, FOUR ? j % 4 : j));
+            }
 #pragma unroll
             for (int n = 0; n < 4; ++n) {
                 int q;

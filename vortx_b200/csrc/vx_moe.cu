@@ -1,16 +1,26 @@
 // A mixture-of-experts layer for a few tokens on block-quantised weights, in three launches:
-//   route   logits = router x (a warp per expert and four tokens), x split into two f16 parts per block of 32
-//           (vx_decode.cuh); the last block to finish picks the experts and lists every expert's tokens
+//   route   logits = router x, in slices of the columns, and x split into two f16 parts per block of 32
 //   inner   silu(gate x) * (up x): a thread block per (expert with tokens, 32 inner rows)
 //   down    y = sum weight * (down h): a thread block per (32 output rows, share of all experts' columns)
-// Bound by the weights' bytes: each is read once per 16 tokens of its expert.  In both products a warp has every
-// eighth 64-byte column chunk of the unit's rows (16-byte cp.async copies, two chunks in flight per warp, no
-// synchronisation between warps until the sums are added up), multiplies it on the tensor cores
-// (m16n8k16: 16 rows of codes, columns 2 i and 2 i + 1 are the two parts of token i, so a thread holds both sums of a
-// (row, token)) and scales every block's sums in f32.
+// Every block of the last two picks the experts from the logits itself (less than one block doing it for all would
+// cost in waiting), and the down kernel does so, and starts to copy its
+// weights, while the inner kernel still runs.
+//
+// Bound by the weights' bytes: each is read once per 8 tokens of its expert.  In both products a warp has every
+// eighth 128-byte column chunk of the unit's rows (16-byte cp.async copies that run ahead over the ends of units and
+// experts, no synchronisation between warps until the sums are added up).  On the tensor cores (m16n8k16) 16 rows of
+// codes are A; columns 2 i and 2 i + 1 of B are the two parts of token i, so a thread holds both sums of a (row, token).
+// A code u (code + 8 or + 128, not negative) is used as the f16 number whose bits it is, u 2^-20 (nibbles moved to bits
+// 4..7) or u 2^-24: a shift and a logic operation, or a byte permutation, per pair and no conversion.  The offset's
+// part of a block's sum, 8 or 128 times the sum of the vector's parts, is taken off with the multiplication that scales
+// the sum.  That makes the partial sums two to three times as large as those of the signed codes, and the tensor cores
+// align products by the exponent field, so the leading zeros of such a number are lost bits (two of 24 for the
+// middle codes): 5e-7 relative to the exact result, 2e-7 with converted codes.  Nibbles left at bits 0..3 lose six more
+// bits: 6e-6.
 #include <algorithm>
 #include <memory>
 #include <new>
+#include <type_traits>
 
 #include "vx_decode.cuh"
 
@@ -20,10 +30,10 @@ using namespace vx;
 
 constexpr uint32_t kMoeWarps = 8, kMoeThreads = kMoeWarps * 32;
 constexpr uint32_t kMaxExperts = 256, kMaxTopK = 16, kMaxTokens = 64;
-constexpr uint32_t kGroup = 16;             // tokens of an expert per pass over its weights
-constexpr uint32_t kPitch = 80;             // a row's 64-byte chunk in shared memory: eight rows meet different banks
-constexpr uint32_t kScaleWords = 3;         // a chunk's scales (2 or 4 halves at any 2-byte offset), as 4-byte words
-constexpr uint32_t kStages = 2;
+constexpr uint32_t kGroup = 8;              // tokens of an expert per pass over its weights: what fits 128 registers
+constexpr uint32_t kPitch = 144;            // a row's 128-byte chunk in shared memory: eight rows meet different banks
+constexpr uint32_t kStages = 2;             // chunks of 32 rows in flight per warp
+constexpr uint32_t kSlice = 512;            // columns of a router row per warp: four 16-byte loads a lane, all in flight
 
 struct Matrix {
     const uint8_t* quants;
@@ -35,57 +45,42 @@ struct MoeParams {
     float* y;
     size_t x_stride, y_stride;
     const float* router;
-    uint32_t tokens, experts, top_k, hidden, inner, splits;
+    uint32_t tokens, experts, top_k, hidden, inner, splits, slices;
     int normalise, down4, x_vec, gate4;
     Matrix gate, up, down;
-    float* logits;       // [tokens][experts]
+    float* logits;       // [slices][tokens][experts]
     uint8_t* xh;         // [tokens][2 parts][hidden / 32][64 bytes], B-operand order
-    float* xs;           // [tokens][hidden / 32], what a block's parts are multiplied with
+    float2* xs;          // [tokens][hidden / 32]: what a block's sum is multiplied with, and what is added then
     uint8_t* hh;         // the inner vectors, per slot = token * top_k + place
-    float* hs;
-    uint32_t* plan;      // [0] experts with tokens, then [experts] which, [experts + 1] where their lists begin
-    uint32_t* list;      // slots by expert, ascending
-    float* weights;      // per slot
-    float* part;         // [splits][tokens][hidden]
-    uint32_t* counters;  // [0] route, [1 + i] output rows 32 i ..; zero between calls
+    float2* hs;
     int32_t* ids_out;
     float* weights_out;
 };
 
-__device__ __forceinline__ uint32_t redux_max(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
-__device__ __forceinline__ uint32_t redux_min(uint32_t v) { return __reduce_min_sync(0xffffffffu, v); }
-
-// Whether this block is the last of `count` to get here; everything the others wrote before is then visible.
-__device__ __forceinline__ bool last_of(uint32_t* counter, uint32_t count, uint32_t* shared) {
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0) *shared = atomicInc(counter, count - 1);  // back to 0 with the last one
-    __syncthreads();
-    const bool last = *shared == count - 1;
-    if (last) __threadfence();
-    return last;
-}
-
 // ------------------------------------------------------------------------------------------------- route ----
-// Sums of one expert's row with tokens t0 .. t0 + 3.
-__device__ __forceinline__ void logits_of(const MoeParams& p, uint32_t expert, uint32_t t0, uint32_t lane) {
+// A slice of one expert's row with tokens t0 .. t0 + 3.
+__device__ __forceinline__ void logits_of(const MoeParams& p, uint32_t expert, uint32_t t0, uint32_t slice, uint32_t lane) {
     const float* w = p.router + (size_t)expert * p.hidden;
-    const uint32_t n = min(4u, p.tokens - t0);
+    const uint32_t n = min(4u, p.tokens - t0), from = slice * kSlice, to = min(p.hidden, from + kSlice);
     float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     if (p.x_vec) {
-#pragma unroll 4
-        for (uint32_t i = lane * 4; i < p.hidden; i += 128) {
-            const float4 a = __ldg(reinterpret_cast<const float4*>(w + i));
+        float4 a[kSlice / 128], b[4][kSlice / 128];  // all asked for before any is used
+#pragma unroll
+        for (uint32_t k = 0; k < kSlice / 128; ++k) {
+            const uint32_t i = from + k * 128 + lane * 4;
+            a[k] = i < to ? __ldg(reinterpret_cast<const float4*>(w + i)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
             for (uint32_t t = 0; t < 4; ++t)
-                if (t < n) {
-                    const float4 b = *reinterpret_cast<const float4*>(p.x + (size_t)(t0 + t) * p.x_stride + i);
-                    sum[t] = fmaf(a.x, b.x, fmaf(a.y, b.y, fmaf(a.z, b.z, fmaf(a.w, b.w, sum[t]))));
-                }
+                b[t][k] = t < n && i < to ? *reinterpret_cast<const float4*>(p.x + (size_t)(t0 + t) * p.x_stride + i) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
+#pragma unroll
+        for (uint32_t k = 0; k < kSlice / 128; ++k)
+#pragma unroll
+            for (uint32_t t = 0; t < 4; ++t)
+                sum[t] = fmaf(a[k].x, b[t][k].x, fmaf(a[k].y, b[t][k].y, fmaf(a[k].z, b[t][k].z, fmaf(a[k].w, b[t][k].w, sum[t]))));
     } else {
 #pragma unroll 4
-        for (uint32_t i = lane; i < p.hidden; i += 32) {
+        for (uint32_t i = from + lane; i < to; i += 32) {
             const float a = __ldg(w + i);
 #pragma unroll
             for (uint32_t t = 0; t < 4; ++t)
@@ -95,101 +90,140 @@ __device__ __forceinline__ void logits_of(const MoeParams& p, uint32_t expert, u
 #pragma unroll
     for (uint32_t t = 0; t < 4; ++t) {
         const float s = warp_add(sum[t]);
-        if (t < n && lane == 0) p.logits[(size_t)(t0 + t) * p.experts + expert] = s;
+        if (t < n && lane == 0) p.logits[((size_t)slice * p.tokens + t0 + t) * p.experts + expert] = s;
     }
 }
 
-// One block of 32 values (a lane each) as two parts in B-operand order.
-__device__ __forceinline__ void split_block(float v, uint32_t lane, bool four, uint8_t* hi, uint8_t* lo, float* scale) {
-    const float up = lift(warp_max(fabsf(v)));
+// One block of 32 values (a lane each) as two parts in B-operand order, and what its sums are to be multiplied with and
+// corrected by.  Values beyond 2^103 count as infinite.
+__device__ __forceinline__ void split_block(float v, uint32_t lane, bool four, uint8_t* hi, uint8_t* lo, float2* factor) {
+    const float up = fmaxf(lift(warp_max(fabsf(v))), __uint_as_float((127u - 89u) << 23));
     const float x = v * up;
     const __half h = __float2half_rn(x), l = __float2half_rn(x - __half2float(h));
     const uint32_t at = frag_lane(lane) * 16 + frag_half(four, lane) * 2;
     *reinterpret_cast<__half*>(hi + at) = h;
     *reinterpret_cast<__half*>(lo + at) = l;
-    if (lane == 0) *scale = 1.0f / up;
+    const float sum = warp_add(__half2float(h) + __half2float(l));
+    if (lane == 0) *factor = make_float2((four ? 1048576.0f : 16777216.0f) / up, (four ? -8.0f : -128.0f) * sum / up);
 }
 
-__global__ void __launch_bounds__(kMoeThreads) moe_route_kernel(const MoeParams p) {
-    __shared__ uint32_t last;
-    __shared__ uint16_t chosen[kMaxTokens * kMaxTopK];
-    __shared__ uint32_t scan[2][kMoeWarps];
+__global__ void __launch_bounds__(kMoeThreads) moe_route_kernel(MoeParams p) {
     pdl_wait();
     pdl_launch();
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nb = p.hidden / 32;
-    const uint32_t quads = (p.tokens + 3) / 4, dots = p.experts * quads, pieces = (nb + 15) / 16;
+    const uint32_t quads = (p.tokens + 3) / 4, dots = p.experts * quads * p.slices, pieces = (nb + 7) / 8;
     for (uint32_t job = blockIdx.x * kMoeWarps + warp; job < dots + p.tokens * pieces; job += gridDim.x * kMoeWarps) {
         if (job < dots) {
-            logits_of(p, job / quads, (job % quads) * 4, lane);
+            const uint32_t slice = job % p.slices, rest = job / p.slices;
+            logits_of(p, rest / quads, (rest % quads) * 4, slice, lane);
         } else {
-            const uint32_t t = (job - dots) / pieces, b0 = (job - dots) % pieces * 16;
-#pragma unroll 4
-            for (uint32_t b = b0; b < min(b0 + 16, nb); ++b) {
-                uint8_t* hi = p.xh + ((size_t)t * 2 * nb + b) * 64;
-                split_block(p.x[(size_t)t * p.x_stride + b * 32 + lane], lane, p.gate4 != 0, hi, hi + (size_t)nb * 64,
-                            p.xs + (size_t)t * nb + b);
-            }
+            const uint32_t t = (job - dots) / pieces, b0 = (job - dots) % pieces * 8;
+            float v[8];
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) v[i] = b0 + i < nb ? p.x[(size_t)t * p.x_stride + (b0 + i) * 32 + lane] : 0.0f;
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i)
+                if (b0 + i < nb) {
+                    uint8_t* hi = p.xh + ((size_t)t * 2 * nb + b0 + i) * 64;
+                    split_block(v[i], lane, p.gate4 != 0, hi, hi + (size_t)nb * 64, p.xs + (size_t)t * nb + b0 + i);
+                }
         }
     }
-    if (!last_of(p.counters, gridDim.x, &last)) return;
+}
 
-    // ---- the top_k experts of every token, a warp each ---------------------------------------------------------
-    for (uint32_t t = warp; t < p.tokens; t += kMoeWarps) {
-        float v[kMaxExperts / 32];
-        uint32_t key[kMaxExperts / 32];  // order of the numbers, NaN lowest; 0 and `gone`: not to be taken (again)
-        uint32_t gone = 0;
-        float all = 0.0f;
+// What every block of the products knows of the routing: the experts that have tokens, and for each the list of its
+// slots (token * top_k + place), tokens ascending.
+struct Plan {
+    uint32_t active;
+    uint16_t expert[kMaxExperts], begin[kMaxExperts + 2], list[kMaxTokens * kMaxTopK];
+    float weight[kMaxTokens * kMaxTopK];
+};
+struct PlanScratch {
+    uint32_t tokens[2][kMaxExperts];  // which tokens an expert has
+    uint16_t chosen[kMaxTokens * kMaxTopK];
+    uint32_t scan[2][kMoeWarps];
+    uint4 keys[1];                    // [tokens][experts, rounded up to four]
+};
+constexpr uint32_t plan_scratch(uint32_t tokens) { return sizeof(PlanScratch) + tokens * kMaxExperts * 4; }
+
+// Numbers as unsigned integers of the same order, NaN below all (0 is below that: no expert).
+__device__ __forceinline__ uint32_t order_of(float v) {
+    const uint32_t u = __float_as_uint(v);
+    return v != v ? 1u : v == 0.0f ? 0x80000000u : u >> 31 ? ~u : u | 0x80000000u;  // -0 and 0 are a tie
+}
+__device__ __forceinline__ float value_of(uint32_t key) {
+    return key == 1u ? NAN : __uint_as_float(key >> 31 ? key & 0x7fffffffu : ~key);
+}
+
+// All threads of the block; ends with a barrier.  An expert's place among a token's logits is how many are larger, or
+// equal and earlier: a thread per (token, expert) counts, which needs no rounds of finding a largest one.
+__device__ void make_plan(const MoeParams& p, Plan* plan, PlanScratch* w, bool outputs) {
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, quads = (p.experts + 3) / 4, row = quads * 4;
+    uint32_t* keys = reinterpret_cast<uint32_t*>(w->keys);
+    w->tokens[0][tid] = w->tokens[1][tid] = 0;
+    for (uint32_t i0 = tid; i0 < p.tokens * row; i0 += 4 * kMoeThreads) {
+        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (uint32_t s0 = 0; s0 < p.slices; s0 += 4) {
+            float part[4][4];  // sixteen loads in flight
 #pragma unroll
-        for (uint32_t i = 0; i < kMaxExperts / 32; ++i) {
-            const uint32_t e = lane + 32 * i;
-            v[i] = e < p.experts ? __ldcg(p.logits + (size_t)t * p.experts + e) : -INFINITY;
-            const uint32_t u = __float_as_uint(v[i]);
-            key[i] = v[i] != v[i] ? 1u : (u >> 31 ? ~u : u | 0x80000000u);
-            if (v[i] == 0.0f) key[i] = 0x80000000u;  // -0 and 0 are a tie
-            if (e >= p.experts) gone |= 1u << i;
-        }
-        float top = 0.0f, chosen_value = 0.0f;
-        for (uint32_t j = 0; j < p.top_k; ++j) {
-            uint32_t best = 0, at = 0;
+            for (uint32_t x = 0; x < 4; ++x) {
+                const uint32_t i = i0 + x * kMoeThreads, t = i / row, e = i - t * row;
 #pragma unroll
-            for (uint32_t i = 0; i < kMaxExperts / 32; ++i)
-                if (!(gone >> i & 1) && key[i] > best) {
-                    best = key[i];
-                    at = lane + 32 * i;
-                }
-            const uint32_t winner = redux_max(best);
-            const uint32_t e = redux_min(best == winner ? at : 0xffffffffu);
-            if (best == winner && at == e) gone |= 1u << (e / 32);
-            const float f = winner == 1u ? NAN : __uint_as_float(winner >> 31 ? winner & 0x7fffffffu : ~winner);
-            if (j == 0) top = f;
-            if (lane == j) {
-                chosen[t * p.top_k + j] = (uint16_t)e;
-                chosen_value = f;
-                if (p.ids_out) p.ids_out[(size_t)t * p.top_k + j] = (int32_t)e;
+                for (uint32_t y = 0; y < 4; ++y)
+                    part[x][y] = i < p.tokens * row && e < p.experts && s0 + y < p.slices
+                                     ? __ldcg(p.logits + ((size_t)(s0 + y) * p.tokens + t) * p.experts + e) : 0.0f;
             }
-        }
-        if (p.normalise) {
-            all = warp_add(lane < p.top_k ? expf(chosen_value - top) : 0.0f);
-        } else {
 #pragma unroll
-            for (uint32_t i = 0; i < kMaxExperts / 32; ++i)
-                if (lane + 32 * i < p.experts) all += expf(v[i] - top);
-            all = warp_add(all);
+            for (uint32_t x = 0; x < 4; ++x)
+#pragma unroll
+                for (uint32_t y = 0; y < 4; ++y) v[x] += part[x][y];
         }
-        if (lane < p.top_k) {
-            const float w = expf(chosen_value - top) / all;
-            p.weights[t * p.top_k + lane] = w;
-            if (p.weights_out) p.weights_out[(size_t)t * p.top_k + lane] = w;
+#pragma unroll
+        for (uint32_t x = 0; x < 4; ++x) {
+            const uint32_t i = i0 + x * kMoeThreads;
+            if (i < p.tokens * row) keys[i] = i % row < p.experts ? order_of(v[x]) : 0u;
         }
     }
     __syncthreads();
-
-    // ---- every expert's slots, ascending; a thread per expert -------------------------------------------------------
-    const uint32_t e = threadIdx.x, slots = p.tokens * p.top_k;
-    uint32_t count = 0;
-    if (e < p.experts)
-        for (uint32_t s = 0; s < slots; ++s) count += chosen[s] == e;
-    uint32_t before = count, used = count ? 1 : 0, place = used;
+    for (uint32_t i = tid; i < p.tokens * row; i += kMoeThreads) {
+        const uint32_t t = i / row, e = i - t * row;
+        const uint32_t mine = keys[i];
+        uint32_t place = 0;
+#pragma unroll 4
+        for (uint32_t q = 0; q < quads; ++q) {
+            const uint4 k = w->keys[t * quads + q];
+            place += k.x > mine || (k.x == mine && 4 * q < e);
+            place += k.y > mine || (k.y == mine && 4 * q + 1 < e);
+            place += k.z > mine || (k.z == mine && 4 * q + 2 < e);
+            place += k.w > mine || (k.w == mine && 4 * q + 3 < e);
+        }
+        if (mine && place < p.top_k) {
+            w->chosen[t * p.top_k + place] = (uint16_t)e;
+            atomicOr(&w->tokens[t / 32][e], 1u << (t % 32));
+            if (outputs && p.ids_out) p.ids_out[(size_t)t * p.top_k + place] = (int32_t)e;
+        }
+    }
+    __syncthreads();
+    for (uint32_t t = warp; t < p.tokens; t += kMoeWarps) {
+        const float mine = lane < p.top_k ? value_of(keys[t * row + w->chosen[t * p.top_k + lane]]) : 0.0f;
+        const float top = __shfl_sync(0xffffffffu, mine, 0);
+        float all = 0.0f;
+        if (p.normalise) {
+            all = lane < p.top_k ? expf(mine - top) : 0.0f;
+        } else {
+            for (uint32_t e = lane; e < p.experts; e += 32) all += expf(value_of(keys[t * row + e]) - top);
+        }
+        all = warp_add(all);
+        if (lane < p.top_k) {
+            const float f = expf(mine - top) / all;
+            plan->weight[t * p.top_k + lane] = f;
+            if (outputs && p.weights_out) p.weights_out[(size_t)t * p.top_k + lane] = f;
+        }
+    }
+    // a thread per expert
+    uint32_t low = w->tokens[0][tid], high = w->tokens[1][tid];
+    const uint32_t count = __popc(low) + __popc(high), used = count ? 1 : 0;
+    uint32_t before = count, place = used;
 #pragma unroll
     for (int o = 1; o < 32; o *= 2) {
         const uint32_t a = __shfl_up_sync(0xffffffffu, before, o), b = __shfl_up_sync(0xffffffffu, place, o);
@@ -199,380 +233,514 @@ __global__ void __launch_bounds__(kMoeThreads) moe_route_kernel(const MoeParams 
         }
     }
     if (lane == 31) {
-        scan[0][warp] = before;
-        scan[1][warp] = place;
+        w->scan[0][warp] = before;
+        w->scan[1][warp] = place;
     }
     __syncthreads();
     uint32_t active = 0;
-    for (uint32_t w = 0; w < kMoeWarps; ++w) {
-        if (w < warp) {
-            before += scan[0][w];
-            place += scan[1][w];
+#pragma unroll
+    for (uint32_t i = 0; i < kMoeWarps; ++i) {
+        if (i < warp) {
+            before += w->scan[0][i];
+            place += w->scan[1][i];
         }
-        active += scan[1][w];
+        active += w->scan[1][i];
     }
     before -= count;
     place -= used;
-    if (threadIdx.x == 0) {
-        p.plan[0] = active;
-        p.plan[1 + p.experts + active] = slots;
+    if (tid == 0) {
+        plan->active = active;
+        plan->begin[active] = (uint16_t)(p.tokens * p.top_k);
     }
     if (used) {
-        p.plan[1 + place] = e;
-        p.plan[1 + p.experts + place] = before;
-        for (uint32_t s = 0; s < slots; ++s)
-            if (chosen[s] == e) p.list[before++] = s;
+        plan->expert[place] = (uint16_t)tid;
+        plan->begin[place] = (uint16_t)before;
+        while (low | high) {
+            const uint32_t t = low ? __ffs(low) - 1 : 32 + __ffs(high) - 1;
+            if (low) low &= low - 1;
+            else high &= high - 1;
+            uint32_t j = 0;
+            while (w->chosen[t * p.top_k + j] != tid) ++j;  // the token has chosen this expert
+            plan->list[before++] = (uint16_t)(t * p.top_k + j);
+        }
     }
+    __syncthreads();
 }
 
 // ---------------------------------------------------------------------------------------------- products ----
-// A warp's stage: ROWS rows of one column chunk (64 bytes: four Q4_0 or two Q8_0 blocks) and their scales.
-template <bool FOUR, int TILES>
-struct Stage {
-    static constexpr uint32_t rows = TILES * 16, blocks = FOUR ? 4 : 2;
-    static constexpr uint32_t scales = rows * kPitch, bytes = scales + rows * kScaleWords * 4;
+// A chunk: 128 bytes of a row's codes, eight Q4_0 or four Q8_0 blocks.
+template <bool FOUR>
+struct Chunk {
+    static constexpr uint32_t blocks = FOUR ? 8 : 4;
+    __device__ static uint32_t count(uint32_t nb) { return (nb + blocks - 1) / blocks; }
 };
 
-// Copies chunk c of 32 rows that begin at row `row0` of the matrix into rows at .. at + 31 of the stage.
-template <bool FOUR>
-__device__ __forceinline__ void fetch_rows(const Matrix& m, size_t row0, uint32_t nb, uint32_t c, uint32_t stage, uint32_t scales, uint32_t at,
-                                           uint32_t lane) {
-    constexpr uint32_t B = FOUR ? 4 : 2;
-    const uint32_t row_bytes = nb * (FOUR ? 16 : 32), col = c * 64 + (lane & 3) * 16;
-    if (col < row_bytes) {
-        const uint8_t* src = m.quants + (row0 + (lane >> 2)) * row_bytes + col;
-        const uint32_t dst = stage + (at + (lane >> 2)) * kPitch + (lane & 3) * 16;
+// Copies a chunk of 32 rows to 32 rows of kPitch bytes; src: the lane's 16 bytes of row lane / 8, `four` the bytes of
+// four rows.
+__device__ __forceinline__ void fetch_rows(const uint8_t* src, size_t four, uint32_t dst, uint32_t lane) {
+    dst += (lane >> 3) * kPitch + (lane & 7) * 16;
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) cp_async16(dst + i * 8 * kPitch, src + (size_t)i * 8 * row_bytes);
-    }
-    const size_t h0 = (row0 + lane) * nb + c * B;
-    const uint32_t words = ((uint32_t)(h0 & 1) + min(B, nb - c * B) + 1) / 2;
-    const uint8_t* src = reinterpret_cast<const uint8_t*>(m.scales) + (h0 >> 1) * 4;
-    const uint32_t dst = scales + (at + lane) * (kScaleWords * 4);
-#pragma unroll
-    for (uint32_t i = 0; i < (FOUR ? 3 : 2); ++i)
-        if (i < words) cp_async4(dst + i * 4, src + i * 4);
+    for (uint32_t i = 0; i < 8; ++i, src += four) cp_async16(dst + i * 4 * kPitch, src);
 }
 
-// The scales of one row's blocks of the chunk, as f32.
-template <bool FOUR>
-__device__ __forceinline__ void scales_of(uint32_t addr, uint32_t odd, float (&d)[FOUR ? 4 : 2]) {
-    uint32_t w0 = lds32(addr), w1 = lds32(addr + 4);
-    if (FOUR) {
-        const uint32_t w2 = lds32(addr + 8);
-        if (odd) {
-            w0 = __funnelshift_r(w0, w1, 16);
-            w1 = __funnelshift_r(w1, w2, 16);
+// Has a chunk's scales of a row fetched into the L2: they are read straight from there, too late to wait for the memory.
+__device__ __forceinline__ void prefetch_scales(const uint16_t* scales) { asm volatile("prefetch.global.L2 [%0];" ::"l"(scales)); }
+
+// The scales of a lane's rows g, g + 8, g + 16, g + 24 for the chunk that begins at block b, as pairs of halves.
+// WHOLE: a row's blocks are a multiple of the chunk's, so chunks are complete and the scales' addresses aligned.
+template <bool FOUR, bool WHOLE>
+struct Scales {
+    static constexpr uint32_t B = Chunk<FOUR>::blocks;
+    uint32_t pair[4][B / 2];
+    __device__ __forceinline__ void load(const uint16_t* row, uint32_t b, uint32_t nb) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint16_t* s = row + i * 8 * nb + b;
+            if (WHOLE && FOUR) {
+                const uint4 v = __ldg(reinterpret_cast<const uint4*>(s));
+                pair[i][0] = v.x;
+                pair[i][1] = v.y;
+                pair[i][B / 2 - 2] = v.z;
+                pair[i][B / 2 - 1] = v.w;
+            } else if (WHOLE) {
+                const uint2 v = __ldg(reinterpret_cast<const uint2*>(s));
+                pair[i][0] = v.x;
+                pair[i][1] = v.y;
+            } else if (nb % 2 == 0) {
+#pragma unroll
+                for (uint32_t k = 0; k < B / 2; ++k) pair[i][k] = b + 2 * k < nb ? __ldg(reinterpret_cast<const uint32_t*>(s + 2 * k)) : 0u;
+            } else {
+#pragma unroll
+                for (uint32_t k = 0; k < B / 2; ++k) {
+                    const uint32_t lo = b + 2 * k < nb ? __ldg(s + 2 * k) : 0u, hi = b + 2 * k + 1 < nb ? __ldg(s + 2 * k + 1) : 0u;
+                    pair[i][k] = lo | hi << 16;
+                }
+            }
         }
-        const float2 a = __half22float2(bits_h2(w0)), b = __half22float2(bits_h2(w1));
-        d[0] = a.x;
-        d[1] = a.y;
-        d[FOUR ? 2 : 0] = b.x;
-        d[FOUR ? 3 : 1] = b.y;
-    } else {
-        if (odd) w0 = __funnelshift_r(w0, w1, 16);
-        const float2 a = __half22float2(bits_h2(w0));
-        d[0] = a.x;
-        d[1] = a.y;
     }
-}
+    __device__ __forceinline__ float of(int row, uint32_t j) const {
+        const __half2 d = bits_h2(pair[row][j / 2]);
+        return j % 2 ? __high2float(d) : __low2float(d);
+    }
+};
 
-// What a lane needs of the vectors: the B operand of token 4 n + g / 2 (part g % 2), the block scales of token 4 n + t.
+// The vectors of a pass as a lane needs them: the B operand of token 4 n + g / 2 (part g % 2), the factors of token
+// 4 n + t; null where there is no such token.
 template <int NT>
 struct Vectors {
-    const uint8_t* parts[NT];  // null: no such token
-    const float* scale[NT];
-};
-
-// acc[m][n] += chunk's 16-row tiles times the vectors: rows g and g + 8 of tile m, token 4 n + t.
-// odd[m]: bit 0 / 1 = whether the scales of rows g / g + 8 begin at an odd half.
-template <bool FOUR, int TILES, int NT>
-__device__ __forceinline__ void multiply(uint32_t stage, uint32_t c, uint32_t nb, const Vectors<NT>& x, const uint32_t (&odd)[TILES], uint32_t lane,
-                                         float (&acc)[TILES][NT][2], const uint4 (&bq)[FOUR ? 4 : 2][NT], const float (&sx)[FOUR ? 4 : 2][NT]) {
-    constexpr uint32_t B = FOUR ? 4 : 2;
-    const uint32_t g = lane >> 2;
-    float d[TILES][2][B];
-#pragma unroll
-    for (int m = 0; m < TILES; ++m)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-            scales_of<FOUR>(stage + Stage<FOUR, TILES>::scales + (m * 16 + h * 8 + g) * (kScaleWords * 4), (odd[m] >> h) & 1, d[m][h]);
-#pragma unroll
-    for (uint32_t j = 0; j < B; ++j) {
-        if (c * B + j >= nb) break;
-        uint32_t a[TILES][2][4];
-        if (FOUR) {
-#pragma unroll
-            for (int m = 0; m < TILES; m += 2) {
-                uint32_t w[4];
-                ldmatrix_x4(w, stage + (m * 16 + lane) * kPitch + j * 16);
-                a_of_nibbles(w[0], w[1], a[m]);
-                a_of_nibbles(w[2], w[3], a[m + 1]);
-            }
-        } else {
-#pragma unroll
-            for (int m = 0; m < TILES; ++m) {
-                uint32_t w[4];
-                ldmatrix_x4(w, stage + (m * 16 + (lane & 15)) * kPitch + j * 32 + (lane >> 4) * 16);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] ^= 0x80808080u;
-                a_of_bytes(w, a[m]);
-            }
-        }
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int m = 0; m < TILES; ++m) {
-                float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                mma_f16(s, a[m][0], bq[j][n].x, bq[j][n].y);
-                mma_f16(s, a[m][1], bq[j][n].z, bq[j][n].w);
-                acc[m][n][0] = fmaf((s[0] + s[1]) * sx[j][n], d[m][0][j], acc[m][n][0]);
-                acc[m][n][1] = fmaf((s[2] + s[3]) * sx[j][n], d[m][1][j], acc[m][n][1]);
-            }
-    }
-}
-
-template <bool FOUR, int NT>
-__device__ __forceinline__ void load_vectors(const Vectors<NT>& x, uint32_t c, uint32_t nb, uint4 (&bq)[FOUR ? 4 : 2][NT],
-                                             float (&sx)[FOUR ? 4 : 2][NT]) {
-    constexpr uint32_t B = FOUR ? 4 : 2;
-#pragma unroll
-    for (uint32_t j = 0; j < B; ++j)
+    const uint8_t* px[NT];
+    const float2* pf[NT];
+    __device__ __forceinline__ Vectors(const uint8_t* h, const float2* f, uint32_t nb, const uint16_t* slots, uint32_t count, uint32_t per_row,
+                                       uint32_t lane) {
+        const uint32_t g = lane >> 2, t = lane & 3;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            bq[j][n] = make_uint4(0, 0, 0, 0);
-            sx[j][n] = 0.0f;
-            if (c * B + j < nb) {
-                if (x.parts[n]) bq[j][n] = *reinterpret_cast<const uint4*>(x.parts[n] + (size_t)(c * B + j) * 64);
-                if (x.scale[n]) sx[j][n] = x.scale[n][c * B + j];
+            const uint32_t i = 4 * n + g / 2, k = 4 * n + t;
+            px[n] = i < count ? h + ((size_t)(slots[i] / per_row) * 2 + (g & 1)) * nb * 64 + t * 16 : nullptr;
+            pf[n] = k < count ? f + (size_t)(slots[k] / per_row) * nb : nullptr;
+        }
+    }
+    __device__ __forceinline__ void load(uint32_t block, bool there, uint4 (&parts)[NT], float2 (&factor)[NT]) const {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            parts[n] = make_uint4(0, 0, 0, 0);
+            factor[n] = make_float2(0.0f, 0.0f);
+            if (there) {
+                if (px[n]) parts[n] = *reinterpret_cast<const uint4*>(px[n] + (size_t)block * 64);
+                if (pf[n]) factor[n] = pf[n][block];
             }
         }
+    }
+};
+
+// acc[m][n] += block j of the two 16-row tiles of a stage: rows 16 m + g and 16 m + g + 8, token 4 n + t.
+template <bool FOUR, int NT, class D>
+__device__ __forceinline__ void multiply(uint32_t stage, uint32_t j, uint32_t lane, const uint4 (&parts)[NT], const float2 (&factor)[NT], D scale,
+                                         float (&acc)[2][NT][2]) {
+    uint32_t a[2][2][4];
+    if (FOUR) {
+        uint32_t w[4];
+        ldmatrix_x4(w, stage + lane * kPitch + j * 16);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t u = w[2 * i + h];
+                a[i][0][h] = (u << 4) & 0x00f000f0u;
+                a[i][0][2 + h] = (u >> 4) & 0x00f000f0u;
+                a[i][1][h] = u & 0x00f000f0u;
+                a[i][1][2 + h] = (u >> 8) & 0x00f000f0u;
+            }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            uint32_t w[4];
+            ldmatrix_x4(w, stage + (i * 16 + (lane & 15)) * kPitch + j * 32 + (lane >> 4) * 16);
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+                const uint32_t u = w[h] ^ 0x80808080u;
+                a[i][h >> 1][h & 1] = __byte_perm(u, 0, 0x4140);
+                a[i][h >> 1][2 + (h & 1)] = __byte_perm(u, 0, 0x4342);
+            }
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float s[4];
+            mma_f16_new(s, a[i][0], parts[n].x, parts[n].y);
+            mma_f16(s, a[i][1], parts[n].z, parts[n].w);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) acc[i][n][h] = fmaf(fmaf(s[2 * h] + s[2 * h + 1], factor[n].x, factor[n].y), scale(2 * i + h), acc[i][n][h]);
+        }
+}
+
+// Sums of chunks c0, c0 + 8, .. < c1 of 32 rows of each of MATS matrices (`rows`: scales of the lane's row g), which are in
+// the ring one after the other.  next() waits for the next 32 rows and says where they are, done() gives them back.
+template <bool FOUR, bool WHOLE, int MATS, int NT, class Next, class Done>
+__device__ __forceinline__ void dot_chunks(const Vectors<NT>& x, uint32_t nb, const uint16_t* const (&rows)[MATS], uint32_t c0, uint32_t c1,
+                                           uint32_t lane, Next next, Done done, float (&acc)[MATS][2][NT][2]) {
+    constexpr uint32_t B = Chunk<FOUR>::blocks;
+#pragma unroll
+    for (int a = 0; a < MATS; ++a)
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) acc[a][m][n][0] = acc[a][m][n][1] = 0.0f;
+    for (uint32_t c = c0; c < c1; c += kMoeWarps) {
+        // with four tokens at most the chunk's vectors stay in registers for all matrices; more are read block by block
+        uint4 parts[NT == 1 ? B : 1][NT];
+        float2 factor[NT == 1 ? B : 1][NT];
+        if (NT == 1) {
+#pragma unroll
+            for (uint32_t j = 0; j < B; ++j) x.load(c * B + j, WHOLE || c * B + j < nb, parts[NT == 1 ? j : 0], factor[NT == 1 ? j : 0]);
+        }
+#pragma unroll
+        for (int a = 0; a < MATS; ++a) {
+            Scales<FOUR, WHOLE> d;
+            d.load(rows[a], c * B, nb);
+            const uint32_t stage = next();
+#pragma unroll
+            for (uint32_t j = 0; j < B; ++j)
+                if (WHOLE || c * B + j < nb) {
+                    const uint32_t k = NT == 1 ? j : 0;
+                    if (NT > 1) x.load(c * B + j, true, parts[k], factor[k]);
+                    multiply<FOUR, NT>(stage, j, lane, parts[k], factor[k], [&](int row) { return d.of(row, j); }, acc[a]);
+                }
+            done();
+        }
+    }
 }
 
 // ------------------------------------------------------------------------------------------------- inner ----
-template <bool FOUR>
-constexpr uint32_t inner_smem() {
-    constexpr uint32_t ring = kMoeWarps * kStages * Stage<FOUR, 4>::bytes, sums = kMoeWarps * 64 * (kGroup + 1) * 4;
-    return ring > sums ? ring : sums;
-}
+constexpr uint32_t kStage = 32 * kPitch;
+constexpr uint32_t kRing = kMoeWarps * kStages * kStage;
+constexpr uint32_t kInnerSums = kMoeWarps * 64 * (kGroup + 1) * 4;
+constexpr uint32_t kInnerSmem = kRing + kInnerSums + sizeof(Plan);
+static_assert(plan_scratch(kMaxTokens) <= kRing + kInnerSums, "the plan is made where ring and sums are later");
 
-template <bool FOUR, int NT>
-__device__ void inner_unit(const MoeParams& p, uint32_t expert, uint32_t rows32, const uint32_t* slots, uint32_t count, uint8_t* smem) {
-    using S = Stage<FOUR, 4>;
-    constexpr uint32_t B = S::blocks;
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const uint32_t nb = p.hidden / 32, chunks = (nb + B - 1) / B, nbf = p.inner / 32;
-    const size_t row0 = (size_t)expert * p.inner + rows32 * 32;
-    Vectors<NT> x;
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        const uint32_t i = 4 * n + g / 2, k = 4 * n + t;
-        x.parts[n] = i < count ? p.xh + ((size_t)(slots[i] / p.top_k) * 2 + (g & 1)) * nb * 64 + t * 16 : nullptr;
-        x.scale[n] = k < count ? p.xs + (size_t)(slots[k] / p.top_k) * nb : nullptr;
+// A pass over a unit's weights: 32 inner rows of an expert, up to kGroup of its tokens.  Block b of the grid has units
+// b, b + grid, ...
+struct InnerPass {
+    uint32_t unit, at, end, rows32, expert;
+    __device__ void enter(const Plan* plan, uint32_t tiles, uint32_t units) {
+        if (unit >= units) return;
+        const uint32_t a = unit / tiles;
+        rows32 = unit - a * tiles;
+        expert = plan->expert[a];
+        at = plan->begin[a];
+        end = plan->begin[a + 1];
     }
-    uint32_t odd[4];  // a chunk begins at an even block
-#pragma unroll
-    for (int m = 0; m < 4; ++m)
-        odd[m] = (uint32_t)((row0 + (m & 1) * 16 + g) * nb & 1) | (uint32_t)((row0 + (m & 1) * 16 + 8 + g) * nb & 1) << 1;
-    const uint32_t ring = smem_addr(smem) + warp * kStages * S::bytes;
-    auto fetch = [&](uint32_t k) {
-        const uint32_t c = warp + k * kMoeWarps;
-        if (c < chunks) {
-            const uint32_t st = ring + (k % kStages) * S::bytes;
-            fetch_rows<FOUR>(p.gate, row0, nb, c, st, st + S::scales, 0, lane);
-            fetch_rows<FOUR>(p.up, row0, nb, c, st, st + S::scales, 32, lane);
-        }
-        cp_async_commit();
-    };
-    float acc[4][NT][2];
-#pragma unroll
-    for (int m = 0; m < 4; ++m)
-#pragma unroll
-        for (int n = 0; n < NT; ++n) acc[m][n][0] = acc[m][n][1] = 0.0f;
-#pragma unroll
-    for (uint32_t k = 0; k < kStages; ++k) fetch(k);
-    for (uint32_t k = 0; warp + k * kMoeWarps < chunks; ++k) {
-        const uint32_t c = warp + k * kMoeWarps;
-        uint4 bq[B][NT];
-        float sx[B][NT];
-        load_vectors<FOUR, NT>(x, c, nb, bq, sx);
-        cp_async_wait<kStages - 1>();
-        __syncwarp();
-        multiply<FOUR, 4, NT>(ring + (k % kStages) * S::bytes, c, nb, x, odd, lane, acc, bq, sx);
-        __syncwarp();
-        fetch(k + kStages);
+    __device__ void next(const Plan* plan, uint32_t tiles, uint32_t units) {
+        at += kGroup;
+        if (at < end) return;
+        unit += gridDim.x;
+        enter(plan, tiles, units);
     }
-    cp_async_wait<0>();
-    __syncthreads();
-    // ---- the eight warps' sums: gate rows 0..31, up rows 32..63 ------------------------------------------------------
-    constexpr uint32_t W = 4 * NT + 1;
-    float* sums = reinterpret_cast<float*>(smem);
-#pragma unroll
-    for (int m = 0; m < 4; ++m)
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) sums[(warp * 64 + m * 16 + h * 8 + g) * W + 4 * n + t] = acc[m][n][h];
-    __syncthreads();
-    for (uint32_t i = warp; i < count; i += kMoeWarps) {
-        float a = 0.0f, b = 0.0f;
-#pragma unroll
-        for (uint32_t w = 0; w < kMoeWarps; ++w) {
-            a += sums[(w * 64 + lane) * W + i];
-            b += sums[(w * 64 + 32 + lane) * W + i];
-        }
-        const float h = a / (1.0f + expf(-a)) * b;
-        const uint32_t slot = slots[i];
-        uint8_t* hi = p.hh + ((size_t)slot * 2 * nbf + rows32) * 64;
-        split_block(h, lane, p.down4 != 0, hi, hi + (size_t)nbf * 64, p.hs + (size_t)slot * nbf + rows32);
-    }
-    __syncthreads();
-}
+};
 
-template <bool FOUR>
-__global__ void __launch_bounds__(kMoeThreads, 2) moe_inner_kernel(const MoeParams p) {
+template <bool FOUR, bool WHOLE>
+__global__ void __launch_bounds__(kMoeThreads, 2) moe_inner_kernel(MoeParams p) {
     extern __shared__ __align__(128) uint8_t smem[];
+    constexpr uint32_t B = Chunk<FOUR>::blocks;
+    Plan* plan = reinterpret_cast<Plan*>(smem + kRing + kInnerSums);
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     pdl_wait();
     pdl_launch();
-    const uint32_t tiles = p.inner / 32, units = p.plan[0] * tiles;
-    for (uint32_t u = blockIdx.x; u < units; u += gridDim.x) {
-        const uint32_t a = u / tiles, rows32 = u - a * tiles, expert = p.plan[1 + a];
-        const uint32_t begin = p.plan[1 + p.experts + a], end = p.plan[2 + p.experts + a];
-        for (uint32_t at = begin; at < end; at += kGroup) {
-            const uint32_t count = min(kGroup, end - at);
-            if (count <= 4) inner_unit<FOUR, 1>(p, expert, rows32, p.list + at, count, smem);
-            else if (count <= 8) inner_unit<FOUR, 2>(p, expert, rows32, p.list + at, count, smem);
-            else inner_unit<FOUR, 4>(p, expert, rows32, p.list + at, count, smem);
+    make_plan(p, plan, reinterpret_cast<PlanScratch*>(smem), blockIdx.x == 0);
+    const uint32_t nb = p.hidden / 32, chunks = Chunk<FOUR>::count(nb), tiles = p.inner / 32, nbf = tiles, units = plan->active * tiles;
+    const uint32_t ring = smem_addr(smem) + warp * kStages * kStage, row_bytes = nb * (FOUR ? 16 : 32);
+    float* sums = reinterpret_cast<float*>(smem + kRing);
+
+    // what is copied runs kStages steps (32 gate rows, 32 up rows, the next chunk's gate rows, ..) ahead of what is multiplied
+    InnerPass ahead;
+    ahead.unit = blockIdx.x;
+    ahead.enter(plan, tiles, units);
+    InnerPass now = ahead;
+    const uint8_t *gate = nullptr, *up = nullptr;  // the lane's 16 bytes of the chunk to come
+    const uint16_t *gate_scales = nullptr, *up_scales = nullptr;
+    uint32_t ahead_c = 0, filled = 0, used = 0;
+    auto start = [&]() {  // of the pass `ahead`
+        const size_t row0 = (size_t)ahead.expert * p.inner + ahead.rows32 * 32;
+        const size_t at = (row0 + (lane >> 3)) * row_bytes + warp * 128 + (lane & 7) * 16, sc = (row0 + lane) * nb + warp * B;
+        gate = p.gate.quants + at;
+        up = p.up.quants + at;
+        gate_scales = p.gate.scales + sc;
+        up_scales = p.up.scales + sc;
+        ahead_c = warp;
+    };
+    start();
+    auto fetch = [&]() {
+        const bool is_up = filled & 1;
+        if (!is_up && ahead_c >= chunks && warp < chunks && ahead.unit < units) {
+            ahead.next(plan, tiles, units);
+            start();
         }
+        if (ahead_c < chunks && ahead.unit < units) {
+            if (WHOLE || ahead_c * 128 + (lane & 7) * 16 < row_bytes)
+                fetch_rows(is_up ? up : gate, (size_t)4 * row_bytes, ring + (filled % kStages) * kStage, lane);
+            prefetch_scales(is_up ? up_scales : gate_scales);
+            if (is_up) {
+                gate += kMoeWarps * 128;
+                up += kMoeWarps * 128;
+                gate_scales += kMoeWarps * B;
+                up_scales += kMoeWarps * B;
+                ahead_c += kMoeWarps;
+            }
+        }
+        ++filled;
+        cp_async_commit();
+    };
+#pragma unroll
+    for (uint32_t k = 0; k < kStages; ++k) fetch();
+
+    for (; now.unit < units; now.next(plan, tiles, units)) {
+        const uint32_t count = min(kGroup, now.end - now.at);
+        const uint16_t* slots = plan->list + now.at;
+        const size_t at = ((size_t)now.expert * p.inner + now.rows32 * 32 + g) * nb;
+        const uint16_t* const rows[2] = {p.gate.scales + at, p.up.scales + at};
+        auto next = [&]() {
+            cp_async_wait<kStages - 1>();
+            __syncwarp();
+            return ring + (used % kStages) * kStage;
+        };
+        auto done = [&]() {
+            ++used;
+            __syncwarp();
+            fetch();
+        };
+        auto pass = [&](auto groups) {
+            constexpr int NT = decltype(groups)::value;
+            float acc[2][2][NT][2];
+            const Vectors<NT> x(p.xh, p.xs, nb, slots, count, p.top_k, lane);
+            dot_chunks<FOUR, WHOLE, 2, NT>(x, nb, rows, warp, chunks, lane, next, done, acc);
+            // the eight warps' sums: gate rows 0..31, up rows 32..63
+            constexpr uint32_t W = 4 * NT + 1;
+#pragma unroll
+            for (int a = 0; a < 2; ++a)
+#pragma unroll
+                for (int m = 0; m < 2; ++m)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) sums[(warp * 64 + a * 32 + m * 16 + h * 8 + g) * W + 4 * n + t] = acc[a][m][n][h];
+            __syncthreads();
+            for (uint32_t i = warp; i < count; i += kMoeWarps) {
+                float a = 0.0f, b = 0.0f;
+#pragma unroll
+                for (uint32_t w = 0; w < kMoeWarps; ++w) {
+                    a += sums[(w * 64 + lane) * W + i];
+                    b += sums[(w * 64 + 32 + lane) * W + i];
+                }
+                const float h = a / (1.0f + expf(-a)) * b;
+                const uint32_t slot = slots[i];
+                uint8_t* hi = p.hh + ((size_t)slot * 2 * nbf + now.rows32) * 64;
+                split_block(h, lane, p.down4 != 0, hi, hi + (size_t)nbf * 64, p.hs + (size_t)slot * nbf + now.rows32);
+            }
+            __syncthreads();
+        };
+        if (count <= 4) pass(std::integral_constant<int, 1>());
+        else pass(std::integral_constant<int, 2>());
     }
+    cp_async_wait<0>();
 }
 
 // -------------------------------------------------------------------------------------------------- down ----
-template <bool FOUR>
-constexpr uint32_t down_ring() {
-    return kMoeWarps * kStages * Stage<FOUR, 2>::bytes;
+constexpr uint32_t kDownSmem = kRing + sizeof(Plan);                       // and [warps][tokens][33] sums, between the two
+constexpr uint32_t down_sums(uint32_t tokens) { return kMoeWarps * tokens * 33 * 4; }
+static_assert(plan_scratch(48) <= kRing && plan_scratch(kMaxTokens) <= kRing + down_sums(49), "the plan is made where ring and sums are later");
+
+// A warp's way through the block's share of all experts' chunks, counted through: chunk `warp` of every eight, and
+// for each expert a pass per kGroup tokens.
+struct DownPass {
+    uint32_t a, at, c, c1;  // expert number in the plan, its tokens from `at` on, chunks c, c + 8, .. < c1
+    uint32_t c0;
+    // enters expert a or the next one that has a chunk for this warp
+    __device__ void enter(const Plan* plan, uint32_t chunks, uint32_t lo, uint32_t hi, uint32_t warp) {
+        for (; a < plan->active && a * chunks < hi; ++a) {
+            const uint32_t first = a * chunks, from = max(lo, first);
+            c1 = min(hi, first + chunks) - first;
+            c0 = from + (warp + kMoeWarps - (from - lo) % kMoeWarps) % kMoeWarps - first;
+            if (c0 < c1) {
+                at = plan->begin[a];
+                c = c0;
+                return;
+            }
+        }
+        a = kMaxExperts;
+    }
+    __device__ bool valid() const { return a < kMaxExperts; }
+    // on to the next pass over this expert's chunks, or to the next expert
+    __device__ void next_pass(const Plan* plan, uint32_t chunks, uint32_t lo, uint32_t hi, uint32_t warp) {
+        at += kGroup;
+        if (at < plan->begin[a + 1]) {
+            c = c0;
+        } else {
+            ++a;
+            enter(plan, chunks, lo, hi, warp);
+        }
+    }
+};
+
+constexpr uint32_t kMaxSplits = 4;  // blocks of a cluster; eight did not all find room at once (19 against 12 us)
+
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The float at shared-memory address `at` of block `rank` of the cluster.
+__device__ __forceinline__ float cluster_load(uint32_t at, uint32_t rank) {
+    uint32_t there;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(there) : "memory");
+    return v;
 }
 
-// This warp's chunks of one expert and up to 4 NT of its tokens; the weighted sums go to the warp's own rows of `mine`.
-template <bool FOUR, int NT>
-__device__ __forceinline__ void down_expert(const MoeParams& p, uint32_t expert, size_t row0, uint32_t c0, uint32_t c1, const uint32_t* slots,
-                                            uint32_t count, uint32_t ring, float* mine, uint32_t lane) {
-    using S = Stage<FOUR, 2>;
-    constexpr uint32_t B = S::blocks;
-    const uint32_t g = lane >> 2, t = lane & 3, nb = p.inner / 32;
-    Vectors<NT> x;
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        const uint32_t i = 4 * n + g / 2, k = 4 * n + t;
-        x.parts[n] = i < count ? p.hh + ((size_t)slots[i] * 2 + (g & 1)) * nb * 64 + t * 16 : nullptr;
-        x.scale[n] = k < count ? p.hs + (size_t)slots[k] * nb : nullptr;
-    }
-    uint32_t odd[2];
-#pragma unroll
-    for (int m = 0; m < 2; ++m) odd[m] = (uint32_t)((row0 + m * 16 + g) * nb & 1) | (uint32_t)((row0 + m * 16 + 8 + g) * nb & 1) << 1;
-    float acc[2][NT][2];
-#pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int n = 0; n < NT; ++n) acc[m][n][0] = acc[m][n][1] = 0.0f;
-    auto fetch = [&](uint32_t c, uint32_t k) {
-        if (c < c1) {
-            const uint32_t st = ring + (k % kStages) * S::bytes;
-            fetch_rows<FOUR>(p.down, row0, nb, c, st, st + S::scales, 0, lane);
+template <bool FOUR, bool WHOLE>
+__global__ void __launch_bounds__(kMoeThreads, 2) moe_down_kernel(MoeParams p) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    constexpr uint32_t B = Chunk<FOUR>::blocks;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    Plan* plan = reinterpret_cast<Plan*>(smem + kRing + down_sums(p.tokens));
+    float* sums = reinterpret_cast<float*>(smem + kRing);  // [warps][tokens][33]
+    float* mine = sums + warp * p.tokens * 33;
+    // The logits are the route kernel's, which had ended before any block of the inner kernel let this one start.
+    make_plan(p, plan, reinterpret_cast<PlanScratch*>(smem), false);
+    for (uint32_t i = lane; i < p.tokens * 33; i += 32) mine[i] = 0.0f;
+    __syncwarp();
+    const uint32_t tile = blockIdx.x, split = blockIdx.y;
+    const uint32_t nb = p.inner / 32, chunks = Chunk<FOUR>::count(nb), row_bytes = nb * (FOUR ? 16 : 32);
+    const uint64_t all = (uint64_t)plan->active * chunks;
+    const uint32_t lo = (uint32_t)(all * split / p.splits), hi = (uint32_t)(all * (split + 1) / p.splits);
+    const uint32_t ring = smem_addr(smem) + warp * kStages * kStage;
+
+    DownPass ahead;
+    ahead.a = lo / chunks;
+    ahead.enter(plan, chunks, lo, hi, warp);
+    DownPass now = ahead;
+    const uint8_t* codes = nullptr;
+    const uint16_t* scales_ahead = nullptr;
+    uint32_t filled = 0, used = 0;
+    auto start = [&]() {
+        if (!ahead.valid()) return;
+        const size_t row0 = (size_t)plan->expert[ahead.a] * p.hidden + tile * 32;
+        codes = p.down.quants + (row0 + (lane >> 3)) * row_bytes + ahead.c * 128 + (lane & 7) * 16;
+        scales_ahead = p.down.scales + (row0 + lane) * nb + ahead.c * B;
+    };
+    start();
+    auto fetch = [&]() {
+        if (ahead.valid()) {
+            if (WHOLE || ahead.c * 128 + (lane & 7) * 16 < row_bytes)
+                fetch_rows(codes, (size_t)4 * row_bytes, ring + (filled % kStages) * kStage, lane);
+            prefetch_scales(scales_ahead);
+            codes += kMoeWarps * 128;
+            scales_ahead += kMoeWarps * B;
+            ahead.c += kMoeWarps;
+            if (ahead.c >= ahead.c1) {
+                ahead.next_pass(plan, chunks, lo, hi, warp);
+                start();
+            }
         }
+        ++filled;
         cp_async_commit();
     };
 #pragma unroll
-    for (uint32_t k = 0; k < kStages; ++k) fetch(c0 + k * kMoeWarps, k);
-    uint32_t k = 0;
-    for (uint32_t c = c0; c < c1; c += kMoeWarps, ++k) {
-        uint4 bq[B][NT];
-        float sx[B][NT];
-        load_vectors<FOUR, NT>(x, c, nb, bq, sx);
-        cp_async_wait<kStages - 1>();
-        __syncwarp();
-        multiply<FOUR, 2, NT>(ring + (k % kStages) * S::bytes, c, nb, x, odd, lane, acc, bq, sx);
-        __syncwarp();
-        fetch(c + kStages * kMoeWarps, k);
+    for (uint32_t k = 0; k < kStages; ++k) fetch();
+    pdl_wait();  // for the inner vectors
+    pdl_launch();
+    while (now.valid()) {
+        const uint32_t begin = now.at, count = min(kGroup, plan->begin[now.a + 1] - begin);
+        const uint16_t* slots = plan->list + begin;
+        const uint16_t* const rows[1] = {p.down.scales + ((size_t)plan->expert[now.a] * p.hidden + tile * 32 + g) * nb};
+        auto next = [&]() {
+            cp_async_wait<kStages - 1>();
+            __syncwarp();
+            return ring + (used % kStages) * kStage;
+        };
+        auto done = [&]() {
+            ++used;
+            __syncwarp();
+            fetch();
+        };
+        auto pass = [&](auto groups) {
+            constexpr int NT = decltype(groups)::value;
+            float acc[1][2][NT][2];
+            const Vectors<NT> x(p.hh, p.hs, nb, slots, count, 1, lane);
+            dot_chunks<FOUR, WHOLE, 1, NT>(x, nb, rows, now.c0, now.c1, lane, next, done, acc);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const uint32_t i = 4 * n + t;
+                if (i < count) {
+                    const uint32_t slot = slots[i];
+                    const float w = plan->weight[slot];
+                    float* to = mine + (slot / p.top_k) * 33;
+#pragma unroll
+                    for (int m = 0; m < 2; ++m)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) to[m * 16 + h * 8 + g] = fmaf(w, acc[0][m][n][h], to[m * 16 + h * 8 + g]);
+                }
+            }
+            __syncwarp();
+        };
+        if (count <= 4) pass(std::integral_constant<int, 1>());
+        else pass(std::integral_constant<int, 2>());
+        now.next_pass(plan, chunks, lo, hi, warp);
     }
     cp_async_wait<0>();
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        const uint32_t i = 4 * n + t;
-        if (i < count) {
-            const uint32_t slot = slots[i];
-            const float w = p.weights[slot];
-            float* to = mine + (slot / p.top_k) * 33;
-#pragma unroll
-            for (int m = 0; m < 2; ++m)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) to[m * 16 + h * 8 + g] = fmaf(w, acc[m][n][h], to[m * 16 + h * 8 + g]);
-        }
-    }
-    __syncwarp();
-}
-
-template <bool FOUR>
-__global__ void __launch_bounds__(kMoeThreads, 2) moe_down_kernel(const MoeParams p) {
-    extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ uint32_t last;
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    float* sums = reinterpret_cast<float*>(smem + down_ring<FOUR>());  // [warps][tokens][33]
-    float* mine = sums + warp * p.tokens * 33;
-    for (uint32_t i = lane; i < p.tokens * 33; i += 32) mine[i] = 0.0f;
-    __syncwarp();
-    pdl_wait();
-    pdl_launch();
-    const uint32_t tile = blockIdx.x, split = blockIdx.y;
-    const uint32_t nb = p.inner / 32, chunks = (nb + (FOUR ? 3 : 1)) / (FOUR ? 4 : 2), active = p.plan[0];
-    const uint64_t all = (uint64_t)active * chunks;
-    // this block's share of all experts' chunks; the warps take them in turn
-    const uint32_t lo = (uint32_t)(all * split / p.splits), hi = (uint32_t)(all * (split + 1) / p.splits);
-    const uint32_t ring = smem_addr(smem) + warp * kStages * Stage<FOUR, 2>::bytes;
-    for (uint32_t a = lo / chunks; a < active && a * chunks < hi; ++a) {
-        const uint32_t first = a * chunks, from = max(lo, first), to = min(hi, first + chunks);
-        // the first chunk >= from whose number is the warp's, counted through all experts
-        const uint32_t c0 = from + (warp + kMoeWarps - (from - lo) % kMoeWarps) % kMoeWarps;
-        if (c0 >= to) continue;
-        const uint32_t expert = p.plan[1 + a], begin = p.plan[1 + p.experts + a], end = p.plan[2 + p.experts + a];
-        const size_t row0 = (size_t)expert * p.hidden + tile * 32;
-        for (uint32_t at = begin; at < end; at += kGroup) {
-            const uint32_t count = min(kGroup, end - at);
-            if (count <= 4) down_expert<FOUR, 1>(p, expert, row0, c0 - first, to - first, p.list + at, count, ring, mine, lane);
-            else if (count <= 8) down_expert<FOUR, 2>(p, expert, row0, c0 - first, to - first, p.list + at, count, ring, mine, lane);
-            else down_expert<FOUR, 4>(p, expert, row0, c0 - first, to - first, p.list + at, count, ring, mine, lane);
-        }
-    }
     __syncthreads();
-    for (uint32_t t = warp; t < p.tokens; t += kMoeWarps) {
+    // The warps' sums, then the cluster's: its blocks have a share of the columns each, of the same rows.
+    for (uint32_t k = warp; k < p.tokens; k += kMoeWarps) {
         float s = 0.0f;
 #pragma unroll
-        for (uint32_t w = 0; w < kMoeWarps; ++w) s += sums[(w * p.tokens + t) * 33 + lane];
-        if (p.splits == 1) p.y[(size_t)t * p.y_stride + tile * 32 + lane] = s;
-        else p.part[((size_t)split * p.tokens + t) * p.hidden + tile * 32 + lane] = s;
+        for (uint32_t w = 0; w < kMoeWarps; ++w) s += sums[(w * p.tokens + k) * 33 + lane];
+        if (p.splits == 1) p.y[(size_t)k * p.y_stride + tile * 32 + lane] = s;
+        else sums[k * 33 + lane] = s;  // row k of warp 0, which only this warp reads
     }
     if (p.splits == 1) return;
-    if (!last_of(p.counters + 1 + tile, p.splits, &last)) return;
-    for (uint32_t t = warp; t < p.tokens; t += kMoeWarps) {
-        float s = 0.0f;
-        for (uint32_t i = 0; i < p.splits; ++i) s += __ldcg(p.part + ((size_t)i * p.tokens + t) * p.hidden + tile * 32 + lane);
-        p.y[(size_t)t * p.y_stride + tile * 32 + lane] = s;
+    cluster_barrier();
+    for (uint32_t k = split * kMoeWarps + warp; k < p.tokens; k += p.splits * kMoeWarps) {
+        const uint32_t at = smem_addr(sums + k * 33 + lane);
+        float part[kMaxSplits], s = 0.0f;
+#pragma unroll
+        for (uint32_t i = 0; i < kMaxSplits; ++i) part[i] = i < p.splits ? cluster_load(at, i) : 0.0f;
+#pragma unroll
+        for (uint32_t i = 0; i < kMaxSplits; ++i) s += part[i];
+        p.y[(size_t)k * p.y_stride + tile * 32 + lane] = s;
     }
+    cluster_barrier();  // nobody leaves while its sums are being read
 }
 
-template <class K>
-cudaError_t launch_pdl(K kernel, dim3 grid, uint32_t smem, cudaStream_t stream, const MoeParams& p) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(kMoeThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, p);
+// The kernels for a matrix: its type, and whether its rows are whole chunks.
+using MoeKernel = void (*)(MoeParams);
+bool whole_chunks(bool four, uint32_t cols) { return cols / 32 % (four ? 8 : 4) == 0; }
+MoeKernel inner_kernel(const MoeParams& p) {
+    if (p.gate4) return whole_chunks(true, p.hidden) ? moe_inner_kernel<true, true> : moe_inner_kernel<true, false>;
+    return whole_chunks(false, p.hidden) ? moe_inner_kernel<false, true> : moe_inner_kernel<false, false>;
+}
+MoeKernel down_kernel(const MoeParams& p) {
+    if (p.down4) return whole_chunks(true, p.inner) ? moe_down_kernel<true, true> : moe_down_kernel<true, false>;
+    return whole_chunks(false, p.inner) ? moe_down_kernel<false, true> : moe_down_kernel<false, false>;
 }
 
 size_t round_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
@@ -626,22 +794,13 @@ vx_status vx_moe_create(vx_context* ctx, const float* router, size_t experts, co
     p.down = {down->d_quants, down->d_scales};
     // Output rows in tiles of 32; few tiles share out the columns too, so that about two blocks per SM have work.
     const uint32_t tiles = p.hidden / 32;
-    p.splits = std::min(16u, std::max(1u, 2 * m->sm_count / tiles));
-    const int inner_bytes = (int)(p.gate4 ? inner_smem<true>() : inner_smem<false>());
-    const int down_bytes = (int)((p.down4 ? down_ring<true>() : down_ring<false>()) + kMoeWarps * max_tokens * 33 * 4);
+    p.splits = std::min(kMaxSplits, std::max(1u, 2 * m->sm_count / tiles));
+    p.slices = (p.hidden + kSlice - 1) / kSlice;
     int per_sm = 0;
-    if (p.gate4) {
-        VX_CUDA(cudaFuncSetAttribute(moe_inner_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, inner_bytes));
-        VX_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, moe_inner_kernel<true>, kMoeThreads, inner_bytes));
-    } else {
-        VX_CUDA(cudaFuncSetAttribute(moe_inner_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, inner_bytes));
-        VX_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, moe_inner_kernel<false>, kMoeThreads, inner_bytes));
-    }
+    VX_CUDA(cudaFuncSetAttribute(inner_kernel(p), cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kInnerSmem));
+    VX_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, inner_kernel(p), kMoeThreads, kInnerSmem));
     m->inner_grid = (uint32_t)std::max(1, per_sm) * m->sm_count;
-    const int most = (int)((p.down4 ? down_ring<true>() : down_ring<false>()) + kMoeWarps * kMaxTokens * 33 * 4);
-    if (p.down4) VX_CUDA(cudaFuncSetAttribute(moe_down_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
-    else VX_CUDA(cudaFuncSetAttribute(moe_down_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
-    (void)down_bytes;
+    VX_CUDA(cudaFuncSetAttribute(down_kernel(p), cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kDownSmem + down_sums(kMaxTokens))));
     // ---- workspace ------------------------------------------------------------------------------------------------------
     const size_t slots = max_tokens * top_k, nbh = hidden / 32, nbf = inner / 32;
     size_t at = 0;
@@ -650,32 +809,19 @@ vx_status vx_moe_create(vx_context* ctx, const float* router, size_t experts, co
         at += round_up(bytes, 256);
         return o;
     };
-    const size_t o_counters = take((1 + tiles) * 4), o_logits = take(max_tokens * experts * 4), o_xh = take(max_tokens * 2 * nbh * 64),
-                 o_xs = take(max_tokens * nbh * 4), o_hh = take(slots * 2 * nbf * 64), o_hs = take(slots * nbf * 4),
-                 o_plan = take((2 + 2 * experts) * 4), o_list = take(slots * 4), o_weights = take(slots * 4),
-                 o_part = take(p.splits > 1 ? p.splits * max_tokens * hidden * 4 : 0);
-    cudaError_t e = device_malloc(ctx, reinterpret_cast<void**>(&m->workspace), at);
+    const size_t o_logits = take(p.slices * max_tokens * experts * 4), o_xh = take(max_tokens * 2 * nbh * 64), o_xs = take(max_tokens * nbh * 8),
+                 o_hh = take(slots * 2 * nbf * 64), o_hs = take(slots * nbf * 8);
+    const cudaError_t e = device_malloc(ctx, reinterpret_cast<void**>(&m->workspace), at);
     if (e != cudaSuccess) {
         (void)cudaGetLastError();
         return fail(VX_ERR_OUT_OF_MEMORY, "allocating %zu bytes of expert-layer workspace failed: %s", at, cudaGetErrorString(e));
     }
-    e = cudaMemsetAsync(m->workspace, 0, (1 + tiles) * 4, ctx->stream);
-    if (e != cudaSuccess) {
-        (void)cudaGetLastError();
-        cudaFree(m->workspace);
-        return fail(VX_ERR_CUDA, "clearing the expert-layer counters failed: %s", cudaGetErrorString(e));
-    }
     uint8_t* w = m->workspace;
-    p.counters = reinterpret_cast<uint32_t*>(w + o_counters);
     p.logits = reinterpret_cast<float*>(w + o_logits);
     p.xh = w + o_xh;
-    p.xs = reinterpret_cast<float*>(w + o_xs);
+    p.xs = reinterpret_cast<float2*>(w + o_xs);
     p.hh = w + o_hh;
-    p.hs = reinterpret_cast<float*>(w + o_hs);
-    p.plan = reinterpret_cast<uint32_t*>(w + o_plan);
-    p.list = reinterpret_cast<uint32_t*>(w + o_list);
-    p.weights = reinterpret_cast<float*>(w + o_weights);
-    p.part = reinterpret_cast<float*>(w + o_part);
+    p.hs = reinterpret_cast<float2*>(w + o_hs);
     *out = m.release();
     return VX_OK;
 }
@@ -710,18 +856,14 @@ vx_status vx_moe_run(vx_context* ctx, const vx_moe* m, const float* x, size_t x_
     p.weights_out = weights;
     p.x_vec = ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(p.router)) & 15u) == 0 && (tokens == 1 || x_stride % 4 == 0);
     DeviceGuard guard(ctx->device);
-    const uint32_t nbh = p.hidden / 32, jobs = p.experts * ((p.tokens + 3) / 4) + p.tokens * ((nbh + 15) / 16);
-    const uint32_t route_grid = std::min((jobs + kMoeWarps - 1) / kMoeWarps, m->sm_count * 4);
-    VX_CUDA(launch_pdl(moe_route_kernel, dim3(route_grid), 0, ctx->stream, p));
+    const uint32_t jobs = p.experts * ((p.tokens + 3) / 4) * p.slices + p.tokens * ((p.hidden / 32 + 7) / 8);
+    const uint32_t route_grid = std::min((jobs + kMoeWarps - 1) / kMoeWarps, m->sm_count * 8);
+    VX_CUDA(launch_after(moe_route_kernel, dim3(route_grid), kMoeThreads, 0, ctx->stream, p));
     // as many units as there can be experts with tokens
     const uint64_t units = (uint64_t)std::min<uint64_t>(p.experts, (uint64_t)p.tokens * p.top_k) * (p.inner / 32);
     const uint32_t grid = (uint32_t)std::min<uint64_t>(units, m->inner_grid);
-    if (p.gate4) VX_CUDA(launch_pdl(moe_inner_kernel<true>, dim3(grid), inner_smem<true>(), ctx->stream, p));
-    else VX_CUDA(launch_pdl(moe_inner_kernel<false>, dim3(grid), inner_smem<false>(), ctx->stream, p));
-    const uint32_t sums = kMoeWarps * p.tokens * 33 * 4;
-    const dim3 down_grid(p.hidden / 32, p.splits);
-    if (p.down4) VX_CUDA(launch_pdl(moe_down_kernel<true>, down_grid, down_ring<true>() + sums, ctx->stream, p));
-    else VX_CUDA(launch_pdl(moe_down_kernel<false>, down_grid, down_ring<false>() + sums, ctx->stream, p));
+    VX_CUDA(launch_after(inner_kernel(p), dim3(grid), kMoeThreads, kInnerSmem, ctx->stream, p));
+    VX_CUDA(launch_after(down_kernel(p), dim3(p.hidden / 32, p.splits), kMoeThreads, kDownSmem + down_sums(p.tokens), ctx->stream, p, dim3(1, p.splits)));
     ctx->launches += 3;
     return VX_OK;
 }

@@ -15,24 +15,31 @@ from .backend import Backend, GpuBuffer, GpuPass
 from .linalg import QuantizedMatrix, _ptr_len
 
 
+_F32, _I32, _U32 = (np.dtype(t) for t in (np.float32, np.int32, np.uint32))
+_WORDS = (_I32, _U32)
+
+
 def _check_len(what: str, length: Optional[int], rows: int, stride: int, width: int) -> None:
     if length is not None and rows and (rows - 1) * stride + width > length:
         raise IndexError(f"{what} is shorter than {rows} rows")
 
 
-def _typed(what: str, t, dtype) -> tuple:
-    """Device pointer and length of t.  Where the element type is known it must have dtype's size and kind; the last
-    dimension of a view must be dense (the others' strides are the call's stride arguments)."""
-    buf = t if isinstance(t, GpuBuffer) else None
-    if hasattr(t, "as_tensor_ref"):
+def _typed(what: str, t, dtypes) -> tuple:
+    """Device pointer and length of t.  Where the element type is known it must be one of dtypes; the last dimension of a
+    view must be dense (the others' strides are the call's stride arguments)."""
+    if type(t) is GpuBuffer:                                # these calls cost as much on the host as on the device
+        if t.dtype in dtypes:
+            return t.ptr, t._len
+        buf = t
+    elif hasattr(t, "as_tensor_ref"):
         view = t.as_tensor_ref()
         buf, rank = view.raw_buffer(), view.rank()
         if rank and view.size(rank - 1) > 1 and view.stride(rank - 1) != 1:
             raise ValueError(f"{what}: the last dimension of the view must have stride 1")
-    if buf is not None:
-        want = np.dtype(dtype)
-        if buf.dtype.itemsize != want.itemsize or (buf.dtype.kind == "f") != (want.kind == "f"):
-            raise TypeError(f"{what} must hold {want.name} elements, not {buf.dtype.name}")
+    else:
+        return _ptr_len(t)
+    if buf.dtype not in dtypes:
+        raise TypeError(f"{what} must hold {dtypes[0].name} elements, not {buf.dtype.name}")
     return _ptr_len(t)
 
 
@@ -43,7 +50,7 @@ class CacheRows:
     `seqs` and `max_pages` follow from the lengths unless plain pointers are given."""
 
     def __init__(self, table, begin, start, rows: int, seqs: Optional[int] = None, max_pages: Optional[int] = None):
-        (tp, tl), (bp, bl), (sp, sl) = (_typed(n, t, np.int32) for n, t in (("table", table), ("begin", begin), ("start", start)))
+        (tp, tl), (bp, bl), (sp, sl) = (_typed(n, t, _WORDS) for n, t in (("table", table), ("begin", begin), ("start", start)))
         if seqs is None:
             if sl is None:
                 raise ValueError("seqs is needed with a plain pointer")
@@ -59,6 +66,7 @@ class CacheRows:
         self.rows, self.seqs, self.max_pages = rows, seqs, max_pages
         self._keep = (table, begin, start)
         self._c = _lib.VxKvRows(tp or None, max_pages, bp or None, sp or None, seqs, rows)
+        self._ref = C.byref(self._c)
 
 
 class QuantizedCache:
@@ -84,7 +92,7 @@ class QuantizedCache:
         stride = self.width if stride is None else stride
         if t is None:
             return None, stride
-        p, n = _typed(what, t, np.float32)
+        p, n = _typed(what, t, (_F32,))
         _check_len(what, n, rows.rows, stride, self.width)
         return p, stride
 
@@ -93,14 +101,14 @@ class QuantizedCache:
         """Quantises the rows of k and v (heads * head_dim f32 each) into their places."""
         kp, ks = self._rows_of("k", k, rows, k_stride)
         vp, vs = self._rows_of("v", v, rows, v_stride)
-        _lib.check(_lib.load().vx_kv_append((backend or self.backend)._ctx, self._h, C.byref(rows._c), kp, ks, vp, vs))
+        _lib.check(_lib.load().vx_kv_append((backend or self.backend)._ctx, self._h, rows._ref, kp, ks, vp, vs))
 
     def read(self, pass_: Optional[GpuPass], k, v, rows: CacheRows, k_stride: Optional[int] = None,
              v_stride: Optional[int] = None, backend: Optional[Backend] = None) -> None:
         """The reverse: k and / or v (None: not wanted) receive the values that the codes stand for."""
         kp, ks = self._rows_of("k", k, rows, k_stride)
         vp, vs = self._rows_of("v", v, rows, v_stride)
-        _lib.check(_lib.load().vx_kv_read((backend or self.backend)._ctx, self._h, C.byref(rows._c), kp, ks, vp, vs))
+        _lib.check(_lib.load().vx_kv_read((backend or self.backend)._ctx, self._h, rows._ref, kp, ks, vp, vs))
 
     def free(self) -> None:
         if self._h and self.backend._ctx:
@@ -148,13 +156,13 @@ class CacheAttention:
         scale defaults to 1 / sqrt(head_dim)."""
         qs = self.width if q_stride is None else q_stride
         os = self.width if out_stride is None else out_stride
-        qp, ql = _typed("q", q, np.float32)
-        op, ol = _typed("out", out, np.float32)
+        qp, ql = _typed("q", q, (_F32,))
+        op, ol = _typed("out", out, (_F32,))
         _check_len("q", ql, rows.rows, qs, self.width)
         _check_len("out", ol, rows.rows, os, self.width)
         mp, words = None, 0
         if mask is not None:
-            mp, ml = _typed("mask", mask, np.uint32)
+            mp, ml = _typed("mask", mask, _WORDS)
             if mask_words is None:
                 if ml is None:
                     raise ValueError("mask_words is needed with a plain pointer")
@@ -162,7 +170,7 @@ class CacheAttention:
             words = mask_words
             _check_len("mask", ml, rows.rows, words, words)
         s = self.cache.head_dim ** -0.5 if scale is None else scale
-        _lib.check(_lib.load().vx_kv_attention_run(backend._ctx, self._h, C.byref(rows._c), qp, qs, op, os, s, mp, words))
+        _lib.check(_lib.load().vx_kv_attention_run(backend._ctx, self._h, rows._ref, qp, qs, op, os, s, mp, words))
 
     def free(self) -> None:
         if self._h and self.backend._ctx:
@@ -186,7 +194,7 @@ class MoeLayer:
         if experts < 0 or top_k < 0 or max_tokens < 0:
             raise ValueError("experts, top_k and max_tokens must not be negative")
         self._h = None
-        rp, rl = _typed("router", router, np.float32)
+        rp, rl = _typed("router", router, (_F32,))
         if rl is not None and rl < experts * gate.cols:
             raise IndexError("router is shorter than experts * hidden")
         h = C.c_void_p()
@@ -204,16 +212,16 @@ class MoeLayer:
             raise ValueError("tokens must not be negative")
         xs = self.hidden if x_stride is None else x_stride
         ys = self.hidden if y_stride is None else y_stride
-        xp, xl = _typed("x", x, np.float32)
-        yp, yl = _typed("y", y, np.float32)
+        xp, xl = _typed("x", x, (_F32,))
+        yp, yl = _typed("y", y, (_F32,))
         _check_len("x", xl, tokens, xs, self.hidden)
         _check_len("y", yl, tokens, ys, self.hidden)
         ip = wp = None
         if ids is not None:
-            ip, n = _typed("ids", ids, np.int32)
+            ip, n = _typed("ids", ids, _WORDS)
             _check_len("ids", n, tokens, self.top_k, self.top_k)
         if weights is not None:
-            wp, n = _typed("weights", weights, np.float32)
+            wp, n = _typed("weights", weights, (_F32,))
             _check_len("weights", n, tokens, self.top_k, self.top_k)
         _lib.check(_lib.load().vx_moe_run(backend._ctx, self._h, xp, xs, yp, ys, tokens, ip, wp))
 
