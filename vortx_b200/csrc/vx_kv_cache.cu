@@ -3,10 +3,10 @@
 // Formats and arithmetic are those of vx_quantize (IEEE division, scale rounded to f16 before the codes are formed,
 // half away from zero); vortx has no counterpart.  One block of threads takes one 32-token tile of one head, keys or
 // values: eight lanes share a block of 32 values (a float4 each, the largest magnitude by three shuffles), so rows are
-// read and written as whole 128-byte lines.  A tile that the call covers completely is put together in shared memory
-// and goes out (comes in) as 16-byte vectors; the others' codes are stored where they belong one word at a time.
+// read and written as whole 128-byte lines, four of them per lane under way.  A tile that the call covers completely
+// is put together in shared memory and goes out as 16-byte vectors; the others' codes are stored where they belong one word at a time.
 // Both are bound by the f32 side of the copy: 4 bytes a value next to 1.06 (Q8_0) or 0.56 (Q4_0).
-#include <cfloat>
+#include <algorithm>
 #include <memory>
 #include <new>
 
@@ -37,79 +37,113 @@ __device__ __forceinline__ TileOf tile_of(const KvRows& r, const KvGeometry& g, 
     return o;
 }
 
-__device__ __forceinline__ uint32_t code_bits(float v, float d, bool four) {
-    float q = d != 0.0f ? roundf(__fdiv_rn(v, d)) : 0.0f;  // roundf: half away from zero
-    if (four) return (uint32_t)(int)fminf(15.0f, fmaxf(0.0f, q + 8.0f));
-    return (uint32_t)((int)fminf(127.0f, fmaxf(-127.0f, q)) + 128);
+// What the format prescribes rests on two f32 quotients, the scale's and v / d.  Products with a reciprocal are within
+// 2^-22 of them and give the same f16 scale and the same code except next to a border between two of them; only there
+// the division is made.  (With divisions throughout the kernel issued 300 instructions per four values and was bound by
+// that: 89 us for 16 x 1024 tokens of 8 heads of 128, keys and values.)
+//
+// f16(top / n).  The border between two f16 numbers is at bit 12 of an f32 mantissa.
+__device__ __forceinline__ uint16_t scale_of(float top, float n, float inv_n) {
+    float q = top * inv_n;
+    const uint32_t off = (__float_as_uint(q) & 0x1fffu) - 0x0ff8u;
+    if (off <= 16u || !(fabsf(q) >= 6.2e-5f)) q = __fdiv_rn(top, n);  // f16's small numbers have other borders
+    return __half_as_ushort(__float2half_rn(q));
+}
+// The codes of four values, offset included: round half away from zero of v / d; r is 1 / d to 2^-22.
+template <bool FOUR>
+__device__ __forceinline__ void codes_of(const float (&v)[4], float d, float r, uint32_t (&c)[4]) {
+    int n[4];
+    float off = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float x = v[i] * r, y = x + 12582912.0f;  // 1.5 2^23: the integer nearest to x in the low bits
+        n[i] = (int)(__float_as_uint(y) - 0x4b400000u);
+        off = fmaxf(off, fabsf(x - (y - 12582912.0f)));
+    }
+    if (off > 0.4999f) {  // one of them next to a tie
+#pragma unroll
+        for (int i = 0; i < 4; ++i) n[i] = (int)roundf(__fdiv_rn(v[i], d));
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] = (uint32_t)(FOUR ? min(15, max(0, n[i] + 8)) : min(127, max(-127, n[i])) + 128);
 }
 
+// Pairs (token, block) that a thread has under way at a time.
+constexpr uint32_t kBatch = 4;
+
+// p / blocks for a pair's number p < 32 blocks <= 512: the error of the rounded-up reciprocal stays below 1 / blocks.
+struct PerToken {
+    uint32_t blocks, inverse;
+    __device__ explicit PerToken(uint32_t nb) : blocks(nb), inverse((65536 + nb - 1) / nb) {}
+    __device__ uint32_t token(uint32_t p) const { return (p * inverse) >> 16; }
+};
+
 template <bool FOUR, bool VALUES>
-__device__ void append_part(const KvRows& r, const KvGeometry& g, const TileOf& o, uint8_t* dst, const float* __restrict__ src,
-                            size_t stride, uint32_t head, bool vec, uint8_t* image) {
-    const uint32_t oct = threadIdx.x / 8, j = threadIdx.x % 8, nb = g.blocks;
+__device__ __forceinline__ void append_part(const KvRows& r, const KvGeometry& g, const TileOf& o, uint8_t* dst, const float* __restrict__ src,
+                                            size_t stride, uint32_t head, bool vec, uint8_t* image) {
+    const uint32_t oct = threadIdx.x / 8, j = threadIdx.x % 8, lane = threadIdx.x % 32, nb = g.blocks;
     const bool whole = o.t0 == 0 && o.t1 == 32;
     uint8_t* to = whole ? image : dst;
-    const uint32_t scales = kv_code_bytes(FOUR, nb);
-    // the eight lanes of a block take part or stay out together
-    for (uint32_t p0 = o.t0 * nb; p0 < o.t1 * nb; p0 += kThreads / 8) {
-        const uint32_t p = p0 + oct;
-        const bool live = p < o.t1 * nb;
-        const uint32_t mask = __ballot_sync(0xffffffffu, live);
-        if (!live) continue;
-        const uint32_t token = p / nb, block = p - token * nb;
-        const uint32_t row = o.q.row0 + (o.tile * 32 + token - o.q.first);
-        const float* from = src + (size_t)row * stride + (size_t)head * nb * 32 + block * 32 + j * 4;
-        float v[4];
-        if (vec) {
-            const float4 f = __ldcs(reinterpret_cast<const float4*>(from));
-            v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
-        } else {
+    const uint32_t scales = kv_code_bytes(FOUR, nb), end = o.t1 * nb;
+    const PerToken per(nb);
+    for (uint32_t p0 = o.t0 * nb; p0 < end; p0 += kBatch * kThreads / 8) {
+        float v[kBatch][4];
 #pragma unroll
-            for (int n = 0; n < 4; ++n) v[n] = __ldcs(from + n);
-        }
-        // the element of largest magnitude, the first one on ties
-        float amax = 0.0f, signed_max = 0.0f;
-        bool bad = false;
+        for (uint32_t i = 0; i < kBatch; ++i) {
+            const uint32_t p = p0 + i * (kThreads / 8) + oct;
+            v[i][0] = v[i][1] = v[i][2] = v[i][3] = 0.0f;
+            if (p < end) {
+                const uint32_t token = per.token(p), block = p - token * nb;
+                const uint32_t row = o.q.row0 + (o.tile * 32 + token - o.q.first);
+                const float* from = src + (size_t)row * stride + (size_t)head * nb * 32 + block * 32 + j * 4;
+                if (vec) {
+                    const float4 f = __ldcs(reinterpret_cast<const float4*>(from));
+                    v[i][0] = f.x; v[i][1] = f.y; v[i][2] = f.z; v[i][3] = f.w;
+                } else {
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-            const float a = fabsf(v[n]);
-            bad |= !(a <= FLT_MAX);
-            if (a > amax) {
-                amax = a;
-                signed_max = v[n];
+                    for (int n = 0; n < 4; ++n) v[i][n] = __ldcs(from + n);
+                }
             }
         }
-        uint32_t at = j;
 #pragma unroll
-        for (int s = 1; s < 8; s *= 2) {
-            const float a = __shfl_xor_sync(mask, amax, s), m = __shfl_xor_sync(mask, signed_max, s);
-            const uint32_t i = __shfl_xor_sync(mask, at, s);
-            bad |= (bool)__shfl_xor_sync(mask, (int)bad, s);
-            if (a > amax || (a == amax && i < at)) {
-                amax = a;
-                signed_max = m;
-                at = i;
+        for (uint32_t i = 0; i < kBatch; ++i) {
+            const uint32_t p = p0 + i * (kThreads / 8) + oct, token = per.token(p), block = p - token * nb;
+            // the largest magnitude as bits: infinities and NaN come out on top
+            uint32_t mine = 0;
+#pragma unroll
+            for (int n = 0; n < 4; ++n) mine = max(mine, __float_as_uint(v[i][n]) & 0x7fffffffu);
+            uint32_t most = mine;
+#pragma unroll
+            for (int x = 1; x < 8; x *= 2) most = max(most, __shfl_xor_sync(0xffffffffu, most, x));
+            float top = __uint_as_float(most);
+            if (FOUR) {  // with its sign: the first element of that magnitude
+                float with = 0.0f;
+#pragma unroll
+                for (int n = 3; n >= 0; --n)
+                    if ((__float_as_uint(v[i][n]) & 0x7fffffffu) == most) with = v[i][n];
+                const uint32_t lanes = __ballot_sync(0xffffffffu, mine == most) >> (lane & 24u);
+                top = __shfl_sync(0xffffffffu, with, (lane & 24u) + __ffs(lanes & 0xffu) - 1);
             }
-        }
-        uint16_t dh = __half_as_ushort(__float2half_rn(FOUR ? __fdiv_rn(signed_max, 7.0f) : __fdiv_rn(amax, 127.0f)));
-        if (bad || (dh & 0x7fffu) >= 0x7c00u) dh = 0x7fffu;
-        const bool nan = dh == 0x7fffu;
-        const float d = nan ? 0.0f : __half2float(__ushort_as_half(dh));
-        uint32_t c[4];
-#pragma unroll
-        for (int n = 0; n < 4; ++n) c[n] = code_bits(nan ? 0.0f : v[n], d, FOUR);
-        if (VALUES) {
-            if (FOUR)
+            uint16_t dh = scale_of(top, FOUR ? 7.0f : 127.0f, FOUR ? 1.0f / 7.0f : 1.0f / 127.0f);
+            if ((dh & 0x7fffu) >= 0x7c00u) dh = 0x7fffu;
+            const bool zero = dh == 0x7fffu || (dh & 0x7fffu) == 0;  // no number, or nothing but zeros
+            const float d = zero ? 1.0f : __half2float(__ushort_as_half(dh)), inv = __fdividef(1.0f, d);
+            uint32_t c[4];
+            if (zero) v[i][0] = v[i][1] = v[i][2] = v[i][3] = 0.0f;
+            codes_of<FOUR>(v[i], d, inv, c);
+            uint32_t w = c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;
+            if (FOUR && !VALUES) w |= __shfl_xor_sync(0xffffffffu, w, 4) << 4;  // byte i of a Q4_0 block: values i and i + 16
+            if (p >= end) continue;
+            if (VALUES && FOUR) {
                 *reinterpret_cast<uint16_t*>(to + v_word(true, block, token, j)) = (uint16_t)(c[0] | c[1] << 4 | c[2] << 8 | c[3] << 12);
-            else
+            } else if (VALUES) {
 #pragma unroll
                 for (int n = 0; n < 4; ++n) to[v_word(false, block, token, j) + 4 * n] = (uint8_t)c[n];
-        } else {
-            uint32_t w = c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;
-            if (FOUR) w |= __shfl_xor_sync(mask, w, 4) << 4;  // byte i of a Q4_0 block: values i and i + 16
-            if (!FOUR || j < 4) *reinterpret_cast<uint32_t*>(to + k_word(FOUR, block, token, j)) = w;
+            } else if (!FOUR || j < 4) {
+                *reinterpret_cast<uint32_t*>(to + k_word(FOUR, block, token, j)) = w;
+            }
+            if (j == 0) *reinterpret_cast<uint16_t*>(to + scales + (VALUES ? v_scale(block, token) : k_scale(block, token))) = dh;
         }
-        if (j == 0) *reinterpret_cast<uint16_t*>(to + scales + (VALUES ? v_scale(block, token) : k_scale(block, token))) = dh;
     }
     if (!whole) return;
     __syncthreads();
@@ -119,89 +153,108 @@ __device__ void append_part(const KvRows& r, const KvGeometry& g, const TileOf& 
 
 __global__ void __launch_bounds__(kThreads)
 kv_append_kernel(KvRows r, KvGeometry g, const float* __restrict__ k, size_t k_stride, const float* __restrict__ v, size_t v_stride,
-                 int k_vec, int v_vec) {
+                 int k_vec, int v_vec, uint32_t heads) {
     __shared__ __align__(16) uint8_t image[kv_part_bytes(false, kMaxBlocks)];
-    const uint32_t head = blockIdx.y;
     const TileOf o = tile_of(r, g, blockIdx.x);
     if (o.t0 >= o.t1) return;
-    uint8_t* rec = kv_record(r, g, o.seq, o.tile, head);
+    const uint32_t first = blockIdx.y * heads, end = min(g.heads, first + heads);
+    uint8_t* rec = kv_record(r, g, o.seq, o.tile, first);
     if (!rec) return;
-    if (blockIdx.z == 0) {
-        if (g.k4) append_part<true, false>(r, g, o, rec, k, k_stride, head, k_vec != 0, image);
-        else append_part<false, false>(r, g, o, rec, k, k_stride, head, k_vec != 0, image);
-    } else {
-        if (g.v4) append_part<true, true>(r, g, o, rec + g.k_bytes, v, v_stride, head, v_vec != 0, image);
-        else append_part<false, true>(r, g, o, rec + g.k_bytes, v, v_stride, head, v_vec != 0, image);
+    for (uint32_t head = first; head < end; ++head, rec += g.record_bytes) {
+        if (head > first) __syncthreads();  // the last head's image has been copied
+        if (blockIdx.z == 0) {
+            if (g.k4) append_part<true, false>(r, g, o, rec, k, k_stride, head, k_vec != 0, image);
+            else append_part<false, false>(r, g, o, rec, k, k_stride, head, k_vec != 0, image);
+        } else {
+            if (g.v4) append_part<true, true>(r, g, o, rec + g.k_bytes, v, v_stride, head, v_vec != 0, image);
+            else append_part<false, true>(r, g, o, rec + g.k_bytes, v, v_stride, head, v_vec != 0, image);
+        }
     }
 }
 
 template <bool FOUR, bool VALUES>
-__device__ void read_part(const KvGeometry& g, const TileOf& o, const uint8_t* src, float* __restrict__ dst, size_t stride,
-                          uint32_t head, bool vec, uint8_t* image) {
+__device__ __forceinline__ void read_part(const KvGeometry& g, const TileOf& o, const uint8_t* src, float* __restrict__ dst, size_t stride,
+                                          uint32_t head, bool vec) {
     const uint32_t oct = threadIdx.x / 8, j = threadIdx.x % 8, nb = g.blocks;
-    const uint32_t scales = kv_code_bytes(FOUR, nb);
-    if (src && o.t1 - o.t0 >= 8) {  // most of the tile is wanted: bring it in as vectors
-        for (uint32_t i = threadIdx.x; i < kv_part_bytes(FOUR, nb) / 16; i += kThreads)
-            reinterpret_cast<uint4*>(image)[i] = reinterpret_cast<const uint4*>(src)[i];
-        __syncthreads();
-        src = image;
-    }
-    for (uint32_t p = o.t0 * nb + oct; p < o.t1 * nb; p += kThreads / 8) {
-        const uint32_t token = p / nb, block = p - token * nb;
-        const uint32_t row = o.q.row0 + (o.tile * 32 + token - o.q.first);
-        float f[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (src) {
-            const uint16_t dh = *reinterpret_cast<const uint16_t*>(src + scales + (VALUES ? v_scale(block, token) : k_scale(block, token)));
-            const float d = __half2float(__ushort_as_half(dh));
-            uint32_t w;
-            if (VALUES && FOUR) {
-                w = *reinterpret_cast<const uint16_t*>(src + v_word(true, block, token, j));
-            } else if (VALUES) {
-                const uint8_t* at = src + v_word(false, block, token, j);
-                w = at[0] | (uint32_t)at[4] << 8 | (uint32_t)at[8] << 16 | (uint32_t)at[12] << 24;
-            } else {
-                w = *reinterpret_cast<const uint32_t*>(src + k_word(FOUR, block, token, FOUR ? j % 4 : j));
-            }
+    const uint32_t scales = kv_code_bytes(FOUR, nb), end = o.t1 * nb;
+    const PerToken per(nb);
+    for (uint32_t p0 = o.t0 * nb; p0 < end; p0 += kBatch * kThreads / 8) {
+        uint32_t w[kBatch], dh[kBatch];  // straight from the record: its neighbours' words come along in the L1
 #pragma unroll
-            for (int n = 0; n < 4; ++n) {
-                int q;
-                if (!FOUR) q = (int)((w >> (8 * n)) & 255u) - 128;
-                else if (VALUES) q = (int)((w >> (4 * n)) & 15u) - 8;
-                else q = (int)((w >> (8 * n + (j < 4 ? 0 : 4))) & 15u) - 8;
-                f[n] = __fmul_rn(d, (float)q);
+        for (uint32_t i = 0; i < kBatch; ++i) {
+            const uint32_t p = p0 + i * (kThreads / 8) + oct, token = per.token(p), block = p - token * nb;
+            w[i] = FOUR ? 0x88888888u : 0x80808080u;  // zeros, for tokens without a place
+            dh[i] = 0;
+            if (src && p < end) {
+                dh[i] = *reinterpret_cast<const uint16_t*>(src + scales + (VALUES ? v_scale(block, token) : k_scale(block, token)));
+                if (VALUES && FOUR) {
+                    w[i] = *reinterpret_cast<const uint16_t*>(src + v_word(true, block, token, j));
+                } else if (VALUES) {
+                    const uint8_t* at = src + v_word(false, block, token, j);
+                    w[i] = at[0] | (uint32_t)at[4] << 8 | (uint32_t)at[8] << 16 | (uint32_t)at[12] << 24;
+                } else {
+                    w[i] = *reinterpret_cast<const uint32_t*>(src + k_word(FOUR, block, token, FOUR ? j % 4 : j));
+                }
             }
         }
-        float* to = dst + (size_t)row * stride + (size_t)head * nb * 32 + block * 32 + j * 4;
-        if (vec) {
-            __stcs(reinterpret_cast<float4*>(to), make_float4(f[0], f[1], f[2], f[3]));
-        } else {
 #pragma unroll
-            for (int n = 0; n < 4; ++n) __stcs(to + n, f[n]);
+        for (uint32_t i = 0; i < kBatch; ++i) {
+            const uint32_t p = p0 + i * (kThreads / 8) + oct, token = per.token(p), block = p - token * nb;
+            if (p >= end) continue;
+            const uint32_t row = o.q.row0 + (o.tile * 32 + token - o.q.first);
+            const float d = __half2float(__ushort_as_half((uint16_t)dh[i]));
+            float f[4];
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                const uint32_t shift = !FOUR ? 8 * n : VALUES ? 4 * n : 8 * n + (j < 4 ? 0 : 4);
+                const uint32_t u = (w[i] >> shift) & (FOUR ? 15u : 255u);
+                f[n] = __fmul_rn(d, __uint_as_float(u | 0x4b000000u) - (FOUR ? 8388616.0f : 8388736.0f));  // 2^23 + u
+            }
+            float* to = dst + (size_t)row * stride + (size_t)head * nb * 32 + block * 32 + j * 4;
+            if (vec) {
+                __stcs(reinterpret_cast<float4*>(to), make_float4(f[0], f[1], f[2], f[3]));
+            } else {
+#pragma unroll
+                for (int n = 0; n < 4; ++n) __stcs(to + n, f[n]);
+            }
         }
     }
 }
 
 __global__ void __launch_bounds__(kThreads)
-kv_read_kernel(KvRows r, KvGeometry g, float* __restrict__ k, size_t k_stride, float* __restrict__ v, size_t v_stride, int k_vec, int v_vec) {
-    __shared__ __align__(16) uint8_t image[kv_part_bytes(false, kMaxBlocks)];
-    const uint32_t head = blockIdx.y;
+kv_read_kernel(KvRows r, KvGeometry g, float* __restrict__ k, size_t k_stride, float* __restrict__ v, size_t v_stride, int k_vec, int v_vec,
+               uint32_t heads) {
     const bool values = k == nullptr || blockIdx.z == 1;
     const TileOf o = tile_of(r, g, blockIdx.x);
     if (o.t0 >= o.t1) return;
-    const uint8_t* rec = kv_record(r, g, o.seq, o.tile, head);
-    if (!values) {
-        if (g.k4) read_part<true, false>(g, o, rec, k, k_stride, head, k_vec != 0, image);
-        else read_part<false, false>(g, o, rec, k, k_stride, head, k_vec != 0, image);
-    } else {
-        if (rec) rec += g.k_bytes;
-        if (g.v4) read_part<true, true>(g, o, rec, v, v_stride, head, v_vec != 0, image);
-        else read_part<false, true>(g, o, rec, v, v_stride, head, v_vec != 0, image);
+    const uint32_t first = blockIdx.y * heads, end = min(g.heads, first + heads);
+    const uint8_t* rec = kv_record(r, g, o.seq, o.tile, first);
+    for (uint32_t head = first; head < end; ++head) {
+        const uint8_t* part = rec ? rec + (size_t)(head - first) * g.record_bytes + (values ? g.k_bytes : 0) : nullptr;
+        if (!values) {
+            if (g.k4) read_part<true, false>(g, o, part, k, k_stride, head, k_vec != 0);
+            else read_part<false, false>(g, o, part, k, k_stride, head, k_vec != 0);
+        } else {
+            if (g.v4) read_part<true, true>(g, o, part, v, v_stride, head, v_vec != 0);
+            else read_part<false, true>(g, o, part, v, v_stride, head, v_vec != 0);
+        }
     }
 }
 
 int vec_ok(const void* p, size_t stride) { return ((reinterpret_cast<uintptr_t>(p) & 15u) == 0 && stride % 4 == 0) ? 1 : 0; }
 
-dim3 tiles_grid(const KvRows& r, const KvGeometry& g, unsigned parts) { return dim3(r.rows / 32 + 2 * r.seqs, g.heads, parts); }
+// Blocks for a call: finding out whose tile it is costs a block as much as a third of a head's work, so blocks take
+// several heads where there are enough tiles to fill the GPU twice over all the same.
+struct TileLaunch {
+    dim3 grid;
+    uint32_t heads;  // of a block
+    TileLaunch(const vx_context* ctx, const KvRows& r, const KvGeometry& g, unsigned parts) {
+        const uint32_t tiles = r.rows / 32 + 2 * r.seqs;
+        const uint64_t one = (uint64_t)tiles * g.heads * parts, fill = (uint64_t)ctx->sm_count * 16;
+        heads = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(1, one / fill), g.heads);
+        grid = dim3(tiles, (g.heads + heads - 1) / heads, parts);
+    }
+};
 
 }  // namespace
 
@@ -316,8 +369,8 @@ vx_status vx_kv_append(vx_context* ctx, vx_kv_cache* cache, const vx_kv_rows* ro
     VX_REQUIRE(r.rows == 1 || (k_stride >= width && v_stride >= width), VX_ERR_INVALID_ARGUMENT,
                "vx_kv_append: rows %zu and %zu elements apart, a row has %zu", k_stride, v_stride, width);
     DeviceGuard guard(ctx->device);
-    kv_append_kernel<<<tiles_grid(r, cache->g, 2), kThreads, 0, ctx->stream>>>(r, cache->g, k, k_stride, v, v_stride, vec_ok(k, k_stride),
-                                                                              vec_ok(v, v_stride));
+    const TileLaunch l(ctx, r, cache->g, 2);
+    kv_append_kernel<<<l.grid, kThreads, 0, ctx->stream>>>(r, cache->g, k, k_stride, v, v_stride, vec_ok(k, k_stride), vec_ok(v, v_stride), l.heads);
     VX_CUDA(cudaGetLastError());
     ctx->launches++;
     return VX_OK;
@@ -334,8 +387,8 @@ vx_status vx_kv_read(vx_context* ctx, const vx_kv_cache* cache, const vx_kv_rows
     VX_REQUIRE(r.rows == 1 || ((!k || k_stride >= width) && (!v || v_stride >= width)), VX_ERR_INVALID_ARGUMENT,
                "vx_kv_read: rows %zu and %zu elements apart, a row has %zu", k_stride, v_stride, width);
     DeviceGuard guard(ctx->device);
-    kv_read_kernel<<<tiles_grid(r, cache->g, k && v ? 2 : 1), kThreads, 0, ctx->stream>>>(r, cache->g, k, k_stride, v, v_stride,
-                                                                                         vec_ok(k, k_stride), vec_ok(v, v_stride));
+    const TileLaunch l(ctx, r, cache->g, k && v ? 2 : 1);
+    kv_read_kernel<<<l.grid, kThreads, 0, ctx->stream>>>(r, cache->g, k, k_stride, v, v_stride, vec_ok(k, k_stride), vec_ok(v, v_stride), l.heads);
     VX_CUDA(cudaGetLastError());
     ctx->launches++;
     return VX_OK;

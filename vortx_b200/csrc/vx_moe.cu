@@ -46,6 +46,7 @@ struct MoeParams {
     size_t x_stride, y_stride;
     const float* router;
     uint32_t tokens, experts, top_k, hidden, inner, splits, slices;
+    uint32_t row_log;    // of the experts, rounded up to a power of two of at least 4
     int normalise, down4, x_vec, gate4;
     Matrix gate, up, down;
     float* logits;       // [slices][tokens][experts]
@@ -89,8 +90,9 @@ __device__ __forceinline__ void logits_of(const MoeParams& p, uint32_t expert, u
     }
 #pragma unroll
     for (uint32_t t = 0; t < 4; ++t) {
+        if (t >= n) break;
         const float s = warp_add(sum[t]);
-        if (t < n && lane == 0) p.logits[((size_t)slice * p.tokens + t0 + t) * p.experts + expert] = s;
+        if (lane == 0) p.logits[((size_t)slice * p.tokens + t0 + t) * p.experts + expert] = s;
     }
 }
 
@@ -104,25 +106,26 @@ __device__ __forceinline__ void split_block(float v, uint32_t lane, bool four, u
     *reinterpret_cast<__half*>(hi + at) = h;
     *reinterpret_cast<__half*>(lo + at) = l;
     const float sum = warp_add(__half2float(h) + __half2float(l));
-    if (lane == 0) *factor = make_float2((four ? 1048576.0f : 16777216.0f) / up, (four ? -8.0f : -128.0f) * sum / up);
+    const float down = __uint_as_float(0x7f000000u - __float_as_uint(up));  // 1 / up, a power of two
+    if (lane == 0) *factor = make_float2((four ? 1048576.0f : 16777216.0f) * down, (four ? -8.0f : -128.0f) * sum * down);
 }
 
 __global__ void __launch_bounds__(kMoeThreads) moe_route_kernel(MoeParams p) {
     pdl_wait();
     pdl_launch();
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nb = p.hidden / 32;
-    const uint32_t quads = (p.tokens + 3) / 4, dots = p.experts * quads * p.slices, pieces = (nb + 7) / 8;
+    const uint32_t quads = (p.tokens + 3) / 4, dots = p.experts * quads * p.slices, pieces = (nb + 3) / 4;
     for (uint32_t job = blockIdx.x * kMoeWarps + warp; job < dots + p.tokens * pieces; job += gridDim.x * kMoeWarps) {
         if (job < dots) {
             const uint32_t slice = job % p.slices, rest = job / p.slices;
             logits_of(p, rest / quads, (rest % quads) * 4, slice, lane);
         } else {
-            const uint32_t t = (job - dots) / pieces, b0 = (job - dots) % pieces * 8;
-            float v[8];
+            const uint32_t t = (job - dots) / pieces, b0 = (job - dots) % pieces * 4;
+            float v[4];
 #pragma unroll
-            for (uint32_t i = 0; i < 8; ++i) v[i] = b0 + i < nb ? p.x[(size_t)t * p.x_stride + (b0 + i) * 32 + lane] : 0.0f;
+            for (uint32_t i = 0; i < 4; ++i) v[i] = b0 + i < nb ? p.x[(size_t)t * p.x_stride + (b0 + i) * 32 + lane] : 0.0f;
 #pragma unroll
-            for (uint32_t i = 0; i < 8; ++i)
+            for (uint32_t i = 0; i < 4; ++i)
                 if (b0 + i < nb) {
                     uint8_t* hi = p.xh + ((size_t)t * 2 * nb + b0 + i) * 64;
                     split_block(v[i], lane, p.gate4 != 0, hi, hi + (size_t)nb * 64, p.xs + (size_t)t * nb + b0 + i);
@@ -140,9 +143,10 @@ struct Plan {
 };
 struct PlanScratch {
     uint32_t tokens[2][kMaxExperts];  // which tokens an expert has
+    uint32_t begin[kMaxExperts];      // of the expert's list
     uint16_t chosen[kMaxTokens * kMaxTopK];
-    uint32_t scan[2][kMoeWarps];
-    uint4 keys[1];                    // [tokens][experts, rounded up to four]
+    uint32_t scan[kMoeWarps];
+    uint4 keys[1];                    // [tokens][experts, rounded up to a power of two]
 };
 constexpr uint32_t plan_scratch(uint32_t tokens) { return sizeof(PlanScratch) + tokens * kMaxExperts * 4; }
 
@@ -157,21 +161,23 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 
 // All threads of the block; ends with a barrier.  An expert's place among a token's logits is how many are larger, or
 // equal and earlier: a thread per (token, expert) counts, which needs no rounds of finding a largest one.
-__device__ void make_plan(const MoeParams& p, Plan* plan, PlanScratch* w, bool outputs) {
-    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, quads = (p.experts + 3) / 4, row = quads * 4;
+// WEIGHTS: the softmax as well; `outputs`: it and the experts go to the caller's arrays.
+template <bool WEIGHTS>
+__device__ __forceinline__ void make_plan(const MoeParams& p, Plan* plan, PlanScratch* w, bool outputs) {
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, row = 1u << p.row_log, quads = row / 4, all = p.tokens << p.row_log;
     uint32_t* keys = reinterpret_cast<uint32_t*>(w->keys);
     w->tokens[0][tid] = w->tokens[1][tid] = 0;
-    for (uint32_t i0 = tid; i0 < p.tokens * row; i0 += 4 * kMoeThreads) {
+    for (uint32_t i0 = tid; i0 < all; i0 += 4 * kMoeThreads) {
         float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         for (uint32_t s0 = 0; s0 < p.slices; s0 += 4) {
             float part[4][4];  // sixteen loads in flight
 #pragma unroll
             for (uint32_t x = 0; x < 4; ++x) {
-                const uint32_t i = i0 + x * kMoeThreads, t = i / row, e = i - t * row;
+                const uint32_t i = i0 + x * kMoeThreads, t = i >> p.row_log, e = i & (row - 1);
+                const float* src = p.logits + ((size_t)s0 * p.tokens + t) * p.experts + e;
 #pragma unroll
-                for (uint32_t y = 0; y < 4; ++y)
-                    part[x][y] = i < p.tokens * row && e < p.experts && s0 + y < p.slices
-                                     ? __ldcg(p.logits + ((size_t)(s0 + y) * p.tokens + t) * p.experts + e) : 0.0f;
+                for (uint32_t y = 0; y < 4; ++y, src += p.tokens * p.experts)
+                    part[x][y] = i < all && e < p.experts && s0 + y < p.slices ? __ldcg(src) : 0.0f;
             }
 #pragma unroll
             for (uint32_t x = 0; x < 4; ++x)
@@ -181,17 +187,17 @@ __device__ void make_plan(const MoeParams& p, Plan* plan, PlanScratch* w, bool o
 #pragma unroll
         for (uint32_t x = 0; x < 4; ++x) {
             const uint32_t i = i0 + x * kMoeThreads;
-            if (i < p.tokens * row) keys[i] = i % row < p.experts ? order_of(v[x]) : 0u;
+            if (i < all) keys[i] = (i & (row - 1)) < p.experts ? order_of(v[x]) : 0u;
         }
     }
     __syncthreads();
-    for (uint32_t i = tid; i < p.tokens * row; i += kMoeThreads) {
-        const uint32_t t = i / row, e = i - t * row;
-        const uint32_t mine = keys[i];
+    for (uint32_t i = tid; i < all; i += kMoeThreads) {
+        const uint32_t t = i >> p.row_log, e = i & (row - 1), mine = keys[i];
+        const uint4* of = w->keys + t * quads;
         uint32_t place = 0;
 #pragma unroll 4
         for (uint32_t q = 0; q < quads; ++q) {
-            const uint4 k = w->keys[t * quads + q];
+            const uint4 k = of[q];
             place += k.x > mine || (k.x == mine && 4 * q < e);
             place += k.y > mine || (k.y == mine && 4 * q + 1 < e);
             place += k.z > mine || (k.z == mine && 4 * q + 2 < e);
@@ -199,70 +205,60 @@ __device__ void make_plan(const MoeParams& p, Plan* plan, PlanScratch* w, bool o
         }
         if (mine && place < p.top_k) {
             w->chosen[t * p.top_k + place] = (uint16_t)e;
-            atomicOr(&w->tokens[t / 32][e], 1u << (t % 32));
+            atomicOr(&w->tokens[t >> 5][e], 1u << (t & 31));
             if (outputs && p.ids_out) p.ids_out[(size_t)t * p.top_k + place] = (int32_t)e;
         }
     }
     __syncthreads();
-    for (uint32_t t = warp; t < p.tokens; t += kMoeWarps) {
-        const float mine = lane < p.top_k ? value_of(keys[t * row + w->chosen[t * p.top_k + lane]]) : 0.0f;
-        const float top = __shfl_sync(0xffffffffu, mine, 0);
-        float all = 0.0f;
-        if (p.normalise) {
-            all = lane < p.top_k ? expf(mine - top) : 0.0f;
-        } else {
-            for (uint32_t e = lane; e < p.experts; e += 32) all += expf(value_of(keys[t * row + e]) - top);
-        }
-        all = warp_add(all);
-        if (lane < p.top_k) {
-            const float f = expf(mine - top) / all;
-            plan->weight[t * p.top_k + lane] = f;
-            if (outputs && p.weights_out) p.weights_out[(size_t)t * p.top_k + lane] = f;
-        }
-    }
-    // a thread per expert
-    uint32_t low = w->tokens[0][tid], high = w->tokens[1][tid];
-    const uint32_t count = __popc(low) + __popc(high), used = count ? 1 : 0;
-    uint32_t before = count, place = used;
+    // a thread per expert: where its list begins, and its place among those that have tokens
+    const uint32_t count = __popc(w->tokens[0][tid]) + __popc(w->tokens[1][tid]), both = count | (count ? 0x10000u : 0u);
+    uint32_t before = both;
 #pragma unroll
     for (int o = 1; o < 32; o *= 2) {
-        const uint32_t a = __shfl_up_sync(0xffffffffu, before, o), b = __shfl_up_sync(0xffffffffu, place, o);
-        if (lane >= (uint32_t)o) {
-            before += a;
-            place += b;
-        }
+        const uint32_t v = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= (uint32_t)o) before += v;
     }
-    if (lane == 31) {
-        w->scan[0][warp] = before;
-        w->scan[1][warp] = place;
-    }
+    if (lane == 31) w->scan[warp] = before;
     __syncthreads();
-    uint32_t active = 0;
+    uint32_t total = 0;
+    before -= both;
 #pragma unroll
     for (uint32_t i = 0; i < kMoeWarps; ++i) {
-        if (i < warp) {
-            before += w->scan[0][i];
-            place += w->scan[1][i];
-        }
-        active += w->scan[1][i];
+        if (i < warp) before += w->scan[i];
+        total += w->scan[i];
     }
-    before -= count;
-    place -= used;
+    w->begin[tid] = before & 0xffffu;
+    if (count) {
+        plan->expert[before >> 16] = (uint16_t)tid;
+        plan->begin[before >> 16] = (uint16_t)before;
+    }
     if (tid == 0) {
-        plan->active = active;
-        plan->begin[active] = (uint16_t)(p.tokens * p.top_k);
+        plan->active = total >> 16;
+        plan->begin[total >> 16] = (uint16_t)total;
     }
-    if (used) {
-        plan->expert[place] = (uint16_t)tid;
-        plan->begin[place] = (uint16_t)before;
-        while (low | high) {
-            const uint32_t t = low ? __ffs(low) - 1 : 32 + __ffs(high) - 1;
-            if (low) low &= low - 1;
-            else high &= high - 1;
-            uint32_t j = 0;
-            while (w->chosen[t * p.top_k + j] != tid) ++j;  // the token has chosen this expert
-            plan->list[before++] = (uint16_t)(t * p.top_k + j);
+    if (WEIGHTS || outputs) {
+        for (uint32_t t = warp; t < p.tokens; t += kMoeWarps) {
+            const uint32_t* of = keys + (t << p.row_log);
+            const float mine = lane < p.top_k ? value_of(of[w->chosen[t * p.top_k + lane]]) : 0.0f;
+            const float top = __shfl_sync(0xffffffffu, mine, 0);
+            float sum = 0.0f;
+            if (p.normalise) {
+                sum = lane < p.top_k ? expf(mine - top) : 0.0f;
+            } else {
+                for (uint32_t e = lane; e < p.experts; e += 32) sum += expf(value_of(of[e]) - top);
+            }
+            sum = warp_add(sum);
+            if (lane < p.top_k) {
+                const float f = expf(mine - top) / sum;
+                plan->weight[t * p.top_k + lane] = f;
+                if (outputs && p.weights_out) p.weights_out[(size_t)t * p.top_k + lane] = f;
+            }
         }
+    }
+    __syncthreads();
+    for (uint32_t slot = tid; slot < p.tokens * p.top_k; slot += kMoeThreads) {
+        const uint32_t e = w->chosen[slot], t = slot / p.top_k, bits = w->tokens[t >> 5][e] & ((1u << (t & 31)) - 1u);
+        plan->list[w->begin[e] + __popc(bits) + (t >= 32 ? __popc(w->tokens[0][e]) : 0)] = (uint16_t)slot;
     }
     __syncthreads();
 }
@@ -468,7 +464,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_inner_kernel(MoeParams p) 
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     pdl_wait();
     pdl_launch();
-    make_plan(p, plan, reinterpret_cast<PlanScratch*>(smem), blockIdx.x == 0);
+    make_plan<false>(p, plan, reinterpret_cast<PlanScratch*>(smem), blockIdx.x == 0);
     const uint32_t nb = p.hidden / 32, chunks = Chunk<FOUR>::count(nb), tiles = p.inner / 32, nbf = tiles, units = plan->active * tiles;
     const uint32_t ring = smem_addr(smem) + warp * kStages * kStage, row_bytes = nb * (FOUR ? 16 : 32);
     float* sums = reinterpret_cast<float*>(smem + kRing);
@@ -626,7 +622,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_down_kernel(MoeParams p) {
     float* sums = reinterpret_cast<float*>(smem + kRing);  // [warps][tokens][33]
     float* mine = sums + warp * p.tokens * 33;
     // The logits are the route kernel's, which had ended before any block of the inner kernel let this one start.
-    make_plan(p, plan, reinterpret_cast<PlanScratch*>(smem), false);
+    make_plan<true>(p, plan, reinterpret_cast<PlanScratch*>(smem), false);
     for (uint32_t i = lane; i < p.tokens * 33; i += 32) mine[i] = 0.0f;
     __syncwarp();
     const uint32_t tile = blockIdx.x, split = blockIdx.y;
@@ -796,6 +792,8 @@ vx_status vx_moe_create(vx_context* ctx, const float* router, size_t experts, co
     const uint32_t tiles = p.hidden / 32;
     p.splits = std::min(kMaxSplits, std::max(1u, 2 * m->sm_count / tiles));
     p.slices = (p.hidden + kSlice - 1) / kSlice;
+    p.row_log = 2;
+    while ((1u << p.row_log) < p.experts) ++p.row_log;
     int per_sm = 0;
     VX_CUDA(cudaFuncSetAttribute(inner_kernel(p), cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kInnerSmem));
     VX_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, inner_kernel(p), kMoeThreads, kInnerSmem));
@@ -856,7 +854,7 @@ vx_status vx_moe_run(vx_context* ctx, const vx_moe* m, const float* x, size_t x_
     p.weights_out = weights;
     p.x_vec = ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(p.router)) & 15u) == 0 && (tokens == 1 || x_stride % 4 == 0);
     DeviceGuard guard(ctx->device);
-    const uint32_t jobs = p.experts * ((p.tokens + 3) / 4) * p.slices + p.tokens * ((p.hidden / 32 + 7) / 8);
+    const uint32_t jobs = p.experts * ((p.tokens + 3) / 4) * p.slices + p.tokens * ((p.hidden / 32 + 3) / 4);
     const uint32_t route_grid = std::min((jobs + kMoeWarps - 1) / kMoeWarps, m->sm_count * 8);
     VX_CUDA(launch_after(moe_route_kernel, dim3(route_grid), kMoeThreads, 0, ctx->stream, p));
     // as many units as there can be experts with tokens
