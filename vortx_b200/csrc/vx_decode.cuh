@@ -117,13 +117,14 @@ __device__ __forceinline__ float ex2(float v) {
 // Whether this block is the last of `count` that get here with this counter; what the others wrote before is then
 // visible.  The counter is zero again afterwards.
 __device__ __forceinline__ bool last_of(uint32_t* counter, uint32_t count, uint32_t* shared) {
-    __threadfence();
     __syncthreads();
-    if (threadIdx.x == 0) *shared = atomicInc(counter, count - 1);
+    if (threadIdx.x == 0) {
+        __threadfence();  // the block's writes, which the barrier has put before this
+        *shared = atomicInc(counter, count - 1);
+        __threadfence();
+    }
     __syncthreads();
-    const bool last = *shared == count - 1;
-    if (last) __threadfence();
-    return last;
+    return *shared == count - 1;
 }
 
 __device__ __forceinline__ float warp_max(float v) {

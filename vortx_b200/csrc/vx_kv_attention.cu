@@ -10,7 +10,7 @@ struct vx_kv_attention {
     const vx_context* ctx = nullptr;
     const vx_kv_cache* cache = nullptr;
     size_t heads = 0, max_seqs = 0;
-    uint32_t grid[5] = {};  // thread blocks by groups of eight rows (1, 2, 4), 0 where there is no such kernel
+    uint32_t grid[3] = {};  // thread blocks by groups of eight rows (1, 2)
     uint8_t* workspace = nullptr;
     size_t ml_offset = 0, counters_offset = 0;
 };
@@ -33,10 +33,6 @@ namespace {
 using namespace vx;
 
 bool attn_dim(size_t d) { return d == 64 || d == 96 || d == 128 || d == 256; }
-// Groups of eight rows that the kernels of a head size exist for: four keep their output in 128 registers of a thread
-// at 128 values a head, two at 256.
-uint32_t most_groups(size_t d) { return d == 64 || d == 128 ? 4 : 2; }
-
 vx_status setup(const vx_kv_cache* c, uint32_t nt, int* per_sm, uint32_t* smem) {
     const bool k4 = c->g.k4, v4 = c->g.v4;
     if (k4) return v4 ? kv_attention_setup<true, true>(c->g.blocks, nt, per_sm, smem) : kv_attention_setup<true, false>(c->g.blocks, nt, per_sm, smem);
@@ -72,7 +68,7 @@ vx_status vx_kv_attention_create(vx_context* ctx, const vx_kv_cache* cache, size
     a->heads = heads;
     a->max_seqs = max_seqs;
     size_t rows = 0, blocks = 0;
-    for (uint32_t nt = 1; nt <= most_groups(cache->head_dim); nt *= 2) {
+    for (uint32_t nt = 1; nt <= 2; ++nt) {
         int per_sm = 0;
         uint32_t smem = 0;
         const vx_status st = setup(cache, nt, &per_sm, &smem);
@@ -139,10 +135,11 @@ vx_status vx_kv_attention_run(vx_context* ctx, const vx_kv_attention* a, const v
     p.part_o = reinterpret_cast<float*>(a->workspace);
     p.part_ml = reinterpret_cast<float2*>(a->workspace + a->ml_offset);
     p.counters = reinterpret_cast<uint32_t*>(a->workspace + a->counters_offset);
-    // Rows of a sequence that share a head of keys, as the host can know them: the average.
+    // Rows of a sequence that share a head of keys, as the host can know them (the average), in groups of 8 or of 16:
+    // two groups of 8 in one block share the conversion of the codes; 32 rows at a time spilled registers (35 against
+    // 30 us for 4 x 8 drafted tokens of 32 heads over 4000).
     const uint64_t each = ((uint64_t)p.r.rows + p.r.seqs - 1) / p.r.seqs * group;
-    uint32_t nt = each <= 8 ? 1 : each <= 16 ? 2 : 4;
-    nt = std::min(nt, most_groups(a->cache->head_dim));
+    const uint32_t nt = each <= 8 ? 1 : 2;
     DeviceGuard guard(ctx->device);
     const vx_status ls = launch(a->cache, nt, a->grid[nt], ctx->stream, p);
     if (ls != VX_OK) return ls;

@@ -24,8 +24,7 @@
 
 namespace vx {
 
-constexpr int kAttnWarps = 4;
-constexpr uint32_t kAttnMinTiles = 4;   // tiles per block below which fewer blocks work
+constexpr uint32_t kAttnMinTiles = 4;   // tiles per block below which fewer blocks work: one per warp
 constexpr uint32_t kAttnJoin = 32;       // parts whose weights are in shared memory at a time
 
 struct AttnParams {
@@ -63,19 +62,36 @@ struct Shares {
     }
 };
 
-template <bool K4, bool V4, int NB, int NT>
-struct AttnShape {
+template <bool K4, bool V4, int NB, int NT, int W>
+struct AttnLayout {  // of W warps
     static constexpr uint32_t k_bytes = kv_part_bytes(K4, NB), v_bytes = kv_part_bytes(V4, NB), record = k_bytes + v_bytes;
     static constexpr uint32_t rows = 8 * NT, dim = 32 * NB;
-    static constexpr uint32_t ring = kAttnWarps * 2 * record;
-    static constexpr uint32_t joined = 2 * rows * dim * 4;  // outputs of two warps, after the loop
+    static constexpr uint32_t ring = W * 2 * record;
+    static constexpr uint32_t joined = W / 2 * rows * dim * 4;  // outputs of half the warps, after the loop
     static constexpr uint32_t tiles = ring > joined ? ring : joined;
     static constexpr uint32_t q_bytes = NB * NT * 2 * 512;
     // the weights' transposition buffer lies over the keys' codes, which have been read by then, where it fits
     static constexpr uint32_t p_warp = rows * 32 * 4;
     static constexpr bool p_over = p_warp <= kv_code_bytes(K4, NB);
-    static constexpr uint32_t p_bytes = p_over ? 0 : kAttnWarps * p_warp;
-    static constexpr uint32_t smem = tiles + q_bytes + p_bytes + rows * 4 + kAttnWarps * rows * 8 + 128;
+    static constexpr uint32_t p_bytes = p_over ? 0 : W * p_warp;
+    static constexpr uint32_t smem = tiles + q_bytes + p_bytes + rows * 4 + W * rows * 8 + 128;
+};
+
+// Twelve warps per SM, as 168 registers allow: three blocks of four where their shared memory fits, else two of six
+// (160 against 125 us for 48 drafted tokens of 32 heads over 12000); six or four in one block for the largest heads.
+constexpr bool attn_fits(uint32_t smem, uint32_t blocks) { return blocks * (smem + 1024) <= 228 * 1024; }
+template <bool K4, bool V4, int NB, int NT>
+constexpr int attn_warps() {
+    if (attn_fits(AttnLayout<K4, V4, NB, NT, 4>::smem, 3)) return 4;
+    if (attn_fits(AttnLayout<K4, V4, NB, NT, 6>::smem, 2)) return 6;
+    if (attn_fits(AttnLayout<K4, V4, NB, NT, 4>::smem, 2)) return 4;
+    return attn_fits(AttnLayout<K4, V4, NB, NT, 6>::smem, 1) ? 6 : 4;
+}
+template <bool K4, bool V4, int NB, int NT>
+struct AttnShape : AttnLayout<K4, V4, NB, NT, attn_warps<K4, V4, NB, NT>()> {
+    static constexpr int warps = attn_warps<K4, V4, NB, NT>();
+    // blocks of an SM, for the registers: 168 a thread where heads of up to 128 values take twelve warps
+    static constexpr int blocks = NB > 4 ? 1 : warps == 4 ? 3 : 2;
 };
 
 // 16-byte slot of the weights' transposition buffer: rows of eight slots, spread so that the writes (one float per
@@ -83,17 +99,17 @@ struct AttnShape {
 __device__ __forceinline__ uint32_t p_slot(uint32_t row, uint32_t slot) { return row * 8 + (slot ^ ((row ^ (row >> 1)) & 1u)); }
 
 template <bool K4, bool V4, int NB, int NT>
-__global__ void __launch_bounds__(kAttnWarps * 32, NT == 1 ? (NB <= 4 ? 3 : 2) : (NT * NB <= 8 ? 3 : 2))
+__global__ void __launch_bounds__(AttnShape<K4, V4, NB, NT>::warps * 32, AttnShape<K4, V4, NB, NT>::blocks)
 kv_attention_kernel(AttnParams p) {
     using Shape = AttnShape<K4, V4, NB, NT>;
-    constexpr uint32_t R = Shape::rows;
+    constexpr uint32_t R = Shape::rows, W = Shape::warps, kHalf = W / 2, kPerWarp = (R + W - 1) / W;
     constexpr float kNone = -INFINITY;
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t* qf = smem + Shape::tiles;
     float* pbuf = reinterpret_cast<float*>(qf + Shape::q_bytes);
     float* inv_lift = pbuf + Shape::p_bytes / 4;
     float2* ml = reinterpret_cast<float2*>(inv_lift + R);
-    uint64_t* shared64 = reinterpret_cast<uint64_t*>(ml + kAttnWarps * R);
+    uint64_t* shared64 = reinterpret_cast<uint64_t*>(ml + W * R);
 
     pdl_wait();
     pdl_launch();
@@ -106,15 +122,53 @@ kv_attention_kernel(AttnParams p) {
     uint64_t pos, hi;      // units of the sequence: where the block is, where its share ends
     uint64_t origin;       // units before the sequence
     Shares shares(0, 1);
-    {
-        const uint32_t per = (p.r.seqs + kAttnWarps * 32 - 1) / (kAttnWarps * 32);
+    auto tiles_of = [&](uint32_t s, uint64_t* items) {
+        const KvSeq q = kv_seq(p.r, p.g, s);
+        *items = seq_items(q, p.g, p.group, R);
+        return seq_tiles_of(q);
+    };
+    auto choose_step = [&](uint64_t tiles, uint64_t items) {
+        const uint64_t even = quotient(tiles + gridDim.x - 1, gridDim.x);
+        const uint64_t apart = items < gridDim.x ? quotient(tiles, gridDim.x - items) + 1 : ~0ull;  // sum ceil(tiles / apart) <= grid
+        if (apart <= even + even / 4 + kAttnMinTiles) step = max((uint32_t)apart, kAttnMinTiles);
+    };
+    // blocks that have a share of `total` units; false for the others
+    auto choose_shares = [&](uint64_t total) {
+        uint64_t blocks = step > 1 ? total : quotient(total + kAttnMinTiles - 1, kAttnMinTiles);
+        if (blocks > gridDim.x) blocks = gridDim.x;
+        if (blockIdx.x >= blocks) return false;
+        shares = Shares(total, blocks);
+        return true;
+    };
+    // Up to 32 sequences: a lane each, every warp for itself.
+    uint64_t my_items = 0;
+    const uint32_t my_tiles = p.r.seqs <= 32 && lane < p.r.seqs ? tiles_of(lane, &my_items) : 0;
+    if (p.r.seqs <= 32 && !__any_sync(0xffffffffu, my_items * my_tiles >> 26)) {
+        const uint32_t tiles = __reduce_add_sync(0xffffffffu, (uint32_t)my_items * my_tiles);
+        if (tiles == 0) return;
+        choose_step(tiles, __reduce_add_sync(0xffffffffu, my_tiles ? (uint32_t)my_items : 0u));
+        const uint32_t mine = (uint32_t)my_items * ((my_tiles + step - 1) / step);
+        uint32_t upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+            const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= (uint32_t)o) upto += v;
+        }
+        if (!choose_shares(__shfl_sync(0xffffffffu, upto, 31))) return;
+        const uint32_t lo = (uint32_t)shares.begin(blockIdx.x);
+        seq = __ffs(__ballot_sync(0xffffffffu, lo < upto)) - 1;
+        origin = __shfl_sync(0xffffffffu, upto - mine, seq);
+        pos = lo - origin;
+        hi = shares.begin(blockIdx.x + 1) - origin;
+    } else {
+        const uint32_t per = (p.r.seqs + W * 32 - 1) / (W * 32);
         const uint32_t s0 = min(p.r.seqs, tid * per), s1 = min(p.r.seqs, s0 + per);
         uint64_t tiles = 0, items = 0;
         for (uint32_t s = s0; s < s1; ++s) {
-            const KvSeq q = kv_seq(p.r, p.g, s);
-            const uint64_t i = seq_items(q, p.g, p.group, R);
-            items += i;
-            tiles += i * seq_tiles_of(q);
+            uint64_t i;
+            const uint32_t t_ = tiles_of(s, &i);
+            if (t_) items += i;
+            tiles += i * t_;
         }
 #pragma unroll
         for (int o = 16; o > 0; o /= 2) {
@@ -123,22 +177,21 @@ kv_attention_kernel(AttnParams p) {
         }
         if (lane == 0) {
             shared64[warp] = tiles;
-            shared64[kAttnWarps + warp] = items;
+            shared64[W + warp] = items;
         }
         __syncthreads();
         tiles = items = 0;
 #pragma unroll
-        for (uint32_t w = 0; w < kAttnWarps; ++w) {
+        for (uint32_t w = 0; w < W; ++w) {
             tiles += shared64[w];
-            items += shared64[kAttnWarps + w];
+            items += shared64[W + w];
         }
         if (tiles == 0) return;
-        const uint64_t even = quotient(tiles + gridDim.x - 1, gridDim.x);
-        const uint64_t apart = items < gridDim.x ? quotient(tiles, gridDim.x - items) + 1 : ~0ull;  // sum ceil(tiles / apart) <= grid
-        if (apart <= even + even / 4 + kAttnMinTiles) step = max((uint32_t)apart, kAttnMinTiles);
+        choose_step(tiles, items);
         auto units_of = [&](uint32_t s) {
-            const KvSeq q = kv_seq(p.r, p.g, s);
-            return seq_items(q, p.g, p.group, R) * ((seq_tiles_of(q) + step - 1) / step);
+            uint64_t i;
+            const uint32_t t_ = tiles_of(s, &i);
+            return i * ((t_ + step - 1) / step);
         };
         uint64_t mine = 0;
         for (uint32_t s = s0; s < s1; ++s) mine += units_of(s);
@@ -153,14 +206,11 @@ kv_attention_kernel(AttnParams p) {
         __syncthreads();
         uint64_t total = 0;
         before -= mine;
-        for (uint32_t w = 0; w < kAttnWarps; ++w) {
+        for (uint32_t w = 0; w < W; ++w) {
             if (w < warp) before += shared64[w];
             total += shared64[w];
         }
-        uint64_t blocks = step > 1 ? total : quotient(total + kAttnMinTiles - 1, kAttnMinTiles);
-        if (blocks > gridDim.x) blocks = gridDim.x;
-        if (blockIdx.x >= blocks) return;
-        shares = Shares(total, blocks);
+        if (!choose_shares(total)) return;
         const uint64_t lo = shares.begin(blockIdx.x);
         hi = shares.begin(blockIdx.x + 1);
         __syncthreads();
@@ -208,10 +258,10 @@ kv_attention_kernel(AttnParams p) {
         if (p.mask == nullptr) last_tile = min(last_tile, (sq.start + (row_first + row_count - 1) / p.group) / kTileTokens + 1);
 
         // ---- q's rows (2 NT a warp) and the first two tiles of every warp come in together -----------------------------
-        float qv[2 * NT][NB];
+        float qv[kPerWarp][NB];
 #pragma unroll
-        for (int x = 0; x < 2 * NT; ++x) {
-            const uint32_t r = warp + x * kAttnWarps, rr = row_first + r, i = rr / p.group, hq = head * p.group + (rr - i * p.group);
+        for (uint32_t x = 0; x < kPerWarp; ++x) {
+            const uint32_t r = warp + x * W, rr = row_first + r, i = rr / p.group, hq = head * p.group + (rr - i * p.group);
             const float* src = p.q + (size_t)(sq.row0 + i) * p.q_stride + (size_t)hq * Shape::dim + lane;
 #pragma unroll
             for (int b = 0; b < NB; ++b) qv[x][b] = r < row_count ? src[b * 32] : 0.0f;
@@ -220,7 +270,7 @@ kv_attention_kernel(AttnParams p) {
         uint32_t have = 0;           // bit k & 1: tile number k has a page
         uint64_t ahead = 0;          // record of this lane's tile of the next 32 of this warp, 0 if it has no page
         auto look_ahead = [&](uint32_t tile) {
-            const uint32_t x = tile + lane * kAttnWarps;
+            const uint32_t x = tile + lane * W;
             ahead = x < last_tile ? reinterpret_cast<uint64_t>(kv_record(p.r, p.g, seq, x, head)) : 0;
         };
         auto fetch = [&](uint32_t k) {  // the warp's tile number k, which `ahead` has
@@ -235,15 +285,15 @@ kv_attention_kernel(AttnParams p) {
             cp_async_commit();
             have = src ? have | 1u << (k & 1) : have & ~(1u << (k & 1));
         };
-        const uint32_t mine = mine0 < last_tile ? (last_tile - mine0 + kAttnWarps - 1) / kAttnWarps : 0;
+        const uint32_t mine = mine0 < last_tile ? (last_tile - mine0 + W - 1) / W : 0;
         look_ahead(mine0);
         fetch(0);
         fetch(1);
 
         // ---- q: scaled, lifted by a power of two per row, split into two f16 parts in B-operand order ----------------
 #pragma unroll
-        for (int x = 0; x < 2 * NT; ++x) {
-            const uint32_t r = warp + x * kAttnWarps;
+        for (uint32_t x = 0; x < kPerWarp; ++x) {
+            const uint32_t r = warp + x * W;
             float most = 0.0f;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
@@ -251,6 +301,7 @@ kv_attention_kernel(AttnParams p) {
                 most = fmaxf(most, fabsf(qv[x][b]));
             }
             const float up = lift(warp_max(most));
+            if (r >= R) break;
             if (lane == 0) inv_lift[r] = 1.0f / up;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
@@ -282,7 +333,7 @@ kv_attention_kernel(AttnParams p) {
         }
 
         for (uint32_t k = 0; k < mine; ++k) {
-            const uint32_t tile = mine0 + k * kAttnWarps;
+            const uint32_t tile = mine0 + k * W;
             cp_async_wait<1>();
             __syncwarp();
             if (have >> (k & 1) & 1) {
@@ -341,23 +392,31 @@ kv_attention_kernel(AttnParams p) {
                     }
                     const uint2 ds = lds64(rec + kv_code_bytes(K4, NB) + b * 64 + g * 8);
                     const float2 d01 = __half22float2(bits_h2(ds.x)), d23 = __half22float2(bits_h2(ds.y));
+                    // steps outside, tiles inside: neighbouring products do not wait for each other
+                    float c[2][NT][4];
+                    uint4 qh[NT], ql[NT];
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        const uint4 qh = lds128(qs + ((b * NT + n) * 2) * 512), ql = lds128(qs + ((b * NT + n) * 2 + 1) * 512);
-#pragma unroll
-                        for (int m = 0; m < 2; ++m) {
-                            float c[4];
-                            mma_f16_new(c, a[m][0], ql.x, ql.y);
-                            mma_f16(c, a[m][1], ql.z, ql.w);
-                            mma_f16(c, a[m][0], qh.x, qh.y);
-                            mma_f16(c, a[m][1], qh.z, qh.w);
-                            const float d0 = m == 0 ? d01.x : d23.x, d1 = m == 0 ? d01.y : d23.y;
-                            s[m][n][0] = fmaf(d0, c[0], s[m][n][0]);
-                            s[m][n][1] = fmaf(d0, c[1], s[m][n][1]);
-                            s[m][n][2] = fmaf(d1, c[2], s[m][n][2]);
-                            s[m][n][3] = fmaf(d1, c[3], s[m][n][3]);
-                        }
+                        qh[n] = lds128(qs + ((b * NT + n) * 2) * 512);
+                        ql[n] = lds128(qs + ((b * NT + n) * 2 + 1) * 512);
                     }
+                    auto step = [&](auto use) {
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int m = 0; m < 2; ++m) use(n, m);
+                    };
+                    step([&](int n, int m) { mma_f16_new(c[m][n], a[m][0], ql[n].x, ql[n].y); });
+                    step([&](int n, int m) { mma_f16(c[m][n], a[m][1], ql[n].z, ql[n].w); });
+                    step([&](int n, int m) { mma_f16(c[m][n], a[m][0], qh[n].x, qh[n].y); });
+                    step([&](int n, int m) { mma_f16(c[m][n], a[m][1], qh[n].z, qh[n].w); });
+                    step([&](int n, int m) {
+                        const float d0 = m == 0 ? d01.x : d23.x, d1 = m == 0 ? d01.y : d23.y;
+                        s[m][n][0] = fmaf(d0, c[m][n][0], s[m][n][0]);
+                        s[m][n][1] = fmaf(d0, c[m][n][1], s[m][n][1]);
+                        s[m][n][2] = fmaf(d1, c[m][n][2], s[m][n][2]);
+                        s[m][n][3] = fmaf(d1, c[m][n][3], s[m][n][3]);
+                    });
                 }
 #pragma unroll
                 for (int m = 0; m < 2; ++m)
@@ -488,38 +547,38 @@ kv_attention_kernel(AttnParams p) {
                                 a[x][1][3] = f16_of_bytes(w4.w, 0x4342);
                             }
                         }
+                        uint32_t hi_[NT][4], lo_[NT][4];
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) {
-                            uint32_t hi_[4], lo_[4];
+                        for (int n = 0; n < NT; ++n)
 #pragma unroll
                             for (int x = 0; x < 4; ++x) {
                                 const __half2 h = __hmul2(bits_h2(ph[n][x]), d[x]);
                                 const __half2 l = __hfma2(bits_h2(pl[n][x]), d[x], __hfma2(bits_h2(ph[n][x]), d[x], __hneg2(h)));
-                                hi_[x] = h2_bits(h);
-                                lo_[x] = h2_bits(l);
+                                hi_[n][x] = h2_bits(h);
+                                lo_[n][x] = h2_bits(l);
                                 if (decltype(some_masked)::value) {  // what is no number in a masked place stays there
                                     const uint32_t on = (ph[n][x] & 0x7fffu ? 0xffffu : 0u) | (ph[n][x] & 0x7fff0000u ? 0xffff0000u : 0u);
-                                    hi_[x] &= on;
-                                    lo_[x] &= on;
+                                    hi_[n][x] &= on;
+                                    lo_[n][x] &= on;
                                 }
                             }
-                            // The tensor cores cut their f32 sums off instead of rounding them: a tile's sum is taken from
-                            // zero and added to the output here, or the loss would grow with the number of tiles.
-                            float o[2][4];
+                        // The tensor cores cut their f32 sums off instead of rounding them: a tile's sum is taken from
+                        // zero and added to the output here, or the loss would grow with the number of tiles.
+                        float o[NT][2][4];
+                        auto step = [&](auto use) {
 #pragma unroll
-                            for (int m = 0; m < 2; ++m) {
-                                mma_f16_new(o[m], a[0][m], lo_[0], lo_[1]);
-                                mma_f16(o[m], a[1][m], lo_[2], lo_[3]);
-                            }
+                            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                            for (int x = 0; x < 2; ++x)
+                                for (int m = 0; m < 2; ++m) use(n, m);
+                        };
+                        step([&](int n, int m) { mma_f16_new(o[n][m], a[0][m], lo_[n][0], lo_[n][1]); });
+                        step([&](int n, int m) { mma_f16(o[n][m], a[1][m], lo_[n][2], lo_[n][3]); });
+                        step([&](int n, int m) { mma_f16(o[n][m], a[0][m], hi_[n][0], hi_[n][1]); });
+                        step([&](int n, int m) { mma_f16(o[n][m], a[1][m], hi_[n][2], hi_[n][3]); });
+                        step([&](int n, int m) {
 #pragma unroll
-                                for (int m = 0; m < 2; ++m) mma_f16(o[m], a[x][m], hi_[2 * x], hi_[2 * x + 1]);
-#pragma unroll
-                            for (int m = 0; m < 2; ++m)
-#pragma unroll
-                                for (int c = 0; c < 4; ++c) acc[2 * b + m][n][c] = fmaf(acc[2 * b + m][n][c], fall[n][c & 1], o[m][c]);
-                        }
+                            for (int c = 0; c < 4; ++c) acc[2 * b + m][n][c] = fmaf(acc[2 * b + m][n][c], fall[n][c & 1], o[n][m][c]);
+                        });
                     }
                 };
                 if (masked) {
@@ -530,7 +589,7 @@ kv_attention_kernel(AttnParams p) {
                 }
             }
             __syncwarp();  // the tile and the weights have been read
-            if (((k + 2) & 31) == 0) look_ahead(mine0 + (k + 2) * kAttnWarps);
+            if (((k + 2) & 31) == 0) look_ahead(mine0 + (k + 2) * W);
             fetch(k + 2);
         }
         cp_async_wait<0>();
@@ -556,7 +615,7 @@ kv_attention_kernel(AttnParams p) {
                 const uint32_t row = n * 8 + 2 * t + e;
                 float m = kNone;
 #pragma unroll
-                for (int w = 0; w < kAttnWarps; ++w) m = fmaxf(m, ml[w * R + row].x);
+                for (uint32_t w = 0; w < W; ++w) m = fmaxf(m, ml[w * R + row].x);
                 const float f = top[n][e] == kNone ? 0.0f : ex2(top[n][e] - m) * down;
 #pragma unroll
                 for (int d = 0; d < 2 * NB; ++d) {
@@ -578,9 +637,9 @@ kv_attention_kernel(AttnParams p) {
                     make_float4(acc[2 * b][n][e], acc[2 * b][n][e + 2], acc[2 * b + 1][n][e], acc[2 * b + 1][n][e + 2]);
             });
         };
-        if (warp >= 2) store(warp - 2);
+        if (warp >= kHalf) store(warp - kHalf);
         __syncthreads();
-        if (warp < 2) {
+        if (warp < kHalf) {
             each([&](int n, int e, int b, uint32_t at) {
                 const float4 f = *reinterpret_cast<const float4*>(joined + warp * R * Shape::dim + at);
                 acc[2 * b][n][e] += f.x;
@@ -602,16 +661,22 @@ kv_attention_kernel(AttnParams p) {
         };
         // a part that saw nothing is zeros, and NaN where a NaN was seen; neither is weighted
         auto weight = [&](float m, float most) { return m == kNone ? 1.0f : ex2(m - most); };
-        for (uint32_t x = tid; x < R * Shape::dim / 4; x += kAttnWarps * 32) {
+        for (uint32_t x = tid; x < R * Shape::dim / 4; x += W * 32) {
             const uint32_t row = x / (Shape::dim / 4), col = (x % (Shape::dim / 4)) * 4;
             float m = kNone, l = 0.0f;
 #pragma unroll
-            for (int w = 0; w < kAttnWarps; ++w) m = fmaxf(m, ml[w * R + row].x);
+            for (uint32_t w = 0; w < W; ++w) m = fmaxf(m, ml[w * R + row].x);
 #pragma unroll
-            for (int w = 0; w < kAttnWarps; ++w) l += ml[w * R + row].y * weight(ml[w * R + row].x, m);
-            const float4 u = *reinterpret_cast<const float4*>(joined + row * Shape::dim + col);
-            const float4 v = *reinterpret_cast<const float4*>(joined + (R + row) * Shape::dim + col);
-            const float4 o = make_float4(u.x + v.x, u.y + v.y, u.z + v.z, u.w + v.w);
+            for (uint32_t w = 0; w < W; ++w) l += ml[w * R + row].y * weight(ml[w * R + row].x, m);
+            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (uint32_t w = 0; w < kHalf; ++w) {
+                const float4 f = *reinterpret_cast<const float4*>(joined + (w * R + row) * Shape::dim + col);
+                o.x += f.x;
+                o.y += f.y;
+                o.z += f.z;
+                o.w += f.w;
+            }
             if (whole) {
                 if (row < row_count) put(row, col, o, l == 0.0f ? 0.0f : 1.0f / l);
             } else {
@@ -628,8 +693,8 @@ kv_attention_kernel(AttnParams p) {
                 float2* of_row = ml;
                 float* weights = reinterpret_cast<float*>(smem);
                 auto slot_of = [&](uint32_t c) { return (size_t)(c0 + c) * 2 + (c == 0 ? 1 : 0); };
-                constexpr uint32_t kLanes = kAttnWarps * 32 / R;  // that share a row: 4, 8 or 16 neighbours
-                {
+                constexpr uint32_t kLanes = 128 / R;  // that share a row: 8 or 16 neighbours of four warps
+                if (tid < 128) {
                     const uint32_t row = tid / kLanes, at = tid % kLanes;
                     float m = kNone, l = 0.0f;
 #pragma unroll 4
@@ -648,14 +713,14 @@ kv_attention_kernel(AttnParams p) {
                     }
                     if (at == 0) of_row[row] = make_float2(m, l == 0.0f ? 0.0f : 1.0f / l);
                 }
-                constexpr uint32_t kEach = (R * Shape::dim / 4 + kAttnWarps * 32 - 1) / (kAttnWarps * 32);
+                constexpr uint32_t kEach = (R * Shape::dim / 4 + W * 32 - 1) / (W * 32);
                 float4 o[kEach];
 #pragma unroll
                 for (uint32_t x = 0; x < kEach; ++x) o[x] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 for (uint32_t from = 0; from < parts; from += kAttnJoin) {
                     const uint32_t count = min(kAttnJoin, parts - from);
                     __syncthreads();
-                    for (uint32_t x = tid; x < count * R; x += kAttnWarps * 32)
+                    for (uint32_t x = tid; x < count * R; x += W * 32)
                         weights[x] = weight(__ldcg(&p.part_ml[slot_of(from + x / R) * R + x % R]).x, of_row[x % R].x);
                     __syncthreads();
 #pragma unroll 8
@@ -663,7 +728,7 @@ kv_attention_kernel(AttnParams p) {
                         const float4* src = reinterpret_cast<const float4*>(p.part_o + slot_of(from + c) * R * Shape::dim);
 #pragma unroll
                         for (uint32_t x = 0; x < kEach; ++x) {
-                            const uint32_t at = tid + x * kAttnWarps * 32;
+                            const uint32_t at = tid + x * W * 32;
                             if (at < R * Shape::dim / 4) {
                                 const float4 f = __ldcg(src + at);
                                 const float w = weights[c * R + at / (Shape::dim / 4)];
@@ -677,7 +742,7 @@ kv_attention_kernel(AttnParams p) {
                 }
 #pragma unroll
                 for (uint32_t x = 0; x < kEach; ++x) {
-                    const uint32_t at = tid + x * kAttnWarps * 32, row = at / (Shape::dim / 4);
+                    const uint32_t at = tid + x * W * 32, row = at / (Shape::dim / 4);
                     if (at < R * Shape::dim / 4 && row < row_count) put(row, at % (Shape::dim / 4) * 4, o[x], of_row[row].y);
                 }
             }
@@ -696,7 +761,7 @@ template <bool K4, bool V4, class F>
 bool attn_pick(uint32_t nb, uint32_t nt, F f) {
     auto go = [&](auto b, auto n) {
         constexpr int B = decltype(b)::value, N = decltype(n)::value;
-        f(kv_attention_kernel<K4, V4, B, N>, AttnShape<K4, V4, B, N>::smem);
+        f(kv_attention_kernel<K4, V4, B, N>, AttnShape<K4, V4, B, N>::smem, (uint32_t)AttnShape<K4, V4, B, N>::warps * 32);
         return true;
     };
     using std::integral_constant;
@@ -704,12 +769,10 @@ bool attn_pick(uint32_t nb, uint32_t nt, F f) {
     if (nb == B && nt == N) return go(integral_constant<int, B>{}, integral_constant<int, N>{});
     VX_ATTN_CASE(2, 1)
     VX_ATTN_CASE(2, 2)
-    VX_ATTN_CASE(2, 4)
     VX_ATTN_CASE(3, 1)
     VX_ATTN_CASE(3, 2)
     VX_ATTN_CASE(4, 1)
     VX_ATTN_CASE(4, 2)
-    VX_ATTN_CASE(4, 4)
     VX_ATTN_CASE(8, 1)
     VX_ATTN_CASE(8, 2)
 #undef VX_ATTN_CASE
@@ -720,11 +783,11 @@ bool attn_pick(uint32_t nb, uint32_t nt, F f) {
     template <>                                                                                                           \
     vx_status kv_attention_setup<K4, V4>(uint32_t nb, uint32_t nt, int* per_sm, uint32_t* smem) {                         \
         cudaError_t e = cudaSuccess;                                                                                      \
-        const bool known = attn_pick<K4, V4>(nb, nt, [&](auto kernel, uint32_t bytes) {                                   \
+        const bool known = attn_pick<K4, V4>(nb, nt, [&](auto kernel, uint32_t bytes, uint32_t threads) {                 \
             *smem = bytes;                                                                                                \
             e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);                    \
             if (e == cudaSuccess)                                                                                         \
-                e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(per_sm, kernel, kAttnWarps * 32, bytes);                \
+                e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(per_sm, kernel, (int)threads, bytes);                   \
         });                                                                                                               \
         VX_REQUIRE(known, VX_ERR_UNSUPPORTED, "attention: no kernel for heads of %u values", nb * 32);                    \
         VX_CUDA(e);                                                                                                       \
@@ -733,7 +796,7 @@ bool attn_pick(uint32_t nb, uint32_t nt, F f) {
     template <>                                                                                                           \
     vx_status kv_attention_launch<K4, V4>(uint32_t nb, uint32_t nt, uint32_t grid, cudaStream_t stream, const AttnParams& p) { \
         cudaError_t e = cudaSuccess;                                                                                      \
-        attn_pick<K4, V4>(nb, nt, [&](auto kernel, uint32_t bytes) { e = launch_after(kernel, dim3(grid), kAttnWarps * 32, bytes, stream, p); }); \
+        attn_pick<K4, V4>(nb, nt, [&](auto kernel, uint32_t bytes, uint32_t threads) { e = launch_after(kernel, dim3(grid), threads, bytes, stream, p); }); \
         VX_CUDA(e);                                                                                                       \
         return VX_OK;                                                                                                     \
     }
