@@ -151,23 +151,34 @@ __device__ __forceinline__ void append_part(const KvRows& r, const KvGeometry& g
     for (uint32_t i = threadIdx.x; i < kv_part_bytes(FOUR, nb) / 16; i += kThreads) reinterpret_cast<uint4*>(dst)[i] = im[i];
 }
 
-__global__ void __launch_bounds__(kThreads)
-kv_append_kernel(KvRows r, KvGeometry g, const float* __restrict__ k, size_t k_stride, const float* __restrict__ v, size_t v_stride,
-                 int k_vec, int v_vec, uint32_t heads) {
+struct KvAppend {
+    KvRows r;
+    KvGeometry g;
+    const float *k, *v;
+    size_t k_stride, v_stride;
+    int k_vec, v_vec;
+    uint32_t heads;  // of a block
+};
+
+__global__ void __launch_bounds__(kThreads) kv_append_kernel(KvAppend p) {
+    pdl_wait();
+    pdl_launch();
+    const KvRows& r = p.r;
+    const KvGeometry& g = p.g;
     __shared__ __align__(16) uint8_t image[kv_part_bytes(false, kMaxBlocks)];
     const TileOf o = tile_of(r, g, blockIdx.x);
     if (o.t0 >= o.t1) return;
-    const uint32_t first = blockIdx.y * heads, end = min(g.heads, first + heads);
+    const uint32_t first = blockIdx.y * p.heads, end = min(g.heads, first + p.heads);
     uint8_t* rec = kv_record(r, g, o.seq, o.tile, first);
     if (!rec) return;
     for (uint32_t head = first; head < end; ++head, rec += g.record_bytes) {
         if (head > first) __syncthreads();  // the last head's image has been copied
         if (blockIdx.z == 0) {
-            if (g.k4) append_part<true, false>(r, g, o, rec, k, k_stride, head, k_vec != 0, image);
-            else append_part<false, false>(r, g, o, rec, k, k_stride, head, k_vec != 0, image);
+            if (g.k4) append_part<true, false>(r, g, o, rec, p.k, p.k_stride, head, p.k_vec != 0, image);
+            else append_part<false, false>(r, g, o, rec, p.k, p.k_stride, head, p.k_vec != 0, image);
         } else {
-            if (g.v4) append_part<true, true>(r, g, o, rec + g.k_bytes, v, v_stride, head, v_vec != 0, image);
-            else append_part<false, true>(r, g, o, rec + g.k_bytes, v, v_stride, head, v_vec != 0, image);
+            if (g.v4) append_part<true, true>(r, g, o, rec + g.k_bytes, p.v, p.v_stride, head, p.v_vec != 0, image);
+            else append_part<false, true>(r, g, o, rec + g.k_bytes, p.v, p.v_stride, head, p.v_vec != 0, image);
         }
     }
 }
@@ -221,22 +232,33 @@ __device__ __forceinline__ void read_part(const KvGeometry& g, const TileOf& o, 
     }
 }
 
-__global__ void __launch_bounds__(kThreads)
-kv_read_kernel(KvRows r, KvGeometry g, float* __restrict__ k, size_t k_stride, float* __restrict__ v, size_t v_stride, int k_vec, int v_vec,
-               uint32_t heads) {
-    const bool values = k == nullptr || blockIdx.z == 1;
+struct KvRead {
+    KvRows r;
+    KvGeometry g;
+    float *k, *v;
+    size_t k_stride, v_stride;
+    int k_vec, v_vec;
+    uint32_t heads;
+};
+
+__global__ void __launch_bounds__(kThreads) kv_read_kernel(KvRead p) {
+    pdl_wait();
+    pdl_launch();
+    const KvRows& r = p.r;
+    const KvGeometry& g = p.g;
+    const bool values = p.k == nullptr || blockIdx.z == 1;
     const TileOf o = tile_of(r, g, blockIdx.x);
     if (o.t0 >= o.t1) return;
-    const uint32_t first = blockIdx.y * heads, end = min(g.heads, first + heads);
+    const uint32_t first = blockIdx.y * p.heads, end = min(g.heads, first + p.heads);
     const uint8_t* rec = kv_record(r, g, o.seq, o.tile, first);
     for (uint32_t head = first; head < end; ++head) {
         const uint8_t* part = rec ? rec + (size_t)(head - first) * g.record_bytes + (values ? g.k_bytes : 0) : nullptr;
         if (!values) {
-            if (g.k4) read_part<true, false>(g, o, part, k, k_stride, head, k_vec != 0);
-            else read_part<false, false>(g, o, part, k, k_stride, head, k_vec != 0);
+            if (g.k4) read_part<true, false>(g, o, part, p.k, p.k_stride, head, p.k_vec != 0);
+            else read_part<false, false>(g, o, part, p.k, p.k_stride, head, p.k_vec != 0);
         } else {
-            if (g.v4) read_part<true, true>(g, o, part, v, v_stride, head, v_vec != 0);
-            else read_part<false, true>(g, o, part, v, v_stride, head, v_vec != 0);
+            if (g.v4) read_part<true, true>(g, o, part, p.v, p.v_stride, head, p.v_vec != 0);
+            else read_part<false, true>(g, o, part, p.v, p.v_stride, head, p.v_vec != 0);
         }
     }
 }
@@ -370,8 +392,8 @@ vx_status vx_kv_append(vx_context* ctx, vx_kv_cache* cache, const vx_kv_rows* ro
                "vx_kv_append: rows %zu and %zu elements apart, a row has %zu", k_stride, v_stride, width);
     DeviceGuard guard(ctx->device);
     const TileLaunch l(ctx, r, cache->g, 2);
-    kv_append_kernel<<<l.grid, kThreads, 0, ctx->stream>>>(r, cache->g, k, k_stride, v, v_stride, vec_ok(k, k_stride), vec_ok(v, v_stride), l.heads);
-    VX_CUDA(cudaGetLastError());
+    const KvAppend p{r, cache->g, k, v, k_stride, v_stride, vec_ok(k, k_stride), vec_ok(v, v_stride), l.heads};
+    VX_CUDA(launch_after(kv_append_kernel, l.grid, kThreads, 0, ctx->stream, p));
     ctx->launches++;
     return VX_OK;
 }
@@ -388,8 +410,8 @@ vx_status vx_kv_read(vx_context* ctx, const vx_kv_cache* cache, const vx_kv_rows
                "vx_kv_read: rows %zu and %zu elements apart, a row has %zu", k_stride, v_stride, width);
     DeviceGuard guard(ctx->device);
     const TileLaunch l(ctx, r, cache->g, k && v ? 2 : 1);
-    kv_read_kernel<<<l.grid, kThreads, 0, ctx->stream>>>(r, cache->g, k, k_stride, v, v_stride, vec_ok(k, k_stride), vec_ok(v, v_stride), l.heads);
-    VX_CUDA(cudaGetLastError());
+    const KvRead p{r, cache->g, k, v, k_stride, v_stride, vec_ok(k, k_stride), vec_ok(v, v_stride), l.heads};
+    VX_CUDA(launch_after(kv_read_kernel, l.grid, kThreads, 0, ctx->stream, p));
     ctx->launches++;
     return VX_OK;
 }
