@@ -46,7 +46,7 @@ struct AttnParams {
 __device__ __forceinline__ uint64_t seq_items(const KvSeq& q, const KvGeometry& g, uint32_t group, uint32_t rows_per_item) {
     return (uint64_t)g.heads * (((uint64_t)q.n * group + rows_per_item - 1) / rows_per_item);
 }
-__device__ __forceinline__ uint32_t seq_tiles_of(const KvSeq& q) { return (q.end + kTileTokens - 1) / kTileTokens; }
+__device__ __forceinline__ uint32_t seq_tiles_of(const KvSeq& q, uint32_t tokens) { return (q.end + tokens - 1) / tokens; }
 // a / b; most often both fit 32 bits, and a 64-bit division is a call.
 __device__ __forceinline__ uint64_t quotient(uint64_t a, uint64_t b) {
     return ((a | b) >> 32) == 0 ? (uint32_t)a / (uint32_t)b : a / b;
@@ -61,6 +61,252 @@ struct Shares {
         return (uint32_t)(tile < large ? quotient(tile, each + 1) : more + quotient(tile - large, each));
     }
 };
+
+// A block's share: of units of `step` tiles of an item (sequence, head, group of rows).  One unit per block where that
+// leaves the blocks nearly equal (few items next to the grid), else the same number of tiles, whichever items they are
+// of.
+struct Share {
+    uint32_t seq = 0, step = 1;
+    uint64_t pos = 0, hi = 0;  // units of the sequence: where the block is, where its share ends
+    uint64_t origin = 0;       // units before the sequence
+    Shares shares;
+    __device__ explicit Share(const AttnParams&) : shares(0, 1) {}
+
+    // All threads of the block (W warps); items have R rows, tiles TT tokens.  False: nothing to do.
+    template <uint32_t R, uint32_t W, uint32_t TT>
+    __device__ __forceinline__ bool find(const AttnParams& p, uint64_t* shared64) {
+        const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+        auto tiles_of = [&](uint32_t s, uint64_t* items) {
+            const KvSeq q = kv_seq(p.r, p.g, s);
+            *items = seq_items(q, p.g, p.group, R);
+            return seq_tiles_of(q, TT);
+        };
+        auto choose_step = [&](uint64_t tiles, uint64_t items) {
+            const uint64_t even = quotient(tiles + gridDim.x - 1, gridDim.x);
+            const uint64_t apart = items < gridDim.x ? quotient(tiles, gridDim.x - items) + 1 : ~0ull;  // sum ceil(tiles / apart) <= grid
+            if (apart <= even + even / 4 + kAttnMinTiles) step = max((uint32_t)apart, kAttnMinTiles);
+        };
+        // blocks that have a share of `total` units; false for the others
+        auto choose_shares = [&](uint64_t total) {
+            uint64_t blocks = step > 1 ? total : quotient(total + kAttnMinTiles - 1, kAttnMinTiles);
+            if (blocks > gridDim.x) blocks = gridDim.x;
+            if (blockIdx.x >= blocks) return false;
+            shares = Shares(total, blocks);
+            return true;
+        };
+        // Up to 32 sequences: a lane each, every warp for itself.
+        uint64_t my_items = 0;
+        const uint32_t my_tiles = p.r.seqs <= 32 && lane < p.r.seqs ? tiles_of(lane, &my_items) : 0;
+        if (p.r.seqs <= 32 && !__any_sync(0xffffffffu, my_items * my_tiles >> 26)) {
+            const uint32_t tiles = __reduce_add_sync(0xffffffffu, (uint32_t)my_items * my_tiles);
+            if (tiles == 0) return false;
+            choose_step(tiles, __reduce_add_sync(0xffffffffu, my_tiles ? (uint32_t)my_items : 0u));
+            const uint32_t mine = (uint32_t)my_items * ((my_tiles + step - 1) / step);
+            uint32_t upto = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o *= 2) {
+                const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= (uint32_t)o) upto += v;
+            }
+            if (!choose_shares(__shfl_sync(0xffffffffu, upto, 31))) return false;
+            const uint32_t lo = (uint32_t)shares.begin(blockIdx.x);
+            seq = __ffs(__ballot_sync(0xffffffffu, lo < upto)) - 1;
+            origin = __shfl_sync(0xffffffffu, upto - mine, seq);
+            pos = lo - origin;
+            hi = shares.begin(blockIdx.x + 1) - origin;
+        } else {
+            const uint32_t per = (p.r.seqs + W * 32 - 1) / (W * 32);
+            const uint32_t s0 = min(p.r.seqs, tid * per), s1 = min(p.r.seqs, s0 + per);
+            uint64_t tiles = 0, items = 0;
+            for (uint32_t s = s0; s < s1; ++s) {
+                uint64_t i;
+                const uint32_t t_ = tiles_of(s, &i);
+                if (t_) items += i;
+                tiles += i * t_;
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o /= 2) {
+                tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
+                items += __shfl_xor_sync(0xffffffffu, items, o);
+            }
+            if (lane == 0) {
+                shared64[warp] = tiles;
+                shared64[W + warp] = items;
+            }
+            __syncthreads();
+            tiles = items = 0;
+#pragma unroll
+            for (uint32_t w = 0; w < W; ++w) {
+                tiles += shared64[w];
+                items += shared64[W + w];
+            }
+            if (tiles == 0) return false;
+            choose_step(tiles, items);
+            auto units_of = [&](uint32_t s) {
+                uint64_t i;
+                const uint32_t t_ = tiles_of(s, &i);
+                return i * ((t_ + step - 1) / step);
+            };
+            uint64_t mine = 0;
+            for (uint32_t s = s0; s < s1; ++s) mine += units_of(s);
+            uint64_t before = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o *= 2) {
+                const uint64_t v = __shfl_up_sync(0xffffffffu, before, o);
+                if (lane >= (uint32_t)o) before += v;
+            }
+            __syncthreads();
+            if (lane == 31) shared64[warp] = before;
+            __syncthreads();
+            uint64_t total = 0;
+            before -= mine;
+            for (uint32_t w = 0; w < W; ++w) {
+                if (w < warp) before += shared64[w];
+                total += shared64[w];
+            }
+            if (!choose_shares(total)) return false;
+            const uint64_t lo = shares.begin(blockIdx.x);
+            hi = shares.begin(blockIdx.x + 1);
+            __syncthreads();
+            if (before <= lo && lo < before + mine) {  // one thread of the block
+                uint64_t at = before;
+                uint32_t s = s0;
+                for (;; ++s) {
+                    const uint64_t w = units_of(s);
+                    if (lo < at + w) break;
+                    at += w;
+                }
+                shared64[0] = s;
+                shared64[1] = at;
+            }
+            __syncthreads();
+            seq = (uint32_t)shared64[0];
+            origin = shared64[1];
+            pos = lo - origin;
+            hi -= origin;
+        }
+        return true;
+    }
+};
+
+// What a block does next: tiles [tile0, tile1) of a head of a sequence for R rows from row_first on.
+struct Segment {
+    KvSeq sq;
+    uint32_t seq, head, row_first, row_count, tile0, tile1, seq_tiles, parts, c0, slot;
+    bool whole;  // else one of `parts` parts, of blocks c0 ..
+};
+template <uint32_t R, uint32_t TT>
+__device__ __forceinline__ bool next_segment(const AttnParams& p, Share& at, Segment& s) {
+    while (at.pos < at.hi) {
+        s.sq = kv_seq(p.r, p.g, at.seq);
+        s.seq_tiles = seq_tiles_of(s.sq, TT);
+        const uint32_t units = (s.seq_tiles + at.step - 1) / at.step;
+        const uint64_t work = seq_items(s.sq, p.g, p.group, R) * units;
+        if (at.pos >= work) {  // on to the next sequence
+            at.pos -= work;
+            at.hi -= work;
+            at.origin += work;
+            ++at.seq;
+            continue;
+        }
+        s.seq = at.seq;
+        const uint32_t groups = (uint32_t)(((uint64_t)s.sq.n * p.group + R - 1) / R);
+        const uint32_t item = (uint32_t)quotient(at.pos, units), unit0 = (uint32_t)(at.pos - (uint64_t)item * units);
+        s.head = item / groups;
+        s.row_first = (item - s.head * groups) * R;
+        s.row_count = min(R, s.sq.n * p.group - s.row_first);
+        const uint32_t count = at.hi - at.pos < units - unit0 ? (uint32_t)(at.hi - at.pos) : units - unit0;
+        s.tile0 = unit0 * at.step;
+        s.tile1 = min(s.seq_tiles, (unit0 + count) * at.step);
+        s.whole = count == units;
+        s.slot = blockIdx.x * 2 + (unit0 == 0 ? 1 : 0);
+        s.parts = 1;
+        s.c0 = 0;
+        if (!s.whole) {  // the first block's second slot, the others' first
+            const uint64_t first = at.origin + (uint64_t)item * units;
+            s.c0 = at.shares.block_of(first);
+            s.parts = at.shares.block_of(first + units - 1) - s.c0 + 1;
+        }
+        at.pos += count;
+        return true;
+    }
+    return false;
+}
+
+// Four neighbouring values of a row of the result.
+__device__ __forceinline__ void put_row(const AttnParams& p, const Segment& s, uint32_t dim, uint32_t row, uint32_t col, float4 o, float n) {
+    const uint32_t rr = s.row_first + row, i = rr / p.group;
+    float* dst = p.out + (size_t)(s.sq.row0 + i) * p.out_stride + (size_t)(s.head * p.group + (rr - i * p.group)) * dim + col;
+    dst[0] = o.x * n;
+    dst[1] = o.y * n;
+    dst[2] = o.z * n;
+    dst[3] = o.w * n;
+}
+// A part that saw nothing is zeros, and NaN where a NaN was seen; neither is weighted.
+__device__ __forceinline__ float part_weight(float m, float most) { return m == -INFINITY ? 1.0f : ex2(m - most); }
+
+// The last block of a split (sequence, head, rows) joins the parts, in their order.  of_row: R pairs, weights: kAttnJoin R
+// floats of shared memory.
+template <uint32_t R, uint32_t DIM, uint32_t THREADS>
+__device__ __forceinline__ void join_parts(const AttnParams& p, const Segment& s, float2* of_row, float* weights) {
+    const uint32_t tid = threadIdx.x;
+    auto slot_of = [&](uint32_t c) { return (size_t)(s.c0 + c) * 2 + (c == 0 ? 1 : 0); };
+    constexpr uint32_t kLanes = 128 / R;  // that share a row: neighbours of the first four warps
+    if (tid < 128) {
+        const uint32_t row = tid / kLanes, at = tid % kLanes;
+        float m = -INFINITY, l = 0.0f;
+#pragma unroll 4
+        for (uint32_t c = at; c < s.parts; c += kLanes) {
+            const float2 f = __ldcg(&p.part_ml[slot_of(c) * R + row]);
+            const float now = fmaxf(m, f.x);
+            l = (m == -INFINITY ? l : l * ex2(m - now)) + f.y * part_weight(f.x, now);
+            m = now;
+        }
+#pragma unroll
+        for (uint32_t o = 1; o < kLanes; o *= 2) {
+            const float m2 = __shfl_xor_sync(0xffffffffu, m, o), l2 = __shfl_xor_sync(0xffffffffu, l, o);
+            const float now = fmaxf(m, m2);
+            l = l * part_weight(m, now) + l2 * part_weight(m2, now);
+            m = now;
+        }
+        if (at == 0) of_row[row] = make_float2(m, l == 0.0f ? 0.0f : 1.0f / l);
+    }
+    // so many rows at a time that a thread has at most four pieces of them
+    constexpr uint32_t kRows = R * DIM <= 16 * THREADS ? R : 16 * THREADS / DIM, kEach = (kRows * DIM / 4 + THREADS - 1) / THREADS;
+    for (uint32_t r0 = 0; r0 < R; r0 += kRows) {
+        float4 o[kEach];
+#pragma unroll
+        for (uint32_t x = 0; x < kEach; ++x) o[x] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (uint32_t from = 0; from < s.parts; from += kAttnJoin) {
+            const uint32_t count = min(kAttnJoin, s.parts - from);
+            __syncthreads();
+            for (uint32_t x = tid; x < count * kRows; x += THREADS)
+                weights[x] = part_weight(__ldcg(&p.part_ml[slot_of(from + x / kRows) * R + r0 + x % kRows]).x, of_row[r0 + x % kRows].x);
+            __syncthreads();
+#pragma unroll 8
+            for (uint32_t c = 0; c < count; ++c) {
+                const float4* src = reinterpret_cast<const float4*>(p.part_o + (slot_of(from + c) * R + r0) * DIM);
+#pragma unroll
+                for (uint32_t x = 0; x < kEach; ++x) {
+                    const uint32_t at = tid + x * THREADS;
+                    if (at < kRows * DIM / 4) {
+                        const float4 f = __ldcg(src + at);
+                        const float w = weights[c * kRows + at / (DIM / 4)];
+                        o[x].x = fmaf(w, f.x, o[x].x);
+                        o[x].y = fmaf(w, f.y, o[x].y);
+                        o[x].z = fmaf(w, f.z, o[x].z);
+                        o[x].w = fmaf(w, f.w, o[x].w);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (uint32_t x = 0; x < kEach; ++x) {
+            const uint32_t at = tid + x * THREADS, row = r0 + at / (DIM / 4);
+            if (at < kRows * DIM / 4 && row < s.row_count) put_row(p, s, DIM, row, at % (DIM / 4) * 4, o[x], of_row[row].y);
+        }
+    }
+}
 
 template <bool K4, bool V4, int NB, int NT, int W>
 struct AttnLayout {  // of W warps
@@ -115,144 +361,15 @@ kv_attention_kernel(AttnParams p) {
     pdl_launch();
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
 
-    // ---- this block's share: of units of `step` tiles of an item (sequence, head, group of rows) -------------------
-    // One unit per block where that leaves the blocks nearly equal (few items next to the grid), else the same number
-    // of tiles, whichever items they are of.
-    uint32_t seq, step = 1;
-    uint64_t pos, hi;      // units of the sequence: where the block is, where its share ends
-    uint64_t origin;       // units before the sequence
-    Shares shares(0, 1);
-    auto tiles_of = [&](uint32_t s, uint64_t* items) {
-        const KvSeq q = kv_seq(p.r, p.g, s);
-        *items = seq_items(q, p.g, p.group, R);
-        return seq_tiles_of(q);
-    };
-    auto choose_step = [&](uint64_t tiles, uint64_t items) {
-        const uint64_t even = quotient(tiles + gridDim.x - 1, gridDim.x);
-        const uint64_t apart = items < gridDim.x ? quotient(tiles, gridDim.x - items) + 1 : ~0ull;  // sum ceil(tiles / apart) <= grid
-        if (apart <= even + even / 4 + kAttnMinTiles) step = max((uint32_t)apart, kAttnMinTiles);
-    };
-    // blocks that have a share of `total` units; false for the others
-    auto choose_shares = [&](uint64_t total) {
-        uint64_t blocks = step > 1 ? total : quotient(total + kAttnMinTiles - 1, kAttnMinTiles);
-        if (blocks > gridDim.x) blocks = gridDim.x;
-        if (blockIdx.x >= blocks) return false;
-        shares = Shares(total, blocks);
-        return true;
-    };
-    // Up to 32 sequences: a lane each, every warp for itself.
-    uint64_t my_items = 0;
-    const uint32_t my_tiles = p.r.seqs <= 32 && lane < p.r.seqs ? tiles_of(lane, &my_items) : 0;
-    if (p.r.seqs <= 32 && !__any_sync(0xffffffffu, my_items * my_tiles >> 26)) {
-        const uint32_t tiles = __reduce_add_sync(0xffffffffu, (uint32_t)my_items * my_tiles);
-        if (tiles == 0) return;
-        choose_step(tiles, __reduce_add_sync(0xffffffffu, my_tiles ? (uint32_t)my_items : 0u));
-        const uint32_t mine = (uint32_t)my_items * ((my_tiles + step - 1) / step);
-        uint32_t upto = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o *= 2) {
-            const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= (uint32_t)o) upto += v;
-        }
-        if (!choose_shares(__shfl_sync(0xffffffffu, upto, 31))) return;
-        const uint32_t lo = (uint32_t)shares.begin(blockIdx.x);
-        seq = __ffs(__ballot_sync(0xffffffffu, lo < upto)) - 1;
-        origin = __shfl_sync(0xffffffffu, upto - mine, seq);
-        pos = lo - origin;
-        hi = shares.begin(blockIdx.x + 1) - origin;
-    } else {
-        const uint32_t per = (p.r.seqs + W * 32 - 1) / (W * 32);
-        const uint32_t s0 = min(p.r.seqs, tid * per), s1 = min(p.r.seqs, s0 + per);
-        uint64_t tiles = 0, items = 0;
-        for (uint32_t s = s0; s < s1; ++s) {
-            uint64_t i;
-            const uint32_t t_ = tiles_of(s, &i);
-            if (t_) items += i;
-            tiles += i * t_;
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o /= 2) {
-            tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
-            items += __shfl_xor_sync(0xffffffffu, items, o);
-        }
-        if (lane == 0) {
-            shared64[warp] = tiles;
-            shared64[W + warp] = items;
-        }
-        __syncthreads();
-        tiles = items = 0;
-#pragma unroll
-        for (uint32_t w = 0; w < W; ++w) {
-            tiles += shared64[w];
-            items += shared64[W + w];
-        }
-        if (tiles == 0) return;
-        choose_step(tiles, items);
-        auto units_of = [&](uint32_t s) {
-            uint64_t i;
-            const uint32_t t_ = tiles_of(s, &i);
-            return i * ((t_ + step - 1) / step);
-        };
-        uint64_t mine = 0;
-        for (uint32_t s = s0; s < s1; ++s) mine += units_of(s);
-        uint64_t before = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o *= 2) {
-            const uint64_t v = __shfl_up_sync(0xffffffffu, before, o);
-            if (lane >= (uint32_t)o) before += v;
-        }
-        __syncthreads();
-        if (lane == 31) shared64[warp] = before;
-        __syncthreads();
-        uint64_t total = 0;
-        before -= mine;
-        for (uint32_t w = 0; w < W; ++w) {
-            if (w < warp) before += shared64[w];
-            total += shared64[w];
-        }
-        if (!choose_shares(total)) return;
-        const uint64_t lo = shares.begin(blockIdx.x);
-        hi = shares.begin(blockIdx.x + 1);
-        __syncthreads();
-        if (before <= lo && lo < before + mine) {  // one thread of the block
-            uint64_t at = before;
-            uint32_t s = s0;
-            for (;; ++s) {
-                const uint64_t w = units_of(s);
-                if (lo < at + w) break;
-                at += w;
-            }
-            shared64[0] = s;
-            shared64[1] = at;
-        }
-        __syncthreads();
-        seq = (uint32_t)shared64[0];
-        origin = shared64[1];
-        pos = lo - origin;
-        hi -= origin;
-    }
+    Share at(p);
+    if (!at.template find<R, W, kTileTokens>(p, shared64)) return;
 
     const uint32_t ring = smem_addr(smem) + warp * 2 * Shape::record;
 
-    while (pos < hi) {
-        const KvSeq sq = kv_seq(p.r, p.g, seq);
-        const uint32_t seq_tiles = seq_tiles_of(sq), units = (seq_tiles + step - 1) / step;
-        const uint64_t work = seq_items(sq, p.g, p.group, R) * units;
-        if (pos >= work) {  // on to the next sequence
-            pos -= work;
-            hi -= work;
-            origin += work;
-            ++seq;
-            continue;
-        }
-        const uint32_t groups = (uint32_t)(((uint64_t)sq.n * p.group + R - 1) / R);
-        const uint32_t item = (uint32_t)quotient(pos, units), unit0 = (uint32_t)(pos - (uint64_t)item * units);
-        const uint32_t head = item / groups, rt = item - head * groups;
-        const uint32_t count = hi - pos < units - unit0 ? (uint32_t)(hi - pos) : units - unit0;
-        const uint32_t tile0 = unit0 * step, tile1 = min(seq_tiles, (unit0 + count) * step);
-        const bool whole = count == units;
-        pos += count;
-        const uint32_t row_first = rt * R, row_count = min(R, sq.n * p.group - row_first);
+    Segment seg;
+    while (next_segment<R, kTileTokens>(p, at, seg)) {
+        const KvSeq& sq = seg.sq;
+        const uint32_t seq = seg.seq, head = seg.head, row_first = seg.row_first, row_count = seg.row_count, tile0 = seg.tile0, tile1 = seg.tile1;
         // with no mask, nothing is attended to behind the last row's own token
         uint32_t last_tile = tile1;
         if (p.mask == nullptr) last_tile = min(last_tile, (sq.start + (row_first + row_count - 1) / p.group) / kTileTokens + 1);
@@ -650,24 +767,13 @@ kv_attention_kernel(AttnParams p) {
             store(warp);
         }
         __syncthreads();
-        const uint32_t slot = blockIdx.x * 2 + (tile0 == 0 ? 1 : 0);
-        auto put = [&](uint32_t row, uint32_t col, float4 o, float n) {
-            const uint32_t rr = row_first + row, i = rr / p.group;
-            float* dst = p.out + (size_t)(sq.row0 + i) * p.out_stride + (size_t)(head * p.group + (rr - i * p.group)) * Shape::dim + col;
-            dst[0] = o.x * n;
-            dst[1] = o.y * n;
-            dst[2] = o.z * n;
-            dst[3] = o.w * n;
-        };
-        // a part that saw nothing is zeros, and NaN where a NaN was seen; neither is weighted
-        auto weight = [&](float m, float most) { return m == kNone ? 1.0f : ex2(m - most); };
         for (uint32_t x = tid; x < R * Shape::dim / 4; x += W * 32) {
             const uint32_t row = x / (Shape::dim / 4), col = (x % (Shape::dim / 4)) * 4;
             float m = kNone, l = 0.0f;
 #pragma unroll
             for (uint32_t w = 0; w < W; ++w) m = fmaxf(m, ml[w * R + row].x);
 #pragma unroll
-            for (uint32_t w = 0; w < W; ++w) l += ml[w * R + row].y * weight(ml[w * R + row].x, m);
+            for (uint32_t w = 0; w < W; ++w) l += ml[w * R + row].y * part_weight(ml[w * R + row].x, m);
             float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
             for (uint32_t w = 0; w < kHalf; ++w) {
@@ -677,76 +783,15 @@ kv_attention_kernel(AttnParams p) {
                 o.z += f.z;
                 o.w += f.w;
             }
-            if (whole) {
-                if (row < row_count) put(row, col, o, l == 0.0f ? 0.0f : 1.0f / l);
+            if (seg.whole) {
+                if (row < row_count) put_row(p, seg, Shape::dim, row, col, o, l == 0.0f ? 0.0f : 1.0f / l);
             } else {
-                *reinterpret_cast<float4*>(p.part_o + ((size_t)slot * R + row) * Shape::dim + col) = o;
-                if (col == 0) p.part_ml[(size_t)slot * R + row] = make_float2(m, l);
+                *reinterpret_cast<float4*>(p.part_o + ((size_t)seg.slot * R + row) * Shape::dim + col) = o;
+                if (col == 0) p.part_ml[(size_t)seg.slot * R + row] = make_float2(m, l);
             }
         }
-        if (!whole) {
-            // ---- the parts of the (sequence, head, rows): blocks c0 .. c1, the first one's second slot, the others' first
-            const uint64_t first = origin + (uint64_t)item * units;
-            const uint32_t c0 = shares.block_of(first), parts = shares.block_of(first + units - 1) - c0 + 1;
-            if (last_of(p.counters + c0, parts, reinterpret_cast<uint32_t*>(shared64))) {
-                // shared: per row the maximum and 1 / sum, then the weights of kAttnJoin parts
-                float2* of_row = ml;
-                float* weights = reinterpret_cast<float*>(smem);
-                auto slot_of = [&](uint32_t c) { return (size_t)(c0 + c) * 2 + (c == 0 ? 1 : 0); };
-                constexpr uint32_t kLanes = 128 / R;  // that share a row: 8 or 16 neighbours of four warps
-                if (tid < 128) {
-                    const uint32_t row = tid / kLanes, at = tid % kLanes;
-                    float m = kNone, l = 0.0f;
-#pragma unroll 4
-                    for (uint32_t c = at; c < parts; c += kLanes) {
-                        const float2 f = __ldcg(&p.part_ml[slot_of(c) * R + row]);
-                        const float now = fmaxf(m, f.x);
-                        l = (m == kNone ? l : l * ex2(m - now)) + f.y * weight(f.x, now);
-                        m = now;
-                    }
-#pragma unroll
-                    for (uint32_t o = 1; o < kLanes; o *= 2) {
-                        const float m2 = __shfl_xor_sync(0xffffffffu, m, o), l2 = __shfl_xor_sync(0xffffffffu, l, o);
-                        const float now = fmaxf(m, m2);
-                        l = l * weight(m, now) + l2 * weight(m2, now);
-                        m = now;
-                    }
-                    if (at == 0) of_row[row] = make_float2(m, l == 0.0f ? 0.0f : 1.0f / l);
-                }
-                constexpr uint32_t kEach = (R * Shape::dim / 4 + W * 32 - 1) / (W * 32);
-                float4 o[kEach];
-#pragma unroll
-                for (uint32_t x = 0; x < kEach; ++x) o[x] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                for (uint32_t from = 0; from < parts; from += kAttnJoin) {
-                    const uint32_t count = min(kAttnJoin, parts - from);
-                    __syncthreads();
-                    for (uint32_t x = tid; x < count * R; x += W * 32)
-                        weights[x] = weight(__ldcg(&p.part_ml[slot_of(from + x / R) * R + x % R]).x, of_row[x % R].x);
-                    __syncthreads();
-#pragma unroll 8
-                    for (uint32_t c = 0; c < count; ++c) {
-                        const float4* src = reinterpret_cast<const float4*>(p.part_o + slot_of(from + c) * R * Shape::dim);
-#pragma unroll
-                        for (uint32_t x = 0; x < kEach; ++x) {
-                            const uint32_t at = tid + x * W * 32;
-                            if (at < R * Shape::dim / 4) {
-                                const float4 f = __ldcg(src + at);
-                                const float w = weights[c * R + at / (Shape::dim / 4)];
-                                o[x].x = fmaf(w, f.x, o[x].x);
-                                o[x].y = fmaf(w, f.y, o[x].y);
-                                o[x].z = fmaf(w, f.z, o[x].z);
-                                o[x].w = fmaf(w, f.w, o[x].w);
-                            }
-                        }
-                    }
-                }
-#pragma unroll
-                for (uint32_t x = 0; x < kEach; ++x) {
-                    const uint32_t at = tid + x * W * 32, row = at / (Shape::dim / 4);
-                    if (at < R * Shape::dim / 4 && row < row_count) put(row, at % (Shape::dim / 4) * 4, o[x], of_row[row].y);
-                }
-            }
-        }
+        if (!seg.whole && last_of(p.counters + seg.c0, seg.parts, reinterpret_cast<uint32_t*>(shared64)))
+            join_parts<R, Shape::dim, W * 32>(p, seg, ml, reinterpret_cast<float*>(smem));
         __syncthreads();
     }
 }
