@@ -192,9 +192,9 @@ VX_API vx_status vx_kv_cache_info(const vx_kv_cache* cache, int32_t* k_type, int
  * sequence s, and token p of sequence s lies in page table[s * max_pages + p / page_tokens].  The three arrays are
  * int32 on the device and are read there when the call's kernels run (a recorded call follows their contents);
  * `rows` is the number of rows that the call's tensors have.  Whatever the arrays hold, nothing outside the tensors
- * and the cache is touched: rows that no sequence names, tokens behind the page table's end and tokens whose page
- * number is negative or too large have no place (they are not written, read back as zeros, and are not attended to);
- * a sequence whose start is negative has no rows.  The places of two rows of a call must differ: sequences that share
+ * and the cache is touched: tokens behind the page table's end and tokens whose page number is negative or too large
+ * have no place (they are not written, read back as zeros, and are not attended to); a sequence whose start is
+ * negative has no rows; rows that no sequence names take no part (nothing is written to or for them).  The places of two rows of a call must differ: sequences that share
  * a page may both read it, and what is kept of a block that two rows write at once is not defined. */
 typedef struct {
     const int32_t* table; /* [seqs][max_pages] */
@@ -217,12 +217,13 @@ VX_API vx_status vx_kv_read(vx_context* ctx, const vx_kv_cache* cache, const vx_
  * j <= i: one new token per sequence, or a piece of a prompt.
  *   out[r, h, :] = sum_p softmax_p(scale * q[r, h, :] . k[p, h / group, :]) v[p, h / group, :],   group = heads / cache heads
  * q and out are rows of heads * head_dim floats, q_stride / out_stride apart; a row that attends to nothing is zeros; rows
- * of no sequence are left as they were.  Scores, softmax and sums are f32; q and the weights of the softmax enter the
- * tensor cores as two f16 parts (22 bits, csrc/vx_decode.cuh).  head_dim is 64, 96, 128 or 256 (VX_ERR_UNSUPPORTED
- * otherwise).  What lies in masked places, NaN included, does not reach the result.
+ * of no sequence are left as they were.  out may be q, with q's stride; it must not overlap q otherwise.  Scores, softmax
+ * and sums are f32; q and the weights of the softmax enter the tensor cores as two f16 parts (22 bits,
+ * csrc/vx_decode.cuh).  head_dim is 64, 96, 128 or 256 (VX_ERR_UNSUPPORTED otherwise).  What lies in masked places, NaN
+ * included, does not reach the result.  One launch.
  * A vx_kv_attention is the workspace of such calls (partial results of sequences that are split over the GPU's SMs),
- * made once for up to max_seqs sequences; calls with it follow each other on its context's stream.  A
- * recorded call keeps using it: graphs that may run at the same time need a vx_kv_attention each. */
+ * made once for up to max_seqs sequences of a cache, which must outlive it; calls with it follow each other on its
+ * context's stream.  A recorded call keeps using it: graphs that may run at the same time need a vx_kv_attention each. */
 typedef struct vx_kv_attention vx_kv_attention;
 VX_API vx_status vx_kv_attention_create(vx_context* ctx, const vx_kv_cache* cache, size_t heads, size_t max_seqs,
                                         vx_kv_attention** out);
@@ -238,13 +239,15 @@ VX_API vx_status vx_kv_attention_run(vx_context* ctx, const vx_kv_attention* att
  *   y = sum_e weight_e * down_e (silu(gate_e x) * (up_e x)),   silu(a) = a / (1 + exp(-a))
  * router is f32 on the device, [experts][hidden] (its pointer is kept).  gate and up hold the experts' matrices one
  * below the other (experts * inner rows, hidden columns, one type), down likewise (experts * hidden rows, inner columns,
- * its own type): the order of a weight file's three-dimensional expert tensors.  The handles are kept, not copied.
- * Only the weights of experts that get a token are read, each once per 16 of its tokens.  Three launches.
+ * its own type): the order of a weight file's three-dimensional expert tensors.  The handles are kept, not copied, and
+ * must outlive the layer.
+ * Only the weights of experts that get a token are read, each once per 8 of its tokens.  Three launches.
  * Sums are f32; x and the inner vector enter the tensor cores as two f16 parts per block (csrc/vx_decode.cuh).
  * experts <= 256, top_k <= 16 and <= experts, max_tokens <= 64.  The layer owns the workspace of its calls, with the same rule
  * as vx_kv_attention for calls that overlap.
  * run: x is `tokens` rows of `hidden` floats, x_stride apart; y likewise.  ids / weights (device, [tokens][top_k], may be
- * NULL) receive the chosen experts, best first, and their weights.  y must not overlap x. */
+ * NULL) receive the chosen experts, best first, and their weights.  y may be x or overlap it.  Inputs whose magnitude
+ * is 2^105 or more count as infinite. */
 typedef struct vx_moe vx_moe;
 VX_API vx_status vx_moe_create(vx_context* ctx, const float* router, size_t experts, const vx_qweights* gate,
                                const vx_qweights* up, const vx_qweights* down, size_t top_k, int32_t normalise,

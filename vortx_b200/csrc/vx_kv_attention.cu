@@ -87,6 +87,7 @@ vx_status vx_kv_attention_create(vx_context* ctx, const vx_kv_cache* cache, size
         return fail(VX_ERR_OUT_OF_MEMORY, "allocating %zu bytes of attention workspace failed: %s", bytes, cudaGetErrorString(e));
     }
     e = cudaMemsetAsync(a->workspace + a->counters_offset, 0, blocks * sizeof(uint32_t), ctx->stream);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->stream);  // an error while the stream is being captured
     if (e != cudaSuccess) {
         (void)cudaGetLastError();
         cudaFree(a->workspace);
@@ -119,6 +120,9 @@ vx_status vx_kv_attention_run(vx_context* ctx, const vx_kv_attention* a, const v
     const size_t width = a->heads * a->cache->head_dim;
     VX_REQUIRE(p.r.rows == 1 || (q_stride >= width && out_stride >= width), VX_ERR_INVALID_ARGUMENT,
                "vx_kv_attention_run: rows %zu and %zu elements apart, a row has %zu", q_stride, out_stride, width);
+    // In place, every block has read its rows of q before any of its heads' results is written.
+    VX_REQUIRE(q != out || p.r.rows == 1 || q_stride == out_stride, VX_ERR_INVALID_ARGUMENT,
+               "vx_kv_attention_run: out is q with rows %zu instead of %zu elements apart", out_stride, q_stride);
     VX_REQUIRE(!mask || (mask_words > 0 && mask_words <= 0x7ffffffull), VX_ERR_INVALID_ARGUMENT, "vx_kv_attention_run: a mask of %zu words a row", mask_words);
     const uint32_t group = (uint32_t)(a->heads / a->cache->g.heads);
     VX_REQUIRE((uint64_t)p.r.rows * group <= 0x7fffffffull, VX_ERR_UNSUPPORTED, "vx_kv_attention_run: too many rows (%u)", p.r.rows);

@@ -97,7 +97,7 @@ __device__ __forceinline__ void logits_of(const MoeParams& p, uint32_t expert, u
 }
 
 // One block of 32 values (a lane each) as two parts in B-operand order, and what its sums are to be multiplied with and
-// corrected by.  Values beyond 2^103 count as infinite.
+// corrected by.  f16 ends just below 2^16: values from 2^105 on count as infinite.
 __device__ __forceinline__ void split_block(float v, uint32_t lane, bool four, uint8_t* hi, uint8_t* lo, float2* factor) {
     const float up = fmaxf(lift(warp_max(fabsf(v))), __uint_as_float((127u - 89u) << 23));
     const float x = v * up;

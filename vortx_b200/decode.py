@@ -20,6 +20,8 @@ _WORDS = (_I32, _U32)
 
 
 def _check_len(what: str, length: Optional[int], rows: int, stride: int, width: int) -> None:
+    if stride < 0:
+        raise ValueError(f"the stride of {what} must not be negative")
     if length is not None and rows and (rows - 1) * stride + width > length:
         raise IndexError(f"{what} is shorter than {rows} rows")
 
@@ -47,7 +49,8 @@ class CacheRows:
     """Which tokens the rows of a call are (vx_kv_rows): row begin[s] + i is token start[s] + i of sequence s, whose token
     p lies in page table[s, p // page_tokens].  The arrays are int32 on the device (table [seqs, max_pages], begin
     [seqs + 1], start [seqs]) and are read when the call runs; `rows` is how many rows the call's tensors have.
-    `seqs` and `max_pages` follow from the lengths unless plain pointers are given."""
+    `seqs` and `max_pages` follow from the lengths unless plain pointers are given.  Pointers are captured at
+    construction."""
 
     def __init__(self, table, begin, start, rows: int, seqs: Optional[int] = None, max_pages: Optional[int] = None):
         (tp, tl), (bp, bl), (sp, sl) = (_typed(n, t, _WORDS) for n, t in (("table", table), ("begin", begin), ("start", start)))
@@ -144,6 +147,8 @@ class CacheAttention:
         if heads < 0 or max_seqs < 0:
             raise ValueError("heads and max_seqs must not be negative")
         self._h = None
+        if not cache._h:
+            raise ValueError("the cache has been freed")
         h = C.c_void_p()
         _lib.check(_lib.load().vx_kv_attention_create(backend._ctx, cache._h, heads, max_seqs, C.byref(h)))
         self.backend, self.cache, self.heads, self.max_seqs, self._h = backend, cache, heads, max_seqs, h
@@ -153,7 +158,7 @@ class CacheAttention:
                  mask_words: Optional[int] = None, q_stride: Optional[int] = None, out_stride: Optional[int] = None) -> None:
         """out[r, h] = attention of q[r, h] over the tokens before the call's and, among the call's own (already appended),
         those whose bits its row of `mask` (32-bit words, mask_words a row) has set; mask None: those up to itself.
-        scale defaults to 1 / sqrt(head_dim)."""
+        scale defaults to 1 / sqrt(head_dim).  out may be q, with q's stride."""
         qs = self.width if q_stride is None else q_stride
         os = self.width if out_stride is None else out_stride
         qp, ql = _typed("q", q, (_F32,))
@@ -169,6 +174,8 @@ class CacheAttention:
                 mask_words = ml // rows.rows if rows.rows else 1
             words = mask_words
             _check_len("mask", ml, rows.rows, words, words)
+        if not self.cache._h:
+            raise ValueError("the cache has been freed")
         s = self.cache.head_dim ** -0.5 if scale is None else scale
         _lib.check(_lib.load().vx_kv_attention_run(backend._ctx, self._h, rows._ref, qp, qs, op, os, s, mp, words))
 
@@ -201,15 +208,18 @@ class MoeLayer:
         _lib.check(_lib.load().vx_moe_create(backend._ctx, rp, experts, gate._h, up._h, down._h, top_k, int(bool(normalise)), max_tokens,
                                              C.byref(h)))
         self.backend, self._h = backend, h
-        self._keep = (router, gate, up, down)
+        self._router_buffer = router if type(router) is GpuBuffer else router.as_tensor_ref().raw_buffer() if hasattr(router, "as_tensor_ref") else None
+        self._router, self._gate, self._up, self._down = router, gate, up, down  # read by every call
         self.experts, self.top_k, self.hidden, self.inner, self.max_tokens = experts, top_k, gate.cols, down.cols, max_tokens
 
     def dispatch(self, backend: Backend, pass_: Optional[GpuPass], y, x, tokens: int = 1, x_stride: Optional[int] = None,
                  y_stride: Optional[int] = None, ids=None, weights=None) -> None:
         """y[t] = the layer's output for x[t], t < tokens; ids (int32) and weights (f32), both [tokens, top_k] and optional, receive
-        the chosen experts, best first, and what their outputs were weighted with."""
+        the chosen experts, best first, and what their outputs were weighted with.  y may be x or overlap it."""
         if tokens < 0:
             raise ValueError("tokens must not be negative")
+        if not (self._gate._h and self._up._h and self._down._h) or (self._router_buffer is not None and not self._router_buffer.ptr):
+            raise ValueError("the layer's weights have been freed")
         xs = self.hidden if x_stride is None else x_stride
         ys = self.hidden if y_stride is None else y_stride
         xp, xl = _typed("x", x, (_F32,))
