@@ -18,6 +18,7 @@
 // middle codes): 5e-7 relative to the exact result, 2e-7 with converted codes.  Nibbles left at bits 0..3 lose six more
 // bits: 6e-6.
 #include <algorithm>
+#include <cstddef>
 #include <memory>
 #include <new>
 #include <type_traits>
@@ -31,8 +32,7 @@ using namespace vx;
 constexpr uint32_t kMoeWarps = 8, kMoeThreads = kMoeWarps * 32;
 constexpr uint32_t kMaxExperts = 256, kMaxTopK = 16, kMaxTokens = 64;
 constexpr uint32_t kGroup = 8;              // tokens of an expert per pass over its weights: what fits 128 registers
-constexpr uint32_t kPitch = 144;            // a row's 128-byte chunk in shared memory: eight rows meet different banks
-constexpr uint32_t kStages = 2;             // chunks of 32 rows in flight per warp
+constexpr uint32_t kStages = 2;             // chunks in flight per warp
 constexpr uint32_t kSlice = 512;            // columns of a router row per warp: four 16-byte loads a lane, all in flight
 
 struct Matrix {
@@ -264,64 +264,91 @@ __device__ __forceinline__ void make_plan(const MoeParams& p, Plan* plan, PlanSc
 }
 
 // ---------------------------------------------------------------------------------------------- products ----
-// A chunk: 128 bytes of a row's codes, eight Q4_0 or four Q8_0 blocks.
-template <bool FOUR>
+// A stage of a warp's ring: 4 KiB of codes, 32 rows of one matrix with 128 bytes each or of two matrices with 64 each
+// (their 16-byte units swizzled, so that eight rows meet different banks), then the rows' scales.
+template <bool FOUR, int MATS>
 struct Chunk {
-    static constexpr uint32_t blocks = FOUR ? 8 : 4;
-    __device__ static uint32_t count(uint32_t nb) { return (nb + blocks - 1) / blocks; }
+    static constexpr uint32_t bytes = MATS == 2 ? 64 : 128, units = bytes / 16;
+    static constexpr uint32_t blocks = bytes / (FOUR ? 16 : 32);
+    __host__ __device__ static uint32_t count(uint32_t nb) { return (nb + blocks - 1) / blocks; }
+    __device__ static uint32_t swizzle(uint32_t row) { return (MATS == 2 ? row >> 1 : row) & (units - 1); }
 };
+constexpr uint32_t kCodes = 4096;
 
-// Copies a chunk of 32 rows to 32 rows of kPitch bytes; src: the lane's 16 bytes of row lane / 8, `four` the bytes of
-// four rows.
-__device__ __forceinline__ void fetch_rows(const uint8_t* src, size_t four, uint32_t dst, uint32_t lane) {
-    dst += (lane >> 3) * kPitch + (lane & 7) * 16;
+// Copies a chunk of 32 rows; src: the lane's 16 bytes of row lane / units.
+template <bool FOUR, int MATS>
+__device__ __forceinline__ void fetch_codes(const uint8_t* src, size_t row_bytes, uint32_t dst, uint32_t lane) {
+    using C = Chunk<FOUR, MATS>;
+    constexpr uint32_t rows = 32 / C::units;  // of a copy
 #pragma unroll
-    for (uint32_t i = 0; i < 8; ++i, src += four) cp_async16(dst + i * 4 * kPitch, src);
+    for (uint32_t i = 0; i < C::units; ++i) {
+        const uint32_t row = lane / C::units + i * rows;
+        cp_async16(dst + row * C::bytes + ((lane % C::units) ^ C::swizzle(row)) * 16, src + i * rows * row_bytes);
+    }
 }
 
-// Has a chunk's scales of a row fetched into the L2: they are read straight from there, too late to wait for the memory.
-__device__ __forceinline__ void prefetch_scales(const uint16_t* scales) { asm volatile("prefetch.global.L2 [%0];" ::"l"(scales)); }
-
-// The scales of a lane's rows g, g + 8, g + 16, g + 24 for the chunk that begins at block b, as pairs of halves.
-// WHOLE: a row's blocks are a multiple of the chunk's, so chunks are complete and the scales' addresses aligned.
-template <bool FOUR, bool WHOLE>
+// A chunk's scales.  WHOLE: a row's blocks are a multiple of the chunk's, so chunks are complete and their scales one
+// aligned piece per row.  Else the 4-byte words that hold them; a row of an odd number of blocks may begin in the middle of one.
+template <bool FOUR, int MATS, bool WHOLE>
 struct Scales {
-    static constexpr uint32_t B = Chunk<FOUR>::blocks;
-    uint32_t pair[4][B / 2];
-    __device__ __forceinline__ void load(const uint16_t* row, uint32_t b, uint32_t nb) {
+    static constexpr uint32_t B = Chunk<FOUR, MATS>::blocks, pitch = 2 * B + (WHOLE ? 0 : 4);
+    // the lane's row; row: of the matrix, first: the chunk's first block
+    __device__ static void fetch(const uint16_t* scales, size_t row, uint32_t first, uint32_t nb, uint32_t dst, uint32_t lane) {
+        dst += lane * pitch;
+        const size_t at = row * nb + first;
+        if (WHOLE) {
+            if (B == 8) cp_async16(dst, scales + at);
+            else if (B == 4) cp_async8(dst, scales + at);
+            else cp_async4(dst, scales + at);
+        } else {
+            const uint32_t odd = (uint32_t)at & 1u;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint16_t* s = row + i * 8 * nb + b;
-            if (WHOLE && FOUR) {
-                const uint4 v = __ldg(reinterpret_cast<const uint4*>(s));
-                pair[i][0] = v.x;
-                pair[i][1] = v.y;
-                pair[i][B / 2 - 2] = v.z;
-                pair[i][B / 2 - 1] = v.w;
-            } else if (WHOLE) {
-                const uint2 v = __ldg(reinterpret_cast<const uint2*>(s));
-                pair[i][0] = v.x;
-                pair[i][1] = v.y;
-            } else if (nb % 2 == 0) {
+            for (uint32_t k = 0; k <= B / 2; ++k)
+                if (first + 2 * k < nb + odd) cp_async4(dst + 4 * k, scales + (at - odd) + 2 * k);
+        }
+    }
+    // Blocks j0 .. j0 + G - 1 of rows g, g + 8, g + 16, g + 24; `first` as above
+    template <uint32_t G>
+    struct Of {
+        uint32_t pair[4][G / 2];
+        __device__ __forceinline__ Of(uint32_t src, uint32_t j0, uint32_t g, uint32_t nb) {
+            src += g * pitch + 2 * j0;
 #pragma unroll
-                for (uint32_t k = 0; k < B / 2; ++k) pair[i][k] = b + 2 * k < nb ? __ldg(reinterpret_cast<const uint32_t*>(s + 2 * k)) : 0u;
-            } else {
+            for (int i = 0; i < 4; ++i, src += 8 * pitch) {
+                if (!WHOLE) {
+                    uint32_t w[G / 2 + 1];
 #pragma unroll
-                for (uint32_t k = 0; k < B / 2; ++k) {
-                    const uint32_t lo = b + 2 * k < nb ? __ldg(s + 2 * k) : 0u, hi = b + 2 * k + 1 < nb ? __ldg(s + 2 * k + 1) : 0u;
-                    pair[i][k] = lo | hi << 16;
+                    for (uint32_t k = 0; k <= G / 2; ++k) w[k] = lds32(src + 4 * k);
+#pragma unroll
+                    for (uint32_t k = 0; k < G / 2; ++k) pair[i][k] = __funnelshift_r(w[k], w[k + 1], 16 * (g & nb & 1u));  // 32 rows begin with an even one
+                } else if (G == 8) {
+                    const uint4 v = lds128(src);
+                    pair[i][0] = v.x;
+                    pair[i][1] = v.y;
+                    pair[i][G / 2 - 2] = v.z;
+                    pair[i][G / 2 - 1] = v.w;
+                } else if (G == 4) {
+                    const uint2 v = lds64(src);
+                    pair[i][0] = v.x;
+                    pair[i][G / 2 - 1] = v.y;
+                } else {
+                    pair[i][0] = lds32(src);
                 }
             }
         }
-    }
-    __device__ __forceinline__ float of(int row, uint32_t j) const {
-        const __half2 d = bits_h2(pair[row][j / 2]);
-        return j % 2 ? __high2float(d) : __low2float(d);
-    }
+        __device__ __forceinline__ float operator()(int row, uint32_t j) const {
+            const __half2 d = bits_h2(pair[row][j / 2]);
+            return j % 2 ? __high2float(d) : __low2float(d);
+        }
+    };
 };
+template <bool FOUR, int MATS, bool WHOLE>
+constexpr uint32_t kStage = kCodes + 32 * MATS * Scales<FOUR, MATS, WHOLE>::pitch;  // a multiple of 128
+template <bool FOUR, int MATS, bool WHOLE>
+constexpr uint32_t kRing = kMoeWarps * kStages * kStage<FOUR, MATS, WHOLE>;
 
 // The vectors of a pass as a lane needs them: the B operand of token 4 n + g / 2 (part g % 2), the factors of token
-// 4 n + t; null where there is no such token.
+// 4 n + t.  Where there is no such token, another one's: its results are not used.
 template <int NT>
 struct Vectors {
     const uint8_t* px[NT];
@@ -331,32 +358,58 @@ struct Vectors {
         const uint32_t g = lane >> 2, t = lane & 3;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const uint32_t i = 4 * n + g / 2, k = 4 * n + t;
-            px[n] = i < count ? h + ((size_t)(slots[i] / per_row) * 2 + (g & 1)) * nb * 64 + t * 16 : nullptr;
-            pf[n] = k < count ? f + (size_t)(slots[k] / per_row) * nb : nullptr;
+            const uint32_t i = min(4 * n + g / 2, count - 1), k = min(4 * n + t, count - 1);
+            px[n] = h + ((size_t)(slots[i] / per_row) * 2 + (g & 1)) * nb * 64 + t * 16;
+            pf[n] = f + (size_t)(slots[k] / per_row) * nb;
         }
     }
-    __device__ __forceinline__ void load(uint32_t block, bool there, uint4 (&parts)[NT], float2 (&factor)[NT]) const {
+    __device__ __forceinline__ void advance(uint32_t blocks) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            parts[n] = make_uint4(0, 0, 0, 0);
-            factor[n] = make_float2(0.0f, 0.0f);
-            if (there) {
-                if (px[n]) parts[n] = *reinterpret_cast<const uint4*>(px[n] + (size_t)block * 64);
-                if (pf[n]) factor[n] = pf[n][block];
-            }
+            px[n] += (size_t)blocks * 64;
+            pf[n] += blocks;
+        }
+    }
+    __device__ __forceinline__ void load(int block, uint4* parts, float2* factor) const {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            parts[n] = *reinterpret_cast<const uint4*>(px[n] + block * 64);
+            factor[n] = pf[n][block];
         }
     }
 };
+// Blocks of the vectors that are in registers: a chunk's, four at most.
+template <bool FOUR, int MATS>
+struct Ahead {
+    static constexpr uint32_t B = Chunk<FOUR, MATS>::blocks;
+    static constexpr uint32_t group = B < 4 ? B : 4;
+    uint4 parts[2 * group];
+    float2 factor[2 * group];
+    template <int NT>
+    __device__ __forceinline__ void load(const Vectors<NT>& x, int block, uint32_t j) {
+        x.load(block, parts + j * NT, factor + j * NT);
+    }
+    // the first blocks of a pass over chunks c0 .. c1 - 1
+    template <int NT>
+    __device__ __forceinline__ void start(Vectors<NT> x, uint32_t c0, uint32_t c1, uint32_t nb) {
+        if (c0 >= c1) return;
+        x.advance(c0 * B);
+#pragma unroll
+        for (uint32_t j = 0; j < group; ++j)
+            if (c0 * B + j < nb) load<NT>(x, j, j);
+    }
+};
 
-// acc[m][n] += block j of the two 16-row tiles of a stage: rows 16 m + g and 16 m + g + 8, token 4 n + t.
-template <bool FOUR, int NT, class D>
-__device__ __forceinline__ void multiply(uint32_t stage, uint32_t j, uint32_t lane, const uint4 (&parts)[NT], const float2 (&factor)[NT], D scale,
+// acc[m][n] += block j of the two 16-row tiles of 32 rows: rows 16 m + g and 16 m + g + 8, token 4 n + t.  codes: where the
+// lane's row begins, its unit swizzled; a stage begins at a multiple of 128 bytes, so the block's number goes into the address's bits.
+template <bool FOUR, int MATS, int NT, class D>
+__device__ __forceinline__ void multiply(uint32_t codes, uint32_t j, const uint4* parts, const float2* factor, D scale,
                                          float (&acc)[2][NT][2]) {
+    using C = Chunk<FOUR, MATS>;
     uint32_t a[2][2][4];
     if (FOUR) {
         uint32_t w[4];
-        ldmatrix_x4(w, stage + lane * kPitch + j * 16);
+        ldmatrix_x4(w, codes ^ j * 16);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -371,7 +424,7 @@ __device__ __forceinline__ void multiply(uint32_t stage, uint32_t j, uint32_t la
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             uint32_t w[4];
-            ldmatrix_x4(w, stage + (i * 16 + (lane & 15)) * kPitch + j * 32 + (lane >> 4) * 16);
+            ldmatrix_x4(w, (codes ^ j * 32) + i * 16 * C::bytes);
 #pragma unroll
             for (int h = 0; h < 4; ++h) {
                 const uint32_t u = w[h] ^ 0x80808080u;
@@ -392,12 +445,18 @@ __device__ __forceinline__ void multiply(uint32_t stage, uint32_t j, uint32_t la
         }
 }
 
-// Sums of chunks c0, c0 + 8, .. < c1 of 32 rows of each of MATS matrices (`rows`: scales of the lane's row g), which are in
-// the ring one after the other.  next() waits for the next 32 rows and says where they are, done() gives them back.
+// Sums of chunks c0, c0 + 8, .. < c1 of 32 rows of each of MATS matrices.  next() waits for the next stage of the ring and
+// says where it is, done() gives it back.  `ahead` holds the vectors' first blocks; a block's place is filled with
+// the one that comes a group later as soon as it has been used.
 template <bool FOUR, bool WHOLE, int MATS, int NT, class Next, class Done>
-__device__ __forceinline__ void dot_chunks(const Vectors<NT>& x, uint32_t nb, const uint16_t* const (&rows)[MATS], uint32_t c0, uint32_t c1,
-                                           uint32_t lane, Next next, Done done, float (&acc)[MATS][2][NT][2]) {
-    constexpr uint32_t B = Chunk<FOUR>::blocks;
+__device__ __forceinline__ void dot_chunks(Vectors<NT> x, Ahead<FOUR, MATS>& ahead, uint32_t nb, uint32_t c0, uint32_t c1, uint32_t lane,
+                                           Next next, Done done, float (&acc)[MATS][2][NT][2]) {
+    using S = Scales<FOUR, MATS, WHOLE>;
+    constexpr uint32_t B = Chunk<FOUR, MATS>::blocks, G = Ahead<FOUR, MATS>::group;
+    using C = Chunk<FOUR, MATS>;
+    // where the lane's row begins for ldmatrix, block 0: a row is a tile's of 32 (Q4_0) or of 16, then its second unit (Q8_0)
+    const uint32_t lane_row = FOUR ? lane : lane & 15, lane_at = lane_row * C::bytes + ((FOUR ? 0 : lane >> 4) ^ C::swizzle(lane_row)) * 16;
+    x.advance(c0 * B);
 #pragma unroll
     for (int a = 0; a < MATS; ++a)
 #pragma unroll
@@ -405,36 +464,36 @@ __device__ __forceinline__ void dot_chunks(const Vectors<NT>& x, uint32_t nb, co
 #pragma unroll
             for (int n = 0; n < NT; ++n) acc[a][m][n][0] = acc[a][m][n][1] = 0.0f;
     for (uint32_t c = c0; c < c1; c += kMoeWarps) {
-        // with four tokens at most the chunk's vectors stay in registers for all matrices; more are read block by block
-        uint4 parts[NT == 1 ? B : 1][NT];
-        float2 factor[NT == 1 ? B : 1][NT];
-        if (NT == 1) {
+        const uint32_t stage = next(), codes = stage + lane_at;
+        const bool more = c + kMoeWarps < c1;
 #pragma unroll
-            for (uint32_t j = 0; j < B; ++j) x.load(c * B + j, WHOLE || c * B + j < nb, parts[NT == 1 ? j : 0], factor[NT == 1 ? j : 0]);
-        }
+        for (uint32_t j0 = 0; j0 < B; j0 += G)
 #pragma unroll
-        for (int a = 0; a < MATS; ++a) {
-            Scales<FOUR, WHOLE> d;
-            d.load(rows[a], c * B, nb);
-            const uint32_t stage = next();
+            for (int a = 0; a < MATS; ++a) {
+                const typename S::template Of<G> d(stage + kCodes + a * 32 * S::pitch, j0, lane >> 2, nb);
 #pragma unroll
-            for (uint32_t j = 0; j < B; ++j)
-                if (WHOLE || c * B + j < nb) {
-                    const uint32_t k = NT == 1 ? j : 0;
-                    if (NT > 1) x.load(c * B + j, true, parts[k], factor[k]);
-                    multiply<FOUR, NT>(stage, j, lane, parts[k], factor[k], [&](int row) { return d.of(row, j); }, acc[a]);
+                for (uint32_t j = 0; j < G; ++j) {
+                    const uint32_t block = c * B + j0 + j;
+                    if (WHOLE || block < nb)
+                        multiply<FOUR, MATS, NT>(codes + a * (kCodes / 2), j0 + j, ahead.parts + j * NT, ahead.factor + j * NT,
+                                                 [&](int row) { return d(row, j); }, acc[a]);
+                    if (a == MATS - 1) {
+                        const uint32_t later = j0 + j + (j0 + G < B ? G : kMoeWarps * B + G - B);
+                        if ((j0 + G < B || more) && (WHOLE || c * B + later < nb)) ahead.template load<NT>(x, later, j);
+                    }
                 }
-            done();
-        }
+            }
+        x.advance(kMoeWarps * B);
+        done();
     }
 }
 
 // ------------------------------------------------------------------------------------------------- inner ----
-constexpr uint32_t kStage = 32 * kPitch;
-constexpr uint32_t kRing = kMoeWarps * kStages * kStage;
-constexpr uint32_t kInnerSums = kMoeWarps * 64 * (kGroup + 1) * 4;
-constexpr uint32_t kInnerSmem = kRing + kInnerSums + sizeof(Plan);
-static_assert(plan_scratch(kMaxTokens) <= kRing + kInnerSums, "the plan is made where ring and sums are later");
+constexpr uint32_t kSums4 = kMoeWarps * 64 * 5;      // floats; two of them, or one for up to eight tokens
+constexpr uint32_t kInnerSums = std::max(2 * kSums4, kMoeWarps * 64 * (kGroup + 1)) * 4;
+template <bool FOUR, bool WHOLE>
+constexpr uint32_t kInnerSmem = kRing<FOUR, 2, WHOLE> + kInnerSums + sizeof(Plan);
+static_assert(plan_scratch(kMaxTokens) <= kMoeWarps * kStages * kCodes + kInnerSums, "the plan is made where ring and sums are later");
 
 // A pass over a unit's weights: 32 inner rows of an expert, up to kGroup of its tokens.  Block b of the grid has units
 // b, b + grid, ...
@@ -459,51 +518,46 @@ struct InnerPass {
 template <bool FOUR, bool WHOLE>
 __global__ void __launch_bounds__(kMoeThreads, 2) moe_inner_kernel(MoeParams p) {
     extern __shared__ __align__(128) uint8_t smem[];
-    constexpr uint32_t B = Chunk<FOUR>::blocks;
+    using C = Chunk<FOUR, 2>;
+    using S = Scales<FOUR, 2, WHOLE>;
+    constexpr uint32_t kRing = ::kRing<FOUR, 2, WHOLE>, kStage = ::kStage<FOUR, 2, WHOLE>;
     Plan* plan = reinterpret_cast<Plan*>(smem + kRing + kInnerSums);
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     pdl_wait();
     pdl_launch();
     make_plan<false>(p, plan, reinterpret_cast<PlanScratch*>(smem), blockIdx.x == 0);
-    const uint32_t nb = p.hidden / 32, chunks = Chunk<FOUR>::count(nb), tiles = p.inner / 32, nbf = tiles, units = plan->active * tiles;
+    const uint32_t nb = p.hidden / 32, chunks = C::count(nb), tiles = p.inner / 32, nbf = tiles, units = plan->active * tiles;
     const uint32_t ring = smem_addr(smem) + warp * kStages * kStage, row_bytes = nb * (FOUR ? 16 : 32);
     float* sums = reinterpret_cast<float*>(smem + kRing);
 
-    // what is copied runs kStages steps (32 gate rows, 32 up rows, the next chunk's gate rows, ..) ahead of what is multiplied
+    // what is copied runs kStages chunks ahead of what is multiplied
     InnerPass ahead;
     ahead.unit = blockIdx.x;
     ahead.enter(plan, tiles, units);
     InnerPass now = ahead;
-    const uint8_t *gate = nullptr, *up = nullptr;  // the lane's 16 bytes of the chunk to come
-    const uint16_t *gate_scales = nullptr, *up_scales = nullptr;
+    size_t ahead_row = 0, ahead_at = 0;  // first row, the lane's 16 bytes of the chunk to come
     uint32_t ahead_c = 0, filled = 0, used = 0;
     auto start = [&]() {  // of the pass `ahead`
-        const size_t row0 = (size_t)ahead.expert * p.inner + ahead.rows32 * 32;
-        const size_t at = (row0 + (lane >> 3)) * row_bytes + warp * 128 + (lane & 7) * 16, sc = (row0 + lane) * nb + warp * B;
-        gate = p.gate.quants + at;
-        up = p.up.quants + at;
-        gate_scales = p.gate.scales + sc;
-        up_scales = p.up.scales + sc;
+        ahead_row = (size_t)ahead.expert * p.inner + ahead.rows32 * 32;
+        ahead_at = (ahead_row + lane / C::units) * row_bytes + warp * C::bytes + lane % C::units * 16;
         ahead_c = warp;
     };
     start();
     auto fetch = [&]() {
-        const bool is_up = filled & 1;
-        if (!is_up && ahead_c >= chunks && warp < chunks && ahead.unit < units) {
+        if (ahead_c >= chunks && warp < chunks && ahead.unit < units) {
             ahead.next(plan, tiles, units);
             start();
         }
         if (ahead_c < chunks && ahead.unit < units) {
-            if (WHOLE || ahead_c * 128 + (lane & 7) * 16 < row_bytes)
-                fetch_rows(is_up ? up : gate, (size_t)4 * row_bytes, ring + (filled % kStages) * kStage, lane);
-            prefetch_scales(is_up ? up_scales : gate_scales);
-            if (is_up) {
-                gate += kMoeWarps * 128;
-                up += kMoeWarps * 128;
-                gate_scales += kMoeWarps * B;
-                up_scales += kMoeWarps * B;
-                ahead_c += kMoeWarps;
+            const uint32_t stage = ring + (filled % kStages) * kStage;
+            if (WHOLE || ahead_c * C::bytes + lane % C::units * 16 < row_bytes) {
+                fetch_codes<FOUR, 2>(p.gate.quants + ahead_at, row_bytes, stage, lane);
+                fetch_codes<FOUR, 2>(p.up.quants + ahead_at, row_bytes, stage + kCodes / 2, lane);
             }
+            S::fetch(p.gate.scales, ahead_row + lane, ahead_c * C::blocks, nb, stage + kCodes, lane);
+            S::fetch(p.up.scales, ahead_row + lane, ahead_c * C::blocks, nb, stage + kCodes + 32 * S::pitch, lane);
+            ahead_at += kMoeWarps * C::bytes;
+            ahead_c += kMoeWarps;
         }
         ++filled;
         cp_async_commit();
@@ -511,11 +565,22 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_inner_kernel(MoeParams p) 
 #pragma unroll
     for (uint32_t k = 0; k < kStages; ++k) fetch();
 
-    for (; now.unit < units; now.next(plan, tiles, units)) {
-        const uint32_t count = min(kGroup, now.end - now.at);
+    // Four tokens' sums are added up in two places in turn, with one barrier a pass; more tokens' use both, with three.
+    uint32_t turn = 0;
+    Ahead<FOUR, 2> vectors;
+    auto begin = [&](auto groups) {
+        constexpr int NT = decltype(groups)::value;
+        return Vectors<NT>(p.xh, p.xs, nb, plan->list + now.at, min(kGroup, now.end - now.at), p.top_k, lane);
+    };
+    auto begin_ahead = [&]() {
+        if (now.unit >= units) return;
+        if (now.end - now.at <= 4) vectors.start(begin(std::integral_constant<int, 1>()), warp, chunks, nb);
+        else vectors.start(begin(std::integral_constant<int, 2>()), warp, chunks, nb);
+    };
+    begin_ahead();
+    while (now.unit < units) {
+        const uint32_t count = min(kGroup, now.end - now.at), rows32 = now.rows32;
         const uint16_t* slots = plan->list + now.at;
-        const size_t at = ((size_t)now.expert * p.inner + now.rows32 * 32 + g) * nb;
-        const uint16_t* const rows[2] = {p.gate.scales + at, p.up.scales + at};
         auto next = [&]() {
             cp_async_wait<kStages - 1>();
             __syncwarp();
@@ -529,10 +594,14 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_inner_kernel(MoeParams p) 
         auto pass = [&](auto groups) {
             constexpr int NT = decltype(groups)::value;
             float acc[2][2][NT][2];
-            const Vectors<NT> x(p.xh, p.xs, nb, slots, count, p.top_k, lane);
-            dot_chunks<FOUR, WHOLE, 2, NT>(x, nb, rows, warp, chunks, lane, next, done, acc);
+            const Vectors<NT> x = begin(groups);
+            dot_chunks<FOUR, WHOLE, 2, NT>(x, vectors, nb, warp, chunks, lane, next, done, acc);
+            now.next(plan, tiles, units);
+            begin_ahead();
             // the eight warps' sums: gate rows 0..31, up rows 32..63
             constexpr uint32_t W = 4 * NT + 1;
+            if (NT > 1) __syncthreads();
+            float* to = sums + (NT > 1 ? 0 : turn * kSums4);
 #pragma unroll
             for (int a = 0; a < 2; ++a)
 #pragma unroll
@@ -540,21 +609,22 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_inner_kernel(MoeParams p) 
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) sums[(warp * 64 + a * 32 + m * 16 + h * 8 + g) * W + 4 * n + t] = acc[a][m][n][h];
+                        for (int h = 0; h < 2; ++h) to[(warp * 64 + a * 32 + m * 16 + h * 8 + g) * W + 4 * n + t] = acc[a][m][n][h];
             __syncthreads();
             for (uint32_t i = warp; i < count; i += kMoeWarps) {
                 float a = 0.0f, b = 0.0f;
 #pragma unroll
                 for (uint32_t w = 0; w < kMoeWarps; ++w) {
-                    a += sums[(w * 64 + lane) * W + i];
-                    b += sums[(w * 64 + 32 + lane) * W + i];
+                    a += to[(w * 64 + lane) * W + i];
+                    b += to[(w * 64 + 32 + lane) * W + i];
                 }
                 const float h = a / (1.0f + expf(-a)) * b;
                 const uint32_t slot = slots[i];
-                uint8_t* hi = p.hh + ((size_t)slot * 2 * nbf + now.rows32) * 64;
-                split_block(h, lane, p.down4 != 0, hi, hi + (size_t)nbf * 64, p.hs + (size_t)slot * nbf + now.rows32);
+                uint8_t* hi = p.hh + ((size_t)slot * 2 * nbf + rows32) * 64;
+                split_block(h, lane, p.down4 != 0, hi, hi + (size_t)nbf * 64, p.hs + (size_t)slot * nbf + rows32);
             }
-            __syncthreads();
+            if (NT > 1) __syncthreads();
+            turn ^= 1;
         };
         if (count <= 4) pass(std::integral_constant<int, 1>());
         else pass(std::integral_constant<int, 2>());
@@ -563,9 +633,14 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_inner_kernel(MoeParams p) 
 }
 
 // -------------------------------------------------------------------------------------------------- down ----
-constexpr uint32_t kDownSmem = kRing + sizeof(Plan);                       // and [warps][tokens][33] sums, between the two
+// Shared memory: the ring, [warps][tokens][33] sums, as much of the plan as the tokens need.
 constexpr uint32_t down_sums(uint32_t tokens) { return kMoeWarps * tokens * 33 * 4; }
-static_assert(plan_scratch(48) <= kRing && plan_scratch(kMaxTokens) <= kRing + down_sums(49), "the plan is made where ring and sums are later");
+template <bool FOUR, bool WHOLE>
+constexpr uint32_t down_smem(uint32_t tokens, uint32_t slots) {
+    return kRing<FOUR, 1, WHOLE> + down_sums(tokens) + (uint32_t)offsetof(Plan, weight) + slots * 4;
+}
+static_assert(plan_scratch(48) <= kMoeWarps * kStages * kCodes && plan_scratch(kMaxTokens) <= kMoeWarps * kStages * kCodes + down_sums(49),
+              "the plan is made where ring and sums are later");
 
 // A warp's way through the block's share of all experts' chunks, counted through: chunk `warp` of every eight, and
 // for each expert a pass per kGroup tokens.
@@ -616,8 +691,9 @@ __device__ __forceinline__ float cluster_load(uint32_t at, uint32_t rank) {
 template <bool FOUR, bool WHOLE>
 __global__ void __launch_bounds__(kMoeThreads, 2) moe_down_kernel(MoeParams p) {
     extern __shared__ __align__(128) uint8_t smem[];
-    constexpr uint32_t B = Chunk<FOUR>::blocks;
+    using C = Chunk<FOUR, 1>;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    constexpr uint32_t kRing = ::kRing<FOUR, 1, WHOLE>, kStage = ::kStage<FOUR, 1, WHOLE>;
     Plan* plan = reinterpret_cast<Plan*>(smem + kRing + down_sums(p.tokens));
     float* sums = reinterpret_cast<float*>(smem + kRing);  // [warps][tokens][33]
     float* mine = sums + warp * p.tokens * 33;
@@ -626,7 +702,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_down_kernel(MoeParams p) {
     for (uint32_t i = lane; i < p.tokens * 33; i += 32) mine[i] = 0.0f;
     __syncwarp();
     const uint32_t tile = blockIdx.x, split = blockIdx.y;
-    const uint32_t nb = p.inner / 32, chunks = Chunk<FOUR>::count(nb), row_bytes = nb * (FOUR ? 16 : 32);
+    const uint32_t nb = p.inner / 32, chunks = C::count(nb), row_bytes = nb * (FOUR ? 16 : 32);
     const uint64_t all = (uint64_t)plan->active * chunks;
     const uint32_t lo = (uint32_t)(all * split / p.splits), hi = (uint32_t)(all * (split + 1) / p.splits);
     const uint32_t ring = smem_addr(smem) + warp * kStages * kStage;
@@ -635,23 +711,21 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_down_kernel(MoeParams p) {
     ahead.a = lo / chunks;
     ahead.enter(plan, chunks, lo, hi, warp);
     DownPass now = ahead;
-    const uint8_t* codes = nullptr;
-    const uint16_t* scales_ahead = nullptr;
+    size_t ahead_row = 0, ahead_at = 0;  // first row, the lane's 16 bytes of the chunk to come
     uint32_t filled = 0, used = 0;
     auto start = [&]() {
         if (!ahead.valid()) return;
-        const size_t row0 = (size_t)plan->expert[ahead.a] * p.hidden + tile * 32;
-        codes = p.down.quants + (row0 + (lane >> 3)) * row_bytes + ahead.c * 128 + (lane & 7) * 16;
-        scales_ahead = p.down.scales + (row0 + lane) * nb + ahead.c * B;
+        ahead_row = (size_t)plan->expert[ahead.a] * p.hidden + tile * 32;
+        ahead_at = (ahead_row + lane / C::units) * row_bytes + ahead.c * C::bytes + lane % C::units * 16;
     };
     start();
     auto fetch = [&]() {
         if (ahead.valid()) {
-            if (WHOLE || ahead.c * 128 + (lane & 7) * 16 < row_bytes)
-                fetch_rows(codes, (size_t)4 * row_bytes, ring + (filled % kStages) * kStage, lane);
-            prefetch_scales(scales_ahead);
-            codes += kMoeWarps * 128;
-            scales_ahead += kMoeWarps * B;
+            const uint32_t stage = ring + (filled % kStages) * kStage;
+            if (WHOLE || ahead.c * C::bytes + lane % C::units * 16 < row_bytes)
+                fetch_codes<FOUR, 1>(p.down.quants + ahead_at, row_bytes, stage, lane);
+            Scales<FOUR, 1, WHOLE>::fetch(p.down.scales, ahead_row + lane, ahead.c * C::blocks, nb, stage + kCodes, lane);
+            ahead_at += kMoeWarps * C::bytes;
             ahead.c += kMoeWarps;
             if (ahead.c >= ahead.c1) {
                 ahead.next_pass(plan, chunks, lo, hi, warp);
@@ -665,10 +739,20 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_down_kernel(MoeParams p) {
     for (uint32_t k = 0; k < kStages; ++k) fetch();
     pdl_wait();  // for the inner vectors
     pdl_launch();
+    Ahead<FOUR, 1> vectors;
+    auto begin = [&](auto groups) {
+        constexpr int NT = decltype(groups)::value;
+        return Vectors<NT>(p.hh, p.hs, nb, plan->list + now.at, min(kGroup, plan->begin[now.a + 1] - now.at), 1, lane);
+    };
+    auto begin_ahead = [&]() {
+        if (!now.valid()) return;
+        if (plan->begin[now.a + 1] - now.at <= 4) vectors.start(begin(std::integral_constant<int, 1>()), now.c0, now.c1, nb);
+        else vectors.start(begin(std::integral_constant<int, 2>()), now.c0, now.c1, nb);
+    };
+    begin_ahead();
     while (now.valid()) {
-        const uint32_t begin = now.at, count = min(kGroup, plan->begin[now.a + 1] - begin);
-        const uint16_t* slots = plan->list + begin;
-        const uint16_t* const rows[1] = {p.down.scales + ((size_t)plan->expert[now.a] * p.hidden + tile * 32 + g) * nb};
+        const uint32_t count = min(kGroup, plan->begin[now.a + 1] - now.at);
+        const uint16_t* slots = plan->list + now.at;
         auto next = [&]() {
             cp_async_wait<kStages - 1>();
             __syncwarp();
@@ -682,8 +766,10 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_down_kernel(MoeParams p) {
         auto pass = [&](auto groups) {
             constexpr int NT = decltype(groups)::value;
             float acc[1][2][NT][2];
-            const Vectors<NT> x(p.hh, p.hs, nb, slots, count, 1, lane);
-            dot_chunks<FOUR, WHOLE, 1, NT>(x, nb, rows, now.c0, now.c1, lane, next, done, acc);
+            const Vectors<NT> x = begin(groups);
+            dot_chunks<FOUR, WHOLE, 1, NT>(x, vectors, nb, now.c0, now.c1, lane, next, done, acc);
+            now.next_pass(plan, chunks, lo, hi, warp);
+            begin_ahead();
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 const uint32_t i = 4 * n + t;
@@ -701,7 +787,6 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_down_kernel(MoeParams p) {
         };
         if (count <= 4) pass(std::integral_constant<int, 1>());
         else pass(std::integral_constant<int, 2>());
-        now.next_pass(plan, chunks, lo, hi, warp);
     }
     cp_async_wait<0>();
     __syncthreads();
@@ -729,14 +814,23 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_down_kernel(MoeParams p) {
 
 // The kernels for a matrix: its type, and whether its rows are whole chunks.
 using MoeKernel = void (*)(MoeParams);
-bool whole_chunks(bool four, uint32_t cols) { return cols / 32 % (four ? 8 : 4) == 0; }
-MoeKernel inner_kernel(const MoeParams& p) {
-    if (p.gate4) return whole_chunks(true, p.hidden) ? moe_inner_kernel<true, true> : moe_inner_kernel<true, false>;
-    return whole_chunks(false, p.hidden) ? moe_inner_kernel<false, true> : moe_inner_kernel<false, false>;
+struct Launch {
+    MoeKernel kernel;
+    uint32_t smem;
+};
+template <bool FOUR>
+Launch inner_of(uint32_t nb) {
+    if (nb % Chunk<FOUR, 2>::blocks == 0) return {moe_inner_kernel<FOUR, true>, kInnerSmem<FOUR, true>};
+    return {moe_inner_kernel<FOUR, false>, kInnerSmem<FOUR, false>};
 }
-MoeKernel down_kernel(const MoeParams& p) {
-    if (p.down4) return whole_chunks(true, p.inner) ? moe_down_kernel<true, true> : moe_down_kernel<true, false>;
-    return whole_chunks(false, p.inner) ? moe_down_kernel<false, true> : moe_down_kernel<false, false>;
+template <bool FOUR>
+Launch down_of(uint32_t nb, uint32_t tokens, uint32_t slots) {
+    if (nb % Chunk<FOUR, 1>::blocks == 0) return {moe_down_kernel<FOUR, true>, down_smem<FOUR, true>(tokens, slots)};
+    return {moe_down_kernel<FOUR, false>, down_smem<FOUR, false>(tokens, slots)};
+}
+Launch inner_launch(const MoeParams& p) { return p.gate4 ? inner_of<true>(p.hidden / 32) : inner_of<false>(p.hidden / 32); }
+Launch down_launch(const MoeParams& p, uint32_t tokens) {
+    return p.down4 ? down_of<true>(p.inner / 32, tokens, tokens * p.top_k) : down_of<false>(p.inner / 32, tokens, tokens * p.top_k);
 }
 
 size_t round_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
@@ -795,10 +889,15 @@ vx_status vx_moe_create(vx_context* ctx, const float* router, size_t experts, co
     p.row_log = 2;
     while ((1u << p.row_log) < p.experts) ++p.row_log;
     int per_sm = 0;
-    VX_CUDA(cudaFuncSetAttribute(inner_kernel(p), cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kInnerSmem));
-    VX_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, inner_kernel(p), kMoeThreads, kInnerSmem));
+    const Launch inner_k = inner_launch(p);
+    VX_CUDA(cudaFuncSetAttribute(inner_k.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)inner_k.smem));
+    VX_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, inner_k.kernel, kMoeThreads, inner_k.smem));
     m->inner_grid = (uint32_t)std::max(1, per_sm) * m->sm_count;
-    VX_CUDA(cudaFuncSetAttribute(down_kernel(p), cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kDownSmem + down_sums(kMaxTokens))));
+    // for every layer of these types, so the most that any needs
+    MoeParams most = p;
+    most.top_k = kMaxTopK;
+    const Launch down_k = down_launch(most, kMaxTokens);
+    VX_CUDA(cudaFuncSetAttribute(down_k.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)down_k.smem));
     // ---- workspace ------------------------------------------------------------------------------------------------------
     const size_t slots = max_tokens * top_k, nbh = hidden / 32, nbf = inner / 32;
     size_t at = 0;
@@ -860,8 +959,9 @@ vx_status vx_moe_run(vx_context* ctx, const vx_moe* m, const float* x, size_t x_
     // as many units as there can be experts with tokens
     const uint64_t units = (uint64_t)std::min<uint64_t>(p.experts, (uint64_t)p.tokens * p.top_k) * (p.inner / 32);
     const uint32_t grid = (uint32_t)std::min<uint64_t>(units, m->inner_grid);
-    VX_CUDA(launch_after(inner_kernel(p), dim3(grid), kMoeThreads, kInnerSmem, ctx->stream, p));
-    VX_CUDA(launch_after(down_kernel(p), dim3(p.hidden / 32, p.splits), kMoeThreads, kDownSmem + down_sums(p.tokens), ctx->stream, p, dim3(1, p.splits)));
+    const Launch inner = inner_launch(p), down = down_launch(p, p.tokens);
+    VX_CUDA(launch_after(inner.kernel, dim3(grid), kMoeThreads, inner.smem, ctx->stream, p));
+    VX_CUDA(launch_after(down.kernel, dim3(p.hidden / 32, p.splits), kMoeThreads, down.smem, ctx->stream, p, dim3(1, p.splits)));
     ctx->launches += 3;
     return VX_OK;
 }
