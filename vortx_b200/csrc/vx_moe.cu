@@ -135,10 +135,11 @@ __global__ void __launch_bounds__(kMoeThreads) moe_route_kernel(MoeParams p) {
 }
 
 // What every block of the products knows of the routing: the experts that have tokens, and for each the list of its
-// slots (token * top_k + place), tokens ascending.
+// slots (token * top_k + place), tokens ascending, and those tokens.
 struct Plan {
     uint32_t active;
     uint16_t expert[kMaxExperts], begin[kMaxExperts + 2], list[kMaxTokens * kMaxTopK];
+    uint8_t token[kMaxTokens * kMaxTopK];
     float weight[kMaxTokens * kMaxTopK];
 };
 struct PlanScratch {
@@ -258,7 +259,9 @@ __device__ __forceinline__ void make_plan(const MoeParams& p, Plan* plan, PlanSc
     __syncthreads();
     for (uint32_t slot = tid; slot < p.tokens * p.top_k; slot += kMoeThreads) {
         const uint32_t e = w->chosen[slot], t = slot / p.top_k, bits = w->tokens[t >> 5][e] & ((1u << (t & 31)) - 1u);
-        plan->list[w->begin[e] + __popc(bits) + (t >= 32 ? __popc(w->tokens[0][e]) : 0)] = (uint16_t)slot;
+        const uint32_t at = w->begin[e] + __popc(bits) + (t >= 32 ? __popc(w->tokens[0][e]) : 0);
+        plan->list[at] = (uint16_t)slot;
+        plan->token[at] = (uint8_t)t;
     }
     __syncthreads();
 }
@@ -353,14 +356,14 @@ template <int NT>
 struct Vectors {
     const uint8_t* px[NT];
     const float2* pf[NT];
-    __device__ __forceinline__ Vectors(const uint8_t* h, const float2* f, uint32_t nb, const uint16_t* slots, uint32_t count, uint32_t per_row,
-                                       uint32_t lane) {
+    template <class Row>
+    __device__ __forceinline__ Vectors(const uint8_t* h, const float2* f, uint32_t nb, const Row* rows, uint32_t count, uint32_t lane) {
         const uint32_t g = lane >> 2, t = lane & 3;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             const uint32_t i = min(4 * n + g / 2, count - 1), k = min(4 * n + t, count - 1);
-            px[n] = h + ((size_t)(slots[i] / per_row) * 2 + (g & 1)) * nb * 64 + t * 16;
-            pf[n] = f + (size_t)(slots[k] / per_row) * nb;
+            px[n] = h + (size_t)(rows[i] * 2u + (g & 1)) * (nb * 64) + t * 16;
+            pf[n] = f + (size_t)rows[k] * nb;
         }
     }
     __device__ __forceinline__ void advance(uint32_t blocks) {
@@ -382,9 +385,11 @@ struct Vectors {
 template <bool FOUR, int MATS>
 struct Ahead {
     static constexpr uint32_t B = Chunk<FOUR, MATS>::blocks;
-    static constexpr uint32_t group = B < 4 ? B : 4;
-    uint4 parts[2 * group];
-    float2 factor[2 * group];
+    template <int NT>
+    static constexpr uint32_t group = std::min(B, NT == 1 || MATS == 2 ? 4u : 2u);
+    static constexpr uint32_t size = std::max(group<1>, 2 * group<2>);
+    uint4 parts[size];
+    float2 factor[size];
     template <int NT>
     __device__ __forceinline__ void load(const Vectors<NT>& x, int block, uint32_t j) {
         x.load(block, parts + j * NT, factor + j * NT);
@@ -395,7 +400,7 @@ struct Ahead {
         if (c0 >= c1) return;
         x.advance(c0 * B);
 #pragma unroll
-        for (uint32_t j = 0; j < group; ++j)
+        for (uint32_t j = 0; j < group<NT>; ++j)
             if (c0 * B + j < nb) load<NT>(x, j, j);
     }
 };
@@ -452,7 +457,7 @@ template <bool FOUR, bool WHOLE, int MATS, int NT, class Next, class Done>
 __device__ __forceinline__ void dot_chunks(Vectors<NT> x, Ahead<FOUR, MATS>& ahead, uint32_t nb, uint32_t c0, uint32_t c1, uint32_t lane,
                                            Next next, Done done, float (&acc)[MATS][2][NT][2]) {
     using S = Scales<FOUR, MATS, WHOLE>;
-    constexpr uint32_t B = Chunk<FOUR, MATS>::blocks, G = Ahead<FOUR, MATS>::group;
+    constexpr uint32_t B = Chunk<FOUR, MATS>::blocks, G = Ahead<FOUR, MATS>::template group<NT>;
     using C = Chunk<FOUR, MATS>;
     // where the lane's row begins for ldmatrix, block 0: a row is a tile's of 32 (Q4_0) or of 16, then its second unit (Q8_0)
     const uint32_t lane_row = FOUR ? lane : lane & 15, lane_at = lane_row * C::bytes + ((FOUR ? 0 : lane >> 4) ^ C::swizzle(lane_row)) * 16;
@@ -498,21 +503,20 @@ static_assert(plan_scratch(kMaxTokens) <= kMoeWarps * kStages * kCodes + kInnerS
 // A pass over a unit's weights: 32 inner rows of an expert, up to kGroup of its tokens.  Block b of the grid has units
 // b, b + grid, ...
 struct InnerPass {
-    uint32_t unit, at, end, rows32, expert;
+    uint32_t unit, a, at;  // a: expert number in the plan, at: of its list
     __device__ void enter(const Plan* plan, uint32_t tiles, uint32_t units) {
         if (unit >= units) return;
-        const uint32_t a = unit / tiles;
-        rows32 = unit - a * tiles;
-        expert = plan->expert[a];
+        a = unit / tiles;
         at = plan->begin[a];
-        end = plan->begin[a + 1];
     }
     __device__ void next(const Plan* plan, uint32_t tiles, uint32_t units) {
         at += kGroup;
-        if (at < end) return;
+        if (at < plan->begin[a + 1]) return;
         unit += gridDim.x;
         enter(plan, tiles, units);
     }
+    __device__ uint32_t count(const Plan* plan) const { return plan->begin[a + 1] - at; }
+    __device__ uint32_t rows32(uint32_t tiles) const { return unit - a * tiles; }
 };
 
 template <bool FOUR, bool WHOLE>
@@ -536,20 +540,19 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_inner_kernel(MoeParams p) 
     ahead.enter(plan, tiles, units);
     InnerPass now = ahead;
     size_t ahead_row = 0, ahead_at = 0;  // first row, the lane's 16 bytes of the chunk to come
-    uint32_t ahead_c = 0, filled = 0, used = 0;
+    uint32_t ahead_c = 0, used = 0;
     auto start = [&]() {  // of the pass `ahead`
-        ahead_row = (size_t)ahead.expert * p.inner + ahead.rows32 * 32;
+        ahead_row = (size_t)plan->expert[ahead.a] * p.inner + ahead.rows32(tiles) * 32;
         ahead_at = (ahead_row + lane / C::units) * row_bytes + warp * C::bytes + lane % C::units * 16;
         ahead_c = warp;
     };
-    start();
-    auto fetch = [&]() {
+    if (ahead.unit < units) start();
+    auto fetch = [&](uint32_t stage) {
         if (ahead_c >= chunks && warp < chunks && ahead.unit < units) {
             ahead.next(plan, tiles, units);
-            start();
+            if (ahead.unit < units) start();
         }
         if (ahead_c < chunks && ahead.unit < units) {
-            const uint32_t stage = ring + (filled % kStages) * kStage;
             if (WHOLE || ahead_c * C::bytes + lane % C::units * 16 < row_bytes) {
                 fetch_codes<FOUR, 2>(p.gate.quants + ahead_at, row_bytes, stage, lane);
                 fetch_codes<FOUR, 2>(p.up.quants + ahead_at, row_bytes, stage + kCodes / 2, lane);
@@ -559,27 +562,26 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_inner_kernel(MoeParams p) 
             ahead_at += kMoeWarps * C::bytes;
             ahead_c += kMoeWarps;
         }
-        ++filled;
         cp_async_commit();
     };
 #pragma unroll
-    for (uint32_t k = 0; k < kStages; ++k) fetch();
+    for (uint32_t k = 0; k < kStages; ++k) fetch(ring + k * kStage);
 
     // Four tokens' sums are added up in two places in turn, with one barrier a pass; more tokens' use both, with three.
     uint32_t turn = 0;
     Ahead<FOUR, 2> vectors;
     auto begin = [&](auto groups) {
         constexpr int NT = decltype(groups)::value;
-        return Vectors<NT>(p.xh, p.xs, nb, plan->list + now.at, min(kGroup, now.end - now.at), p.top_k, lane);
+        return Vectors<NT>(p.xh, p.xs, nb, plan->token + now.at, min(kGroup, now.count(plan)), lane);
     };
     auto begin_ahead = [&]() {
         if (now.unit >= units) return;
-        if (now.end - now.at <= 4) vectors.start(begin(std::integral_constant<int, 1>()), warp, chunks, nb);
+        if (now.count(plan) <= 4) vectors.start(begin(std::integral_constant<int, 1>()), warp, chunks, nb);
         else vectors.start(begin(std::integral_constant<int, 2>()), warp, chunks, nb);
     };
     begin_ahead();
     while (now.unit < units) {
-        const uint32_t count = min(kGroup, now.end - now.at), rows32 = now.rows32;
+        const uint32_t count = min(kGroup, now.count(plan)), rows32 = now.rows32(tiles);
         const uint16_t* slots = plan->list + now.at;
         auto next = [&]() {
             cp_async_wait<kStages - 1>();
@@ -587,9 +589,9 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_inner_kernel(MoeParams p) 
             return ring + (used % kStages) * kStage;
         };
         auto done = [&]() {
-            ++used;
             __syncwarp();
-            fetch();
+            fetch(ring + (used % kStages) * kStage);
+            ++used;
         };
         auto pass = [&](auto groups) {
             constexpr int NT = decltype(groups)::value;
@@ -712,16 +714,15 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_down_kernel(MoeParams p) {
     ahead.enter(plan, chunks, lo, hi, warp);
     DownPass now = ahead;
     size_t ahead_row = 0, ahead_at = 0;  // first row, the lane's 16 bytes of the chunk to come
-    uint32_t filled = 0, used = 0;
+    uint32_t used = 0;
     auto start = [&]() {
         if (!ahead.valid()) return;
         ahead_row = (size_t)plan->expert[ahead.a] * p.hidden + tile * 32;
         ahead_at = (ahead_row + lane / C::units) * row_bytes + ahead.c * C::bytes + lane % C::units * 16;
     };
     start();
-    auto fetch = [&]() {
+    auto fetch = [&](uint32_t stage) {
         if (ahead.valid()) {
-            const uint32_t stage = ring + (filled % kStages) * kStage;
             if (WHOLE || ahead.c * C::bytes + lane % C::units * 16 < row_bytes)
                 fetch_codes<FOUR, 1>(p.down.quants + ahead_at, row_bytes, stage, lane);
             Scales<FOUR, 1, WHOLE>::fetch(p.down.scales, ahead_row + lane, ahead.c * C::blocks, nb, stage + kCodes, lane);
@@ -732,17 +733,16 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_down_kernel(MoeParams p) {
                 start();
             }
         }
-        ++filled;
         cp_async_commit();
     };
 #pragma unroll
-    for (uint32_t k = 0; k < kStages; ++k) fetch();
+    for (uint32_t k = 0; k < kStages; ++k) fetch(ring + k * kStage);
     pdl_wait();  // for the inner vectors
     pdl_launch();
     Ahead<FOUR, 1> vectors;
     auto begin = [&](auto groups) {
         constexpr int NT = decltype(groups)::value;
-        return Vectors<NT>(p.hh, p.hs, nb, plan->list + now.at, min(kGroup, plan->begin[now.a + 1] - now.at), 1, lane);
+        return Vectors<NT>(p.hh, p.hs, nb, plan->list + now.at, min(kGroup, plan->begin[now.a + 1] - now.at), lane);
     };
     auto begin_ahead = [&]() {
         if (!now.valid()) return;
@@ -759,9 +759,9 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_down_kernel(MoeParams p) {
             return ring + (used % kStages) * kStage;
         };
         auto done = [&]() {
-            ++used;
             __syncwarp();
-            fetch();
+            fetch(ring + (used % kStages) * kStage);
+            ++used;
         };
         auto pass = [&](auto groups) {
             constexpr int NT = decltype(groups)::value;
