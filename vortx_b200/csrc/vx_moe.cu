@@ -350,8 +350,12 @@ constexpr uint32_t kStage = kCodes + 32 * MATS * Scales<FOUR, MATS, WHOLE>::pitc
 template <bool FOUR, int MATS, bool WHOLE>
 constexpr uint32_t kRing = kMoeWarps * kStages * kStage<FOUR, MATS, WHOLE>;
 
-// The vectors of a pass as a lane needs them: the B operand of token 4 n + g / 2 (part g % 2), the factors of token
-// 4 n + t.  Where there is no such token, another one's: its results are not used.
+// The vectors of a pass as a lane needs them, NT = 1 for up to four tokens, 2 for up to eight.  B's columns are both parts
+// of four tokens, or eight tokens, of which the two parts are multiplied one after the other: a lane has the operand
+// of token g / 2, part g % 2, or of token g, both parts, and the results and factors of NT tokens.  Where there is no such
+// token, another one's: its results are not used.
+template <int NT>
+__device__ __forceinline__ uint32_t token_of(uint32_t n, uint32_t t) { return NT == 1 ? t : 2 * t + n; }
 template <int NT>
 struct Vectors {
     const uint8_t* px[NT];
@@ -361,8 +365,8 @@ struct Vectors {
         const uint32_t g = lane >> 2, t = lane & 3;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const uint32_t i = min(4 * n + g / 2, count - 1), k = min(4 * n + t, count - 1);
-            px[n] = h + (size_t)(rows[i] * 2u + (g & 1)) * (nb * 64) + t * 16;
+            const uint32_t i = min(NT == 1 ? g / 2 : g, count - 1), k = min(token_of<NT>(n, t), count - 1);
+            px[n] = h + (size_t)(rows[i] * 2u + (NT == 1 ? g & 1 : n)) * (nb * 64) + t * 16;
             pf[n] = f + (size_t)rows[k] * nb;
         }
     }
@@ -405,7 +409,7 @@ struct Ahead {
     }
 };
 
-// acc[m][n] += block j of the two 16-row tiles of 32 rows: rows 16 m + g and 16 m + g + 8, token 4 n + t.  codes: where the
+// acc[m][n] += block j of the two 16-row tiles of 32 rows: rows 16 m + g and 16 m + g + 8, token token_of(n, t).  codes: where the
 // lane's row begins, its unit swizzled; a stage begins at a multiple of 128 bytes, so the block's number goes into the address's bits.
 template <bool FOUR, int MATS, int NT, class D>
 __device__ __forceinline__ void multiply(uint32_t codes, uint32_t j, const uint4* parts, const float2* factor, D scale,
@@ -438,16 +442,28 @@ __device__ __forceinline__ void multiply(uint32_t codes, uint32_t j, const uint4
             }
         }
     }
+    float s[2][4];
+    auto both = [&](auto use) {  // neighbouring products do not wait for each other
+        use(0);
+        use(1);
+    };
+    if (NT > 1) {
+        both([&](int i) { mma_f16_new(s[i], a[i][0], parts[NT - 1].x, parts[NT - 1].y); });
+        both([&](int i) { mma_f16(s[i], a[i][1], parts[NT - 1].z, parts[NT - 1].w); });
+        both([&](int i) { mma_f16(s[i], a[i][0], parts[0].x, parts[0].y); });
+    } else {
+        both([&](int i) { mma_f16_new(s[i], a[i][0], parts[0].x, parts[0].y); });
+    }
+    both([&](int i) { mma_f16(s[i], a[i][1], parts[0].z, parts[0].w); });
+    both([&](int i) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            float s[4];
-            mma_f16_new(s, a[i][0], parts[n].x, parts[n].y);
-            mma_f16(s, a[i][1], parts[n].z, parts[n].w);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) acc[i][n][h] = fmaf(fmaf(s[2 * h] + s[2 * h + 1], factor[n].x, factor[n].y), scale(2 * i + h), acc[i][n][h]);
-        }
+            for (int h = 0; h < 2; ++h) {
+                const float sum = NT == 1 ? s[i][2 * h] + s[i][2 * h + 1] : s[i][2 * h + n];
+                acc[i][n][h] = fmaf(fmaf(sum, factor[n].x, factor[n].y), scale(2 * i + h), acc[i][n][h]);
+            }
+    });
 }
 
 // Sums of chunks c0, c0 + 8, .. < c1 of 32 rows of each of MATS matrices.  next() waits for the next stage of the ring and
@@ -611,7 +627,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_inner_kernel(MoeParams p) 
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) to[(warp * 64 + a * 32 + m * 16 + h * 8 + g) * W + 4 * n + t] = acc[a][m][n][h];
+                        for (int h = 0; h < 2; ++h) to[(warp * 64 + a * 32 + m * 16 + h * 8 + g) * W + token_of<NT>(n, t)] = acc[a][m][n][h];
             __syncthreads();
             for (uint32_t i = warp; i < count; i += kMoeWarps) {
                 float a = 0.0f, b = 0.0f;
@@ -772,7 +788,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_down_kernel(MoeParams p) {
             begin_ahead();
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const uint32_t i = 4 * n + t;
+                const uint32_t i = token_of<NT>(n, t);
                 if (i < count) {
                     const uint32_t slot = slots[i];
                     const float w = plan->weight[slot];
