@@ -70,6 +70,17 @@ def test_every_group_size_of_one_expert(backend, tokens):
     l.check(_rng(tokens).standard_normal((tokens, 128)).astype(np.float32))
 
 
+@pytest.mark.parametrize("gt", [vb.Q8_0, vb.Q4_0])
+@pytest.mark.parametrize("experts,hidden,inner,top_k,tokens", [(8, 1536, 1376, 2, 6), (2, 512, 4800, 2, 11), (4, 160, 4000, 2, 5), (3, 96, 3424, 3, 8)])
+def test_units_that_four_warps_share(backend, gt, experts, hidden, inner, top_k, tokens):
+    """More units than thread blocks and columns that do not fill eight warps: two units of a block at a time."""
+    l = Layer(backend, experts, hidden, inner, top_k, True, gt, vb.Q8_0, max_tokens=tokens, seed=experts)
+    x = _rng(tokens).standard_normal((tokens, hidden)).astype(np.float32)
+    first = l.run(x)
+    l.check(x, first)
+    assert all(np.array_equal(a, b) for a, b in zip(first, l.run(x)))
+
+
 def test_calls_follow_each_other_and_repeat_bit_for_bit(backend):
     """Different token counts through one layer; the same call again gives the same bits."""
     l = Layer(backend, 16, 512, 256, 4, max_tokens=32, seed=2)

@@ -466,10 +466,10 @@ __device__ __forceinline__ void multiply(uint32_t codes, uint32_t j, const uint4
     });
 }
 
-// Sums of chunks c0, c0 + 8, .. < c1 of 32 rows of each of MATS matrices.  next() waits for the next stage of the ring and
+// Sums of chunks c0, c0 + TEAM, .. < c1 of 32 rows of each of MATS matrices.  next() waits for the next stage of the ring and
 // says where it is, done() gives it back.  `ahead` holds the vectors' first blocks; a block's place is filled with
 // the one that comes a group later as soon as it has been used.
-template <bool FOUR, bool WHOLE, int MATS, int NT, class Next, class Done>
+template <bool FOUR, bool WHOLE, int MATS, uint32_t TEAM, int NT, class Next, class Done>
 __device__ __forceinline__ void dot_chunks(Vectors<NT> x, Ahead<FOUR, MATS>& ahead, uint32_t nb, uint32_t c0, uint32_t c1, uint32_t lane,
                                            Next next, Done done, float (&acc)[MATS][2][NT][2]) {
     using S = Scales<FOUR, MATS, WHOLE>;
@@ -484,9 +484,9 @@ __device__ __forceinline__ void dot_chunks(Vectors<NT> x, Ahead<FOUR, MATS>& ahe
         for (int m = 0; m < 2; ++m)
 #pragma unroll
             for (int n = 0; n < NT; ++n) acc[a][m][n][0] = acc[a][m][n][1] = 0.0f;
-    for (uint32_t c = c0; c < c1; c += kMoeWarps) {
+    for (uint32_t c = c0; c < c1; c += TEAM) {
         const uint32_t stage = next(), codes = stage + lane_at;
-        const bool more = c + kMoeWarps < c1;
+        const bool more = c + TEAM < c1;
 #pragma unroll
         for (uint32_t j0 = 0; j0 < B; j0 += G)
 #pragma unroll
@@ -499,25 +499,25 @@ __device__ __forceinline__ void dot_chunks(Vectors<NT> x, Ahead<FOUR, MATS>& ahe
                         multiply<FOUR, MATS, NT>(codes + a * (kCodes / 2), j0 + j, ahead.parts + j * NT, ahead.factor + j * NT,
                                                  [&](int row) { return d(row, j); }, acc[a]);
                     if (a == MATS - 1) {
-                        const uint32_t later = j0 + j + (j0 + G < B ? G : kMoeWarps * B + G - B);
+                        const uint32_t later = j0 + j + (j0 + G < B ? G : TEAM * B + G - B);
                         if ((j0 + G < B || more) && (WHOLE || c * B + later < nb)) ahead.template load<NT>(x, later, j);
                     }
                 }
             }
-        x.advance(kMoeWarps * B);
+        x.advance(TEAM * B);
         done();
     }
 }
 
 // ------------------------------------------------------------------------------------------------- inner ----
-constexpr uint32_t kSums4 = kMoeWarps * 64 * 5;      // floats; two of them, or one for up to eight tokens
-constexpr uint32_t kInnerSums = std::max(2 * kSums4, kMoeWarps * 64 * (kGroup + 1)) * 4;
+constexpr uint32_t kSums4 = 64 * 5;  // floats of a warp; two of them, or one for up to eight tokens
+constexpr uint32_t kSums = std::max(2 * kSums4, 64 * (kGroup + 1)), kInnerSums = kMoeWarps * kSums * 4;
 template <bool FOUR, bool WHOLE>
 constexpr uint32_t kInnerSmem = kRing<FOUR, 2, WHOLE> + kInnerSums + sizeof(Plan);
 static_assert(plan_scratch(kMaxTokens) <= kMoeWarps * kStages * kCodes + kInnerSums, "the plan is made where ring and sums are later");
 
-// A pass over a unit's weights: 32 inner rows of an expert, up to kGroup of its tokens.  Block b of the grid has units
-// b, b + grid, ...
+// A pass over a unit's weights: 32 inner rows of an expert, up to kGroup of its tokens.  TEAM warps share its columns;
+// team k of all has units k, k + teams, ...
 struct InnerPass {
     uint32_t unit, a, at;  // a: expert number in the plan, at: of its list
     __device__ void enter(const Plan* plan, uint32_t tiles, uint32_t units) {
@@ -525,17 +525,17 @@ struct InnerPass {
         a = unit / tiles;
         at = plan->begin[a];
     }
-    __device__ void next(const Plan* plan, uint32_t tiles, uint32_t units) {
+    __device__ void next(const Plan* plan, uint32_t tiles, uint32_t units, uint32_t step) {
         at += kGroup;
         if (at < plan->begin[a + 1]) return;
-        unit += gridDim.x;
+        unit += step;
         enter(plan, tiles, units);
     }
     __device__ uint32_t count(const Plan* plan) const { return plan->begin[a + 1] - at; }
     __device__ uint32_t rows32(uint32_t tiles) const { return unit - a * tiles; }
 };
 
-template <bool FOUR, bool WHOLE>
+template <bool FOUR, bool WHOLE, uint32_t TEAM>
 __global__ void __launch_bounds__(kMoeThreads, 2) moe_inner_kernel(MoeParams p) {
     extern __shared__ __align__(128) uint8_t smem[];
     using C = Chunk<FOUR, 2>;
@@ -548,24 +548,26 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_inner_kernel(MoeParams p) 
     make_plan<false>(p, plan, reinterpret_cast<PlanScratch*>(smem), blockIdx.x == 0);
     const uint32_t nb = p.hidden / 32, chunks = C::count(nb), tiles = p.inner / 32, nbf = tiles, units = plan->active * tiles;
     const uint32_t ring = smem_addr(smem) + warp * kStages * kStage, row_bytes = nb * (FOUR ? 16 : 32);
-    float* sums = reinterpret_cast<float*>(smem + kRing);
+    const uint32_t team = warp / TEAM, member = warp % TEAM, step = gridDim.x * (kMoeWarps / TEAM);
+    float* sums = reinterpret_cast<float*>(smem + kRing) + team * TEAM * kSums;
+    auto barrier = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(TEAM * 32) : "memory"); };  // of the team
 
     // what is copied runs kStages chunks ahead of what is multiplied
     InnerPass ahead;
-    ahead.unit = blockIdx.x;
+    ahead.unit = blockIdx.x * (kMoeWarps / TEAM) + team;
     ahead.enter(plan, tiles, units);
     InnerPass now = ahead;
     size_t ahead_row = 0, ahead_at = 0;  // first row, the lane's 16 bytes of the chunk to come
     uint32_t ahead_c = 0, used = 0;
     auto start = [&]() {  // of the pass `ahead`
         ahead_row = (size_t)plan->expert[ahead.a] * p.inner + ahead.rows32(tiles) * 32;
-        ahead_at = (ahead_row + lane / C::units) * row_bytes + warp * C::bytes + lane % C::units * 16;
-        ahead_c = warp;
+        ahead_at = (ahead_row + lane / C::units) * row_bytes + member * C::bytes + lane % C::units * 16;
+        ahead_c = member;
     };
     if (ahead.unit < units) start();
     auto fetch = [&](uint32_t stage) {
-        if (ahead_c >= chunks && warp < chunks && ahead.unit < units) {
-            ahead.next(plan, tiles, units);
+        if (ahead_c >= chunks && member < chunks && ahead.unit < units) {
+            ahead.next(plan, tiles, units, step);
             if (ahead.unit < units) start();
         }
         if (ahead_c < chunks && ahead.unit < units) {
@@ -575,8 +577,8 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_inner_kernel(MoeParams p) 
             }
             S::fetch(p.gate.scales, ahead_row + lane, ahead_c * C::blocks, nb, stage + kCodes, lane);
             S::fetch(p.up.scales, ahead_row + lane, ahead_c * C::blocks, nb, stage + kCodes + 32 * S::pitch, lane);
-            ahead_at += kMoeWarps * C::bytes;
-            ahead_c += kMoeWarps;
+            ahead_at += TEAM * C::bytes;
+            ahead_c += TEAM;
         }
         cp_async_commit();
     };
@@ -592,8 +594,8 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_inner_kernel(MoeParams p) 
     };
     auto begin_ahead = [&]() {
         if (now.unit >= units) return;
-        if (now.count(plan) <= 4) vectors.start(begin(std::integral_constant<int, 1>()), warp, chunks, nb);
-        else vectors.start(begin(std::integral_constant<int, 2>()), warp, chunks, nb);
+        if (now.count(plan) <= 4) vectors.start(begin(std::integral_constant<int, 1>()), member, chunks, nb);
+        else vectors.start(begin(std::integral_constant<int, 2>()), member, chunks, nb);
     };
     begin_ahead();
     while (now.unit < units) {
@@ -613,13 +615,13 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_inner_kernel(MoeParams p) 
             constexpr int NT = decltype(groups)::value;
             float acc[2][2][NT][2];
             const Vectors<NT> x = begin(groups);
-            dot_chunks<FOUR, WHOLE, 2, NT>(x, vectors, nb, warp, chunks, lane, next, done, acc);
-            now.next(plan, tiles, units);
+            dot_chunks<FOUR, WHOLE, 2, TEAM, NT>(x, vectors, nb, member, chunks, lane, next, done, acc);
+            now.next(plan, tiles, units, step);
             begin_ahead();
-            // the eight warps' sums: gate rows 0..31, up rows 32..63
+            // the team's sums: gate rows 0..31, up rows 32..63
             constexpr uint32_t W = 4 * NT + 1;
-            if (NT > 1) __syncthreads();
-            float* to = sums + (NT > 1 ? 0 : turn * kSums4);
+            if (NT > 1) barrier();
+            float* to = sums + (NT > 1 ? 0 : turn * TEAM * kSums4);
 #pragma unroll
             for (int a = 0; a < 2; ++a)
 #pragma unroll
@@ -627,12 +629,12 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_inner_kernel(MoeParams p) 
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) to[(warp * 64 + a * 32 + m * 16 + h * 8 + g) * W + token_of<NT>(n, t)] = acc[a][m][n][h];
-            __syncthreads();
-            for (uint32_t i = warp; i < count; i += kMoeWarps) {
+                        for (int h = 0; h < 2; ++h) to[(member * 64 + a * 32 + m * 16 + h * 8 + g) * W + token_of<NT>(n, t)] = acc[a][m][n][h];
+            barrier();
+            for (uint32_t i = member; i < count; i += TEAM) {
                 float a = 0.0f, b = 0.0f;
 #pragma unroll
-                for (uint32_t w = 0; w < kMoeWarps; ++w) {
+                for (uint32_t w = 0; w < TEAM; ++w) {
                     a += to[(w * 64 + lane) * W + i];
                     b += to[(w * 64 + 32 + lane) * W + i];
                 }
@@ -641,7 +643,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_inner_kernel(MoeParams p) 
                 uint8_t* hi = p.hh + ((size_t)slot * 2 * nbf + rows32) * 64;
                 split_block(h, lane, p.down4 != 0, hi, hi + (size_t)nbf * 64, p.hs + (size_t)slot * nbf + rows32);
             }
-            if (NT > 1) __syncthreads();
+            if (NT > 1) barrier();
             turn ^= 1;
         };
         if (count <= 4) pass(std::integral_constant<int, 1>());
@@ -783,7 +785,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_down_kernel(MoeParams p) {
             constexpr int NT = decltype(groups)::value;
             float acc[1][2][NT][2];
             const Vectors<NT> x = begin(groups);
-            dot_chunks<FOUR, WHOLE, 1, NT>(x, vectors, nb, now.c0, now.c1, lane, next, done, acc);
+            dot_chunks<FOUR, WHOLE, 1, kMoeWarps, NT>(x, vectors, nb, now.c0, now.c1, lane, next, done, acc);
             now.next_pass(plan, chunks, lo, hi, warp);
             begin_ahead();
 #pragma unroll
@@ -834,17 +836,22 @@ struct Launch {
     MoeKernel kernel;
     uint32_t smem;
 };
+template <bool FOUR, bool WHOLE>
+Launch inner_of(uint32_t team) {
+    return {team == 8 ? moe_inner_kernel<FOUR, WHOLE, 8> : moe_inner_kernel<FOUR, WHOLE, 4>, kInnerSmem<FOUR, WHOLE>};
+}
 template <bool FOUR>
-Launch inner_of(uint32_t nb) {
-    if (nb % Chunk<FOUR, 2>::blocks == 0) return {moe_inner_kernel<FOUR, true>, kInnerSmem<FOUR, true>};
-    return {moe_inner_kernel<FOUR, false>, kInnerSmem<FOUR, false>};
+Launch inner_of(uint32_t nb, uint32_t team) {
+    return nb % Chunk<FOUR, 2>::blocks == 0 ? inner_of<FOUR, true>(team) : inner_of<FOUR, false>(team);
 }
 template <bool FOUR>
 Launch down_of(uint32_t nb, uint32_t tokens, uint32_t slots) {
     if (nb % Chunk<FOUR, 1>::blocks == 0) return {moe_down_kernel<FOUR, true>, down_smem<FOUR, true>(tokens, slots)};
     return {moe_down_kernel<FOUR, false>, down_smem<FOUR, false>(tokens, slots)};
 }
-Launch inner_launch(const MoeParams& p) { return p.gate4 ? inner_of<true>(p.hidden / 32) : inner_of<false>(p.hidden / 32); }
+Launch inner_launch(const MoeParams& p, uint32_t team) {
+    return p.gate4 ? inner_of<true>(p.hidden / 32, team) : inner_of<false>(p.hidden / 32, team);
+}
 Launch down_launch(const MoeParams& p, uint32_t tokens) {
     return p.down4 ? down_of<true>(p.inner / 32, tokens, tokens * p.top_k) : down_of<false>(p.inner / 32, tokens, tokens * p.top_k);
 }
@@ -905,9 +912,11 @@ vx_status vx_moe_create(vx_context* ctx, const float* router, size_t experts, co
     p.row_log = 2;
     while ((1u << p.row_log) < p.experts) ++p.row_log;
     int per_sm = 0;
-    const Launch inner_k = inner_launch(p);
-    VX_CUDA(cudaFuncSetAttribute(inner_k.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)inner_k.smem));
-    VX_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, inner_k.kernel, kMoeThreads, inner_k.smem));
+    for (uint32_t team : {4u, 8u}) {
+        const Launch inner = inner_launch(p, team);
+        VX_CUDA(cudaFuncSetAttribute(inner.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)inner.smem));
+        VX_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, inner.kernel, kMoeThreads, inner.smem));
+    }
     m->inner_grid = (uint32_t)std::max(1, per_sm) * m->sm_count;
     // for every layer of these types, so the most that any needs
     MoeParams most = p;
@@ -974,8 +983,16 @@ vx_status vx_moe_run(vx_context* ctx, const vx_moe* m, const float* x, size_t x_
     VX_CUDA(launch_after(moe_route_kernel, dim3(route_grid), kMoeThreads, 0, ctx->stream, p));
     // as many units as there can be experts with tokens
     const uint64_t units = (uint64_t)std::min<uint64_t>(p.experts, (uint64_t)p.tokens * p.top_k) * (p.inner / 32);
-    const uint32_t grid = (uint32_t)std::min<uint64_t>(units, m->inner_grid);
-    const Launch inner = inner_launch(p), down = down_launch(p, p.tokens);
+    // Eight warps share a unit's columns, or four do and a block has two units at a time: whichever takes fewer chunks one after the
+    // other (8 experts of 8192 x 512, two tokens: 20 us with four, 26 with eight; 8 of 14336 x 4096, 8 tokens: 219 and 205).
+    const uint32_t chunks = p.gate4 ? Chunk<true, 2>::count(p.hidden / 32) : Chunk<false, 2>::count(p.hidden / 32);
+    auto turns = [&](uint32_t team) {
+        const uint64_t at_once = (uint64_t)m->inner_grid * (kMoeWarps / team);
+        return (units + at_once - 1) / at_once * ((chunks + team - 1) / team);
+    };
+    const uint32_t team = turns(4) < turns(8) ? 4 : 8, teams = kMoeWarps / team;
+    const uint32_t grid = (uint32_t)std::min<uint64_t>((units + teams - 1) / teams, m->inner_grid);
+    const Launch inner = inner_launch(p, team), down = down_launch(p, p.tokens);
     VX_CUDA(launch_after(inner.kernel, dim3(grid), kMoeThreads, inner.smem, ctx->stream, p));
     VX_CUDA(launch_after(down.kernel, dim3(p.hidden / 32, p.splits), kMoeThreads, down.smem, ctx->stream, p, dim3(1, p.splits)));
     ctx->launches += 3;
