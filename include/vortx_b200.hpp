@@ -9,6 +9,7 @@
  *   Tensor<T>, TensorRef<T>, TensorMut<T> src/tensor/tensor_impl.rs:117-121, tensor_ref.rs:11-151, tensor_mut.rs:10-163
  *   Gemm, Reduce, OpAssign, Repeat, Contiguous   src/linalg/{gemm,reduce,op_assign,repeat,contiguous}.rs
  *   QuantizedMatrix, Gemv, GemvBatch      no reference counterpart (block-quantised weights)
+ *   QuantizedCache, CacheRows, CacheAttention, tree_mask, MoeLayer   no reference counterpart (a decode step)
  * Where the reference panics (assert_eq! on shapes, out-of-range axes) these throw: ShapeMismatch for
  * Gemm::dispatch's shape asserts (src/linalg/gemm.rs:70-104), Error otherwise.  Where the reference returns
  * None (unsqueeze, broadcast) these return an empty std::optional.  Nothing here computes on the host: a
@@ -467,6 +468,130 @@ public:
 private:
     vx_context* ctx_;
     vx_gemv_batch* batch_ = nullptr;
+};
+
+/* ------------------------------------------------------------------ a decode step ---- */
+/* Which tokens the rows of a call are (vx_kv_rows): table [seqs][max_pages], begin [seqs + 1], start [seqs], on the
+ * device and read when the call runs; the buffers must outlive the calls. */
+struct CacheRows {
+    vx_kv_rows c{};
+    CacheRows(const GpuBuffer<int32_t>& table, const GpuBuffer<int32_t>& begin, const GpuBuffer<int32_t>& start, size_t rows) {
+        const size_t seqs = start.len();
+        if (begin.len() < seqs + 1 || (seqs && table.len() < seqs))
+            throw Error(VX_ERR_OUT_OF_BOUNDS, "CacheRows: table or begin is shorter than the sequences need");
+        c.table = table.ptr();
+        c.max_pages = seqs ? table.len() / seqs : 0;
+        c.begin = begin.ptr();
+        c.start = start.ptr();
+        c.seqs = seqs;
+        c.rows = rows;
+    }
+};
+
+/* `n` rows of `width` elements, dense: the last dimension has stride 1 and there are as many elements. */
+template <class View>
+void check_rows(const char* what, const View& v, size_t n, size_t width) {
+    if (!v.is_contiguous() || v.len() < n * width) throw ShapeMismatch(VX_ERR_SHAPE, std::string(what) + " is not that many dense rows");
+}
+
+/* Keys and values in Q8_0 / Q4_0 blocks (vx_kv_cache). */
+class QuantizedCache {
+public:
+    QuantizedCache(const GpuBackend& b, vx_qtype k_type, vx_qtype v_type, size_t heads, size_t head_dim, size_t pages, size_t page_tokens = 64)
+        : ctx_(b.ctx()), width_(heads * head_dim), head_dim_(head_dim) {
+        check(vx_kv_cache_create(ctx_, k_type, v_type, heads, head_dim, pages, page_tokens, &c_));
+    }
+    QuantizedCache(const QuantizedCache&) = delete;
+    QuantizedCache& operator=(const QuantizedCache&) = delete;
+    ~QuantizedCache() {
+        if (c_) vx_kv_cache_free(ctx_, c_);
+    }
+    void append(const GpuBackend& b, const TensorRef<float>& k, const TensorRef<float>& v, const CacheRows& rows) const {
+        check_rows("QuantizedCache: k", k, rows.c.rows, width_);
+        check_rows("QuantizedCache: v", v, rows.c.rows, width_);
+        check(vx_kv_append(b.ctx(), c_, &rows.c, k.buffer(), width_, v.buffer(), width_));
+    }
+    void read(const GpuBackend& b, const TensorMut<float>& k, const TensorMut<float>& v, const CacheRows& rows) const {
+        check_rows("QuantizedCache: k", k, rows.c.rows, width_);
+        check_rows("QuantizedCache: v", v, rows.c.rows, width_);
+        check(vx_kv_read(b.ctx(), c_, &rows.c, k.buffer(), width_, v.buffer(), width_));
+    }
+    const vx_kv_cache* handle() const { return c_; }
+    size_t head_dim() const { return head_dim_; }
+
+private:
+    vx_context* ctx_;
+    vx_kv_cache* c_ = nullptr;
+    size_t width_, head_dim_;
+};
+
+/* The mask of a tree of drafted tokens: token i continues token parents[i] < i, or none (-1); a row has the bits of its token
+ * and that one's ancestors, (n + 31) / 32 words. */
+inline std::vector<uint32_t> tree_mask(const std::vector<int32_t>& parents) {
+    const size_t n = parents.size(), words = (n + 31) / 32;
+    std::vector<uint32_t> mask(n * words, 0);
+    for (size_t i = 0; i < n; ++i) {
+        if (parents[i] < -1 || parents[i] >= (int64_t)i) throw Error(VX_ERR_INVALID_ARGUMENT, "tree_mask: a token cannot continue a later one");
+        if (parents[i] >= 0)
+            for (size_t w = 0; w < words; ++w) mask[i * words + w] = mask[(size_t)parents[i] * words + w];
+        mask[i * words + i / 32] |= 1u << (i % 32);
+    }
+    return mask;
+}
+
+/* Attention of new or drafted tokens over the cache, which must outlive it (vx_kv_attention). */
+class CacheAttention {
+public:
+    CacheAttention(const GpuBackend& b, const QuantizedCache& cache, size_t heads, size_t max_seqs)
+        : ctx_(b.ctx()), width_(heads * cache.head_dim()) {
+        check(vx_kv_attention_create(ctx_, cache.handle(), heads, max_seqs, &a_));
+    }
+    CacheAttention(const CacheAttention&) = delete;
+    CacheAttention& operator=(const CacheAttention&) = delete;
+    ~CacheAttention() {
+        if (a_) vx_kv_attention_free(ctx_, a_);
+    }
+    /* mask null: a row attends to its sequence's tokens up to itself. */
+    void dispatch(const GpuBackend& b, const TensorMut<float>& out, const TensorRef<float>& q, const CacheRows& rows, float scale,
+                  const GpuBuffer<uint32_t>* mask = nullptr) const {
+        check_rows("CacheAttention: q", q, rows.c.rows, width_);
+        check_rows("CacheAttention: out", out, rows.c.rows, width_);
+        const size_t words = mask && rows.c.rows ? mask->len() / rows.c.rows : 0;
+        check(vx_kv_attention_run(b.ctx(), a_, &rows.c, q.buffer(), width_, out.buffer(), width_, scale, mask ? mask->ptr() : nullptr, words));
+    }
+
+private:
+    vx_context* ctx_;
+    vx_kv_attention* a_ = nullptr;
+    size_t width_;
+};
+
+/* A routed layer of gated experts (vx_moe); router and weights must outlive it. */
+class MoeLayer {
+public:
+    MoeLayer(const GpuBackend& b, const TensorRef<float>& router, const QuantizedMatrix& gate, const QuantizedMatrix& up, const QuantizedMatrix& down,
+             size_t experts, size_t top_k, bool normalise = true, size_t max_tokens = 32)
+        : ctx_(b.ctx()), hidden_(gate.cols()), top_k_(top_k) {
+        check_rows("MoeLayer: router", router, experts, hidden_);
+        check(vx_moe_create(ctx_, router.buffer(), experts, gate.handle(), up.handle(), down.handle(), top_k, normalise, max_tokens, &m_));
+    }
+    MoeLayer(const MoeLayer&) = delete;
+    MoeLayer& operator=(const MoeLayer&) = delete;
+    ~MoeLayer() {
+        if (m_) vx_moe_free(ctx_, m_);
+    }
+    /* ids (null: not wanted): [tokens][top_k], the chosen experts, best first. */
+    void dispatch(const GpuBackend& b, const TensorMut<float>& y, const TensorRef<float>& x, size_t tokens, const GpuBuffer<int32_t>* ids = nullptr) const {
+        check_rows("MoeLayer: x", x, tokens, hidden_);
+        check_rows("MoeLayer: y", y, tokens, hidden_);
+        if (ids && ids->len() < tokens * top_k_) throw Error(VX_ERR_OUT_OF_BOUNDS, "MoeLayer: ids is shorter than tokens * top_k");
+        check(vx_moe_run(b.ctx(), m_, x.buffer(), hidden_, y.buffer(), hidden_, tokens, ids ? ids->ptr() : nullptr, nullptr));
+    }
+
+private:
+    vx_context* ctx_;
+    vx_moe* m_ = nullptr;
+    size_t hidden_, top_k_;
 };
 
 }  // namespace vortx

@@ -1,15 +1,15 @@
 // A mixture-of-experts layer for a few tokens on block-quantised weights, in three launches:
 //   route   logits = router x, in slices of the columns, and x split into two f16 parts per block of 32
-//   inner   silu(gate x) * (up x): a thread block per (expert with tokens, 32 inner rows)
+//   inner   silu(gate x) * (up x): four or eight warps per (expert with tokens, 32 inner rows)
 //   down    y = sum weight * (down h): a thread block per (32 output rows, share of all experts' columns)
-// Every block of the last two picks the experts from the logits itself (less than one block doing it for all would
-// cost in waiting), and the down kernel does so, and starts to copy its
-// weights, while the inner kernel still runs.
+// Every block of the last two picks the experts from the logits itself (2.5 us; less than one block doing it for all would
+// cost in waiting), and the down kernel does so, and starts to copy its weights, while the inner kernel still runs.
 //
-// Bound by the weights' bytes: each is read once per 8 tokens of its expert.  In both products a warp has every
-// eighth 128-byte column chunk of the unit's rows (16-byte cp.async copies that run ahead over the ends of units and
-// experts, no synchronisation between warps until the sums are added up).  On the tensor cores (m16n8k16) 16 rows of
-// codes are A; columns 2 i and 2 i + 1 of B are the two parts of token i, so a thread holds both sums of a (row, token).
+// The weights' bytes are the floor: each is read once per 8 tokens of its expert.  In both products a warp has every
+// fourth or eighth chunk of the columns (64 bytes of a gate and an up row, 128 of a down row; codes and scales by
+// cp.async copies that run ahead over the ends of units and experts; no synchronisation between warps until the
+// sums are added up).  On the tensor cores (m16n8k16) 16 rows of codes are A; B's columns are the two parts of four
+// tokens, or eight tokens, whose parts are then multiplied one after the other into the same sums.
 // A code u (code + 8 or + 128, not negative) is used as the f16 number whose bits it is, u 2^-20 (nibbles moved to bits
 // 4..7) or u 2^-24: a shift and a logic operation, or a byte permutation, per pair and no conversion.  The offset's
 // part of a block's sum, 8 or 128 times the sum of the vector's parts, is taken off with the multiplication that scales
@@ -17,6 +17,11 @@
 // align products by the exponent field, so the leading zeros of such a number are lost bits (two of 24 for the
 // middle codes): 5e-7 relative to the exact result, 2e-7 with converted codes.  Nibbles left at bits 0..3 lose six more
 // bits: 6e-6.
+// Measured (recorded calls): 8 tokens, 2 of 8 experts of 14336 x 4096, Q4_0 gate and up, Q8_0 down: inner 122 us (3.8 TB/s),
+// down 77 us (5.7 TB/s); 32 tokens, 4 of 32 experts of 1408 x 2048, Q4_0: inner 47 us, down 35 us; one token of 4 such
+// experts: 20 us, of which 5 are the router's.  Reading the weights takes 0.58 of the memory's rate in the inner kernel, which is bound by
+// its instructions (78 per 32 x 32 weights, 28 of them to take the codes apart, at 0.53 a cycle and scheduler: 128
+// registers leave four warps to hide latencies), 0.87 in the down kernel.
 #include <algorithm>
 #include <cstddef>
 #include <memory>
