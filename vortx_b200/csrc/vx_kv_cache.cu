@@ -49,27 +49,28 @@ __device__ __forceinline__ uint16_t scale_of(float top, float n, float inv_n) {
     if (off <= 16u || !(fabsf(q) >= 6.2e-5f)) q = __fdiv_rn(top, n);  // f16's small numbers have other borders
     return __half_as_ushort(__float2half_rn(q));
 }
-// The codes of four values, offset included: round half away from zero of v / d; r is 1 / d to 2^-22.
+// The codes of eight values, offset included: round half away from zero of v / d; r is 1 / d to 2^-22.
 template <bool FOUR>
-__device__ __forceinline__ void codes_of(const float (&v)[4], float d, float r, uint32_t (&c)[4]) {
-    int n[4];
+__device__ __forceinline__ void codes_of(const float (&v)[8], float d, float r, uint32_t (&c)[8]) {
+    int n[8];
     float off = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 8; ++i) {
         const float x = v[i] * r, y = x + 12582912.0f;  // 1.5 2^23: the integer nearest to x in the low bits
         n[i] = (int)(__float_as_uint(y) - 0x4b400000u);
         off = fmaxf(off, fabsf(x - (y - 12582912.0f)));
     }
     if (off > 0.4999f) {  // one of them next to a tie
 #pragma unroll
-        for (int i = 0; i < 4; ++i) n[i] = (int)roundf(__fdiv_rn(v[i], d));
+        for (int i = 0; i < 8; ++i) n[i] = (int)roundf(__fdiv_rn(v[i], d));
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) c[i] = (uint32_t)(FOUR ? min(15, max(0, n[i] + 8)) : min(127, max(-127, n[i])) + 128);
+    for (int i = 0; i < 8; ++i) c[i] = (uint32_t)(FOUR ? min(15, max(0, n[i] + 8)) : min(127, max(-127, n[i])) + 128);
 }
+__device__ __forceinline__ uint32_t word_of(const uint32_t (&c)[8], int i) { return c[i] | c[i + 1] << 8 | c[i + 2] << 16 | c[i + 3] << 24; }
 
 // Pairs (token, block) that a thread has under way at a time.
-constexpr uint32_t kBatch = 4;
+constexpr uint32_t kBatch = 2, kStep = kThreads / 4;
 
 // p / blocks for a pair's number p < 32 blocks <= 512: the error of the rounded-up reciprocal stays below 1 / blocks.
 struct PerToken {
@@ -81,66 +82,81 @@ struct PerToken {
 template <bool FOUR, bool VALUES>
 __device__ __forceinline__ void append_part(const KvRows& r, const KvGeometry& g, const TileOf& o, uint8_t* dst, const float* __restrict__ src,
                                             size_t stride, uint32_t head, bool vec, uint8_t* image) {
-    const uint32_t oct = threadIdx.x / 8, j = threadIdx.x % 8, lane = threadIdx.x % 32, nb = g.blocks;
+    const uint32_t quad = threadIdx.x / 4, j = threadIdx.x % 4, lane = threadIdx.x % 32, nb = g.blocks;
     const bool whole = o.t0 == 0 && o.t1 == 32;
     uint8_t* to = whole ? image : dst;
     const uint32_t scales = kv_code_bytes(FOUR, nb), end = o.t1 * nb;
     const PerToken per(nb);
-    for (uint32_t p0 = o.t0 * nb; p0 < end; p0 += kBatch * kThreads / 8) {
-        float v[kBatch][4];
+    src += (size_t)head * nb * 32 + j * 4;
+    for (uint32_t p0 = o.t0 * nb; p0 < end; p0 += kBatch * kStep) {
+        float v[kBatch][8];  // values 4 j .. 4 j + 3 and 16 + 4 j .. of a block
 #pragma unroll
         for (uint32_t i = 0; i < kBatch; ++i) {
-            const uint32_t p = p0 + i * (kThreads / 8) + oct;
-            v[i][0] = v[i][1] = v[i][2] = v[i][3] = 0.0f;
+            const uint32_t p = p0 + i * kStep + quad;
+#pragma unroll
+            for (int n = 0; n < 8; ++n) v[i][n] = 0.0f;
             if (p < end) {
                 const uint32_t token = per.token(p), block = p - token * nb;
                 const uint32_t row = o.q.row0 + (o.tile * 32 + token - o.q.first);
-                const float* from = src + (size_t)row * stride + (size_t)head * nb * 32 + block * 32 + j * 4;
-                if (vec) {
-                    const float4 f = __ldcs(reinterpret_cast<const float4*>(from));
-                    v[i][0] = f.x; v[i][1] = f.y; v[i][2] = f.z; v[i][3] = f.w;
-                } else {
+                const float* from = src + (size_t)row * stride + block * 32;
 #pragma unroll
-                    for (int n = 0; n < 4; ++n) v[i][n] = __ldcs(from + n);
+                for (int h = 0; h < 2; ++h) {
+                    if (vec) {
+                        const float4 f = __ldcs(reinterpret_cast<const float4*>(from + 16 * h));
+                        v[i][4 * h] = f.x; v[i][4 * h + 1] = f.y; v[i][4 * h + 2] = f.z; v[i][4 * h + 3] = f.w;
+                    } else {
+#pragma unroll
+                        for (int n = 0; n < 4; ++n) v[i][4 * h + n] = __ldcs(from + 16 * h + n);
+                    }
                 }
             }
         }
 #pragma unroll
         for (uint32_t i = 0; i < kBatch; ++i) {
-            const uint32_t p = p0 + i * (kThreads / 8) + oct, token = per.token(p), block = p - token * nb;
+            const uint32_t p = p0 + i * kStep + quad, token = per.token(p), block = p - token * nb;
             // the largest magnitude as bits: infinities and NaN come out on top
-            uint32_t mine = 0;
+            uint32_t most = 0;
 #pragma unroll
-            for (int n = 0; n < 4; ++n) mine = max(mine, __float_as_uint(v[i][n]) & 0x7fffffffu);
-            uint32_t most = mine;
-#pragma unroll
-            for (int x = 1; x < 8; x *= 2) most = max(most, __shfl_xor_sync(0xffffffffu, most, x));
+            for (int n = 0; n < 8; ++n) most = max(most, __float_as_uint(v[i][n]) & 0x7fffffffu);
+            most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+            most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
             float top = __uint_as_float(most);
             if (FOUR) {  // with its sign: the first element of that magnitude
-                float with = 0.0f;
+                float with[2] = {0.0f, 0.0f};
+                bool has[2] = {false, false};
 #pragma unroll
-                for (int n = 3; n >= 0; --n)
-                    if ((__float_as_uint(v[i][n]) & 0x7fffffffu) == most) with = v[i][n];
-                const uint32_t lanes = __ballot_sync(0xffffffffu, mine == most) >> (lane & 24u);
-                top = __shfl_sync(0xffffffffu, with, (lane & 24u) + __ffs(lanes & 0xffu) - 1);
+                for (int n = 7; n >= 0; --n)
+                    if ((__float_as_uint(v[i][n]) & 0x7fffffffu) == most) {
+                        with[n / 4] = v[i][n];
+                        has[n / 4] = true;
+                    }
+                const uint32_t first = __ballot_sync(0xffffffffu, has[0]) >> (lane & 28u) & 15u, second = __ballot_sync(0xffffffffu, has[1]) >> (lane & 28u) & 15u;
+                top = __shfl_sync(0xffffffffu, first ? with[0] : with[1], (lane & 28u) + __ffs(first ? first : second) - 1);
             }
             uint16_t dh = scale_of(top, FOUR ? 7.0f : 127.0f, FOUR ? 1.0f / 7.0f : 1.0f / 127.0f);
             if ((dh & 0x7fffu) >= 0x7c00u) dh = 0x7fffu;
             const bool zero = dh == 0x7fffu || (dh & 0x7fffu) == 0;  // no number, or nothing but zeros
             const float d = zero ? 1.0f : __half2float(__ushort_as_half(dh)), inv = __fdividef(1.0f, d);
-            uint32_t c[4];
-            if (zero) v[i][0] = v[i][1] = v[i][2] = v[i][3] = 0.0f;
+            uint32_t c[8];
+            if (zero) {
+#pragma unroll
+                for (int n = 0; n < 8; ++n) v[i][n] = 0.0f;
+            }
             codes_of<FOUR>(v[i], d, inv, c);
-            uint32_t w = c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;
-            if (FOUR && !VALUES) w |= __shfl_xor_sync(0xffffffffu, w, 4) << 4;  // byte i of a Q4_0 block: values i and i + 16
             if (p >= end) continue;
             if (VALUES && FOUR) {
-                *reinterpret_cast<uint16_t*>(to + v_word(true, block, token, j)) = (uint16_t)(c[0] | c[1] << 4 | c[2] << 8 | c[3] << 12);
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    *reinterpret_cast<uint16_t*>(to + v_word(true, block, token, j + 4 * h)) =
+                        (uint16_t)(c[4 * h] | c[4 * h + 1] << 4 | c[4 * h + 2] << 8 | c[4 * h + 3] << 12);
             } else if (VALUES) {
 #pragma unroll
-                for (int n = 0; n < 4; ++n) to[v_word(false, block, token, j) + 4 * n] = (uint8_t)c[n];
-            } else if (!FOUR || j < 4) {
-                *reinterpret_cast<uint32_t*>(to + k_word(FOUR, block, token, j)) = w;
+                for (int n = 0; n < 8; ++n) to[v_word(false, block, token, j + n / 4 * 4) + 4 * (n % 4)] = (uint8_t)c[n];
+            } else if (FOUR) {  // byte i of a Q4_0 block: values i and i + 16
+                *reinterpret_cast<uint32_t*>(to + k_word(true, block, token, j)) = word_of(c, 0) | word_of(c, 4) << 4;
+            } else {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) *reinterpret_cast<uint32_t*>(to + k_word(false, block, token, j + 4 * h)) = word_of(c, 4 * h);
             }
             if (j == 0) *reinterpret_cast<uint16_t*>(to + scales + (VALUES ? v_scale(block, token) : k_scale(block, token))) = dh;
         }
@@ -186,47 +202,54 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(KvAppend p) {
 template <bool FOUR, bool VALUES>
 __device__ __forceinline__ void read_part(const KvGeometry& g, const TileOf& o, const uint8_t* src, float* __restrict__ dst, size_t stride,
                                           uint32_t head, bool vec) {
-    const uint32_t oct = threadIdx.x / 8, j = threadIdx.x % 8, nb = g.blocks;
+    const uint32_t quad = threadIdx.x / 4, j = threadIdx.x % 4, nb = g.blocks;
     const uint32_t scales = kv_code_bytes(FOUR, nb), end = o.t1 * nb;
     const PerToken per(nb);
-    for (uint32_t p0 = o.t0 * nb; p0 < end; p0 += kBatch * kThreads / 8) {
-        uint32_t w[kBatch], dh[kBatch];  // straight from the record: its neighbours' words come along in the L1
+    dst += (size_t)head * nb * 32 + j * 4;
+    for (uint32_t p0 = o.t0 * nb; p0 < end; p0 += kBatch * kStep) {
+        uint32_t w[kBatch][2], dh[kBatch];  // straight from the record: its neighbours' words come along in the L1
 #pragma unroll
         for (uint32_t i = 0; i < kBatch; ++i) {
-            const uint32_t p = p0 + i * (kThreads / 8) + oct, token = per.token(p), block = p - token * nb;
-            w[i] = FOUR ? 0x88888888u : 0x80808080u;  // zeros, for tokens without a place
+            const uint32_t p = p0 + i * kStep + quad, token = per.token(p), block = p - token * nb;
+            w[i][0] = w[i][1] = FOUR ? 0x88888888u : 0x80808080u;  // zeros, for tokens without a place
             dh[i] = 0;
             if (src && p < end) {
                 dh[i] = *reinterpret_cast<const uint16_t*>(src + scales + (VALUES ? v_scale(block, token) : k_scale(block, token)));
-                if (VALUES && FOUR) {
-                    w[i] = *reinterpret_cast<const uint16_t*>(src + v_word(true, block, token, j));
-                } else if (VALUES) {
-                    const uint8_t* at = src + v_word(false, block, token, j);
-                    w[i] = at[0] | (uint32_t)at[4] << 8 | (uint32_t)at[8] << 16 | (uint32_t)at[12] << 24;
-                } else {
-                    w[i] = *reinterpret_cast<const uint32_t*>(src + k_word(FOUR, block, token, FOUR ? j % 4 : j));
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if (VALUES && FOUR) {
+                        w[i][h] = *reinterpret_cast<const uint16_t*>(src + v_word(true, block, token, j + 4 * h));
+                    } else if (VALUES) {
+                        const uint8_t* at = src + v_word(false, block, token, j + 4 * h);
+                        w[i][h] = at[0] | (uint32_t)at[4] << 8 | (uint32_t)at[8] << 16 | (uint32_t)at[12] << 24;
+                    } else if (!FOUR || h == 0) {
+                        w[i][h] = *reinterpret_cast<const uint32_t*>(src + k_word(FOUR, block, token, FOUR ? j : j + 4 * h));
+                    }
                 }
             }
         }
 #pragma unroll
         for (uint32_t i = 0; i < kBatch; ++i) {
-            const uint32_t p = p0 + i * (kThreads / 8) + oct, token = per.token(p), block = p - token * nb;
+            const uint32_t p = p0 + i * kStep + quad, token = per.token(p), block = p - token * nb;
             if (p >= end) continue;
             const uint32_t row = o.q.row0 + (o.tile * 32 + token - o.q.first);
             const float d = __half2float(__ushort_as_half((uint16_t)dh[i]));
-            float f[4];
+            float* to = dst + (size_t)row * stride + block * 32;
 #pragma unroll
-            for (int n = 0; n < 4; ++n) {
-                const uint32_t shift = !FOUR ? 8 * n : VALUES ? 4 * n : 8 * n + (j < 4 ? 0 : 4);
-                const uint32_t u = (w[i] >> shift) & (FOUR ? 15u : 255u);
-                f[n] = __fmul_rn(d, __uint_as_float(u | 0x4b000000u) - (FOUR ? 8388616.0f : 8388736.0f));  // 2^23 + u
-            }
-            float* to = dst + (size_t)row * stride + (size_t)head * nb * 32 + block * 32 + j * 4;
-            if (vec) {
-                __stcs(reinterpret_cast<float4*>(to), make_float4(f[0], f[1], f[2], f[3]));
-            } else {
+            for (int h = 0; h < 2; ++h) {
+                float f[4];
 #pragma unroll
-                for (int n = 0; n < 4; ++n) __stcs(to + n, f[n]);
+                for (int n = 0; n < 4; ++n) {
+                    const uint32_t shift = !FOUR ? 8 * n : VALUES ? 4 * n : 8 * n + 4 * h;
+                    const uint32_t u = (w[i][FOUR && !VALUES ? 0 : h] >> shift) & (FOUR ? 15u : 255u);
+                    f[n] = __fmul_rn(d, __uint_as_float(u | 0x4b000000u) - (FOUR ? 8388616.0f : 8388736.0f));  // 2^23 + u
+                }
+                if (vec) {
+                    __stcs(reinterpret_cast<float4*>(to + 16 * h), make_float4(f[0], f[1], f[2], f[3]));
+                } else {
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) __stcs(to + 16 * h + n, f[n]);
+                }
             }
         }
     }
