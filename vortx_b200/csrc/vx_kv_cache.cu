@@ -46,28 +46,76 @@ __device__ __forceinline__ TileOf tile_of(const KvRows& r, const KvGeometry& g, 
 __device__ __forceinline__ uint16_t scale_of(float top, float n, float inv_n) {
     float q = top * inv_n;
     const uint32_t off = (__float_as_uint(q) & 0x1fffu) - 0x0ff8u;
-    if (off <= 16u || !(fabsf(q) >= 6.2e-5f)) q = __fdiv_rn(top, n);  // f16's small numbers have other borders
+    if (off <= 16u || (!(fabsf(q) >= 6.2e-5f) && q != 0.0f)) q = __fdiv_rn(top, n);  // f16's small numbers have other borders
     return __half_as_ushort(__float2half_rn(q));
 }
-// The codes of eight values, offset included: round half away from zero of v / d; r is 1 / d to 2^-22.
+// The codes of eight values in the words' low bytes, offset included: round half away from zero of v / d; r is 1 / d to 2^-22.
+// `special`: the scale is no number, and all codes are zeros, or one of f16's small ones, whose error can take a code out
+// of its range; else the largest is 7 or 127 (1 + 2^-11) before it is rounded.
 template <bool FOUR>
-__device__ __forceinline__ void codes_of(const float (&v)[8], float d, float r, uint32_t (&c)[8]) {
-    int n[8];
+__device__ __forceinline__ void codes_of(const float (&v)[8], float d, float r, bool special, uint32_t (&c)[8]) {
+    constexpr float kMagic = 12582912.0f + (FOUR ? 8.0f : 128.0f);  // 1.5 2^23: the nearest integer in the sum's low bits
     float off = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const float x = v[i] * r, y = x + 12582912.0f;  // 1.5 2^23: the integer nearest to x in the low bits
-        n[i] = (int)(__float_as_uint(y) - 0x4b400000u);
-        off = fmaxf(off, fabsf(x - (y - 12582912.0f)));
+        const float y = fmaf(v[i], r, kMagic);
+        c[i] = __float_as_uint(y);
+        off = fmaxf(off, fabsf(fmaf(v[i], r, kMagic - y)));
     }
-    if (off > 0.4999f) {  // one of them next to a tie
+    if (off > 0.4999f || special) {  // one of them next to a tie
 #pragma unroll
-        for (int i = 0; i < 8; ++i) n[i] = (int)roundf(__fdiv_rn(v[i], d));
+        for (int i = 0; i < 8; ++i) {
+            const int n = d == d ? (int)roundf(__fdiv_rn(v[i], d)) : 0;
+            c[i] = (uint32_t)(FOUR ? min(15, max(0, n + 8)) : min(127, max(-127, n)) + 128);
+        }
     }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = (uint32_t)(FOUR ? min(15, max(0, n[i] + 8)) : min(127, max(-127, n[i])) + 128);
 }
-__device__ __forceinline__ uint32_t word_of(const uint32_t (&c)[8], int i) { return c[i] | c[i + 1] << 8 | c[i + 2] << 16 | c[i + 3] << 24; }
+// Four low bytes.
+__device__ __forceinline__ uint32_t word_of(const uint32_t (&c)[8], int i) {
+    return __byte_perm(__byte_perm(c[i], c[i + 1], 0x0040), __byte_perm(c[i + 2], c[i + 3], 0x0040), 0x5410);
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+// The largest magnitude of a block that four lanes share, for Q4_0 with the sign of the first element that has it; NaN if
+// there is one.
+template <bool FOUR>
+__device__ __forceinline__ float largest_of(const float (&v)[8], uint32_t lane, bool there) {
+    float high = FOUR ? v[0] : fabsf(v[0]), low = v[0];
+#pragma unroll
+    for (int n = 1; n < 8; ++n) {
+        high = max_nan(high, FOUR ? v[n] : fabsf(v[n]));
+        if (FOUR) low = min_nan(low, v[n]);
+    }
+#pragma unroll
+    for (int x = 1; x < 4; x *= 2) {
+        high = max_nan(high, __shfl_xor_sync(0xffffffffu, high, x));
+        if (FOUR) low = min_nan(low, __shfl_xor_sync(0xffffffffu, low, x));
+    }
+    if (!FOUR) return high;
+    float top = high > -low ? high : low;
+    if (__any_sync(0xffffffffu, there && high == -low)) {  // both signs (or zeros): which comes first
+        float with[2] = {0.0f, 0.0f};
+        bool has[2] = {false, false};
+#pragma unroll
+        for (int n = 7; n >= 0; --n)
+            if (fabsf(v[n]) == fabsf(top)) {
+                with[n / 4] = v[n];
+                has[n / 4] = true;
+            }
+        const uint32_t first = __ballot_sync(0xffffffffu, has[0]) >> (lane & 28u) & 15u, second = __ballot_sync(0xffffffffu, has[1]) >> (lane & 28u) & 15u;
+        const float one = __shfl_sync(0xffffffffu, first ? with[0] : with[1], (lane & 28u) + (first | second ? __ffs(first ? first : second) - 1 : 0));
+        if (first | second) top = one;  // else NaN
+    }
+    return top;
+}
 
 // Pairs (token, block) that a thread has under way at a time.
 constexpr uint32_t kBatch = 2, kStep = kThreads / 4;
@@ -114,41 +162,20 @@ __device__ __forceinline__ void append_part(const KvRows& r, const KvGeometry& g
 #pragma unroll
         for (uint32_t i = 0; i < kBatch; ++i) {
             const uint32_t p = p0 + i * kStep + quad, token = per.token(p), block = p - token * nb;
-            // the largest magnitude as bits: infinities and NaN come out on top
-            uint32_t most = 0;
-#pragma unroll
-            for (int n = 0; n < 8; ++n) most = max(most, __float_as_uint(v[i][n]) & 0x7fffffffu);
-            most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-            most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-            float top = __uint_as_float(most);
-            if (FOUR) {  // with its sign: the first element of that magnitude
-                float with[2] = {0.0f, 0.0f};
-                bool has[2] = {false, false};
-#pragma unroll
-                for (int n = 7; n >= 0; --n)
-                    if ((__float_as_uint(v[i][n]) & 0x7fffffffu) == most) {
-                        with[n / 4] = v[i][n];
-                        has[n / 4] = true;
-                    }
-                const uint32_t first = __ballot_sync(0xffffffffu, has[0]) >> (lane & 28u) & 15u, second = __ballot_sync(0xffffffffu, has[1]) >> (lane & 28u) & 15u;
-                top = __shfl_sync(0xffffffffu, first ? with[0] : with[1], (lane & 28u) + __ffs(first ? first : second) - 1);
-            }
+            const float top = largest_of<FOUR>(v[i], lane, p < end);
             uint16_t dh = scale_of(top, FOUR ? 7.0f : 127.0f, FOUR ? 1.0f / 7.0f : 1.0f / 127.0f);
             if ((dh & 0x7fffu) >= 0x7c00u) dh = 0x7fffu;
-            const bool zero = dh == 0x7fffu || (dh & 0x7fffu) == 0;  // no number, or nothing but zeros
-            const float d = zero ? 1.0f : __half2float(__ushort_as_half(dh)), inv = __fdividef(1.0f, d);
+            // without a scale (all zeros, or too small for one) the codes are those of zeros
+            const uint32_t size = dh & 0x7fffu;
+            const float d = size == 0 ? 1.0f : __half2float(__ushort_as_half(dh)), inv = __fdividef(1.0f, d);
             uint32_t c[8];
-            if (zero) {
-#pragma unroll
-                for (int n = 0; n < 8; ++n) v[i][n] = 0.0f;
-            }
-            codes_of<FOUR>(v[i], d, inv, c);
+            codes_of<FOUR>(v[i], d, inv, size - 1 < 0x3ffu || size == 0x7fffu, c);
             if (p >= end) continue;
             if (VALUES && FOUR) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
                     *reinterpret_cast<uint16_t*>(to + v_word(true, block, token, j + 4 * h)) =
-                        (uint16_t)(c[4 * h] | c[4 * h + 1] << 4 | c[4 * h + 2] << 8 | c[4 * h + 3] << 12);
+                        (uint16_t)__byte_perm((c[4 * h] & 15u) | c[4 * h + 1] << 4, (c[4 * h + 2] & 15u) | c[4 * h + 3] << 4, 0x0040);
             } else if (VALUES) {
 #pragma unroll
                 for (int n = 0; n < 8; ++n) to[v_word(false, block, token, j + n / 4 * 4) + 4 * (n % 4)] = (uint8_t)c[n];
