@@ -479,6 +479,7 @@ struct CacheRows {
         const size_t seqs = start.len();
         if (begin.len() < seqs + 1 || (seqs && table.len() < seqs))
             throw Error(VX_ERR_OUT_OF_BOUNDS, "CacheRows: table or begin is shorter than the sequences need");
+        if (seqs && table.len() % seqs) throw Error(VX_ERR_INVALID_ARGUMENT, "CacheRows: not the same number of pages for every sequence");
         c.table = table.ptr();
         c.max_pages = seqs ? table.len() / seqs : 0;
         c.begin = begin.ptr();
@@ -557,6 +558,7 @@ public:
         check_rows("CacheAttention: q", q, rows.c.rows, width_);
         check_rows("CacheAttention: out", out, rows.c.rows, width_);
         const size_t words = mask && rows.c.rows ? mask->len() / rows.c.rows : 0;
+        if (mask && mask->len() != words * rows.c.rows) throw Error(VX_ERR_INVALID_ARGUMENT, "CacheAttention: not the same number of words for every row");
         check(vx_kv_attention_run(b.ctx(), a_, &rows.c, q.buffer(), width_, out.buffer(), width_, scale, mask ? mask->ptr() : nullptr, words));
     }
 

@@ -66,6 +66,7 @@ def test_rows_struct():
     (ValueError, (0x1000, 0x1000, 0x1000, 1), {"max_pages": 1}),
     (ValueError, (0x1000, 0x1000, 0x1000, 1), {"seqs": 1}),
     (ValueError, (_i32(1), _i32(2), _i32(1), -1), {}),
+    (ValueError, (_i32(7), _i32(4), _i32(3), 1), {}),                    # not the same number of pages each
     (ValueError, (0x1000, 0x1000, 0x1000, 1), {"seqs": -1, "max_pages": 1}),
 ])
 def test_rows_refuse(error, args, kw):
@@ -105,6 +106,8 @@ def test_freed_and_short_are_refused():
         att.dispatch(_NoBackend(), None, _buf(3 * 256), _buf(3 * 256), rows)
     with pytest.raises(ValueError):
         att.dispatch(_NoBackend(), None, _buf(3 * 256), _buf(3 * 256), rows, mask=0x1000)
+    with pytest.raises(ValueError, match="words"):
+        att.dispatch(_NoBackend(), None, _buf(3 * 256), _buf(3 * 256), rows, mask=_buf(4, np.uint32))
     layer = vb.MoeLayer.__new__(vb.MoeLayer)
     w = vb.QuantizedMatrix.__new__(vb.QuantizedMatrix)
     w._h, w.backend = None, _NoBackend()

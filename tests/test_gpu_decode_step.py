@@ -276,3 +276,51 @@ def test_a_workspace_each_for_graphs_at_the_same_time(backend):
         q.free()
         out.free()
         b.close()
+
+
+FIRST_CALL = """
+import sys, numpy as np, torch, vortx_b200 as vb
+from test_gpu_decode_step import Decoder, _read
+torch.zeros(1, device="cuda")
+stream = torch.cuda.Stream()
+with vb.Backend(0, stream=stream.cuda_stream) as b:
+    d = Decoder(b, 2, 2, seed=3)
+    rows = d.rows(b.init_buffer(np.array([0, 1, 2], np.int32)), b.init_buffer(np.array([0, 40], np.int32)), 2)
+    rng = np.random.Generator(np.random.Philox(1))
+    for t in (d.k, d.v, d.q, d.p):
+        b.write_buffer(t, 0, rng.standard_normal(t.len()).astype(np.float32))
+    b.synchronize()
+    width = d.heads * d.dim
+    def calls():
+        d.cache.append(None, d.k, d.v, rows, k_stride=width, v_stride=width)
+        d.attention.dispatch(b, None, d.a, d.q, rows)
+        d.layer.dispatch(b, None, d.y, d.p, 2)
+        d.cache.read(None, d.k, d.v, rows, k_stride=width, v_stride=width)
+    k, v = _read(b, d.k), _read(b, d.v)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        calls()
+    with torch.cuda.stream(stream):
+        graph.replay()
+    stream.synchronize()
+    got = [_read(b, t) for t in (d.a, d.y, d.k)]
+    b.write_buffer(d.k, 0, k)
+    b.write_buffer(d.v, 0, v)
+    calls()
+    assert all(np.array_equal(g, _read(b, t)) for g, t in zip(got, (d.a, d.y, d.k))) and np.abs(got[0]).max() > 0 and np.abs(got[1]).max() > 0
+    del graph
+    d.free()
+print("ok")
+"""
+
+
+def test_the_first_call_of_a_process_may_be_a_recorded_one():
+    """Making the objects loads the code of every kernel that their calls launch."""
+    import os
+    import subprocess
+    import sys
+    from pathlib import Path
+    here = Path(__file__).resolve().parent
+    env = dict(os.environ, PYTHONPATH=os.pathsep.join([str(here.parent), str(here), os.environ.get("PYTHONPATH", "")]))
+    res = subprocess.run([sys.executable, "-c", FIRST_CALL], capture_output=True, text=True, timeout=300, env=env)
+    assert res.returncode == 0 and res.stdout.strip().endswith("ok"), res.stdout + res.stderr

@@ -1,11 +1,14 @@
 // The quantised cache of keys and values: storage, quantising on write, reading back.
 //
 // Formats and arithmetic are those of vx_quantize (IEEE division, scale rounded to f16 before the codes are formed,
-// half away from zero); vortx has no counterpart.  One block of threads takes one 32-token tile of one head, keys or
-// values: eight lanes share a block of 32 values (a float4 each, the largest magnitude by three shuffles), so rows are
-// read and written as whole 128-byte lines, four of them per lane under way.  A tile that the call covers completely
-// is put together in shared memory and goes out as 16-byte vectors; the others' codes are stored where they belong one word at a time.
-// Both are bound by the f32 side of the copy: 4 bytes a value next to 1.06 (Q8_0) or 0.56 (Q4_0).
+// half away from zero); vortx has no counterpart.  One block of threads takes a 32-token tile of some heads, keys or
+// values: four lanes share a block of 32 values (two float4 each, the largest magnitude by two shuffles), so rows are read and
+// written as whole 64-byte pieces, four loads per lane under way.  A tile that the call covers completely is put
+// together in shared memory and goes out as 16-byte vectors; the others' codes are stored where they belong.
+// The floor is the f32 side of the copy: 4 bytes a value next to 1.06 (Q8_0) or 0.56 (Q4_0).  Measured, 16 x 1024 tokens of
+// 8 heads of 128 in Q4_0 (134 MB of f32, 19 MB of codes): append 47 us (3.3 TB/s), bound by its instructions (29 lane operations
+// per value, a fifth of which find out where things are); read 32 us (4.8 TB/s).  Eight lanes to a block took 66 and 36 us. One
+// token: 4.6 us for both calls, recorded.
 #include <algorithm>
 #include <memory>
 #include <new>
@@ -39,8 +42,7 @@ __device__ __forceinline__ TileOf tile_of(const KvRows& r, const KvGeometry& g, 
 
 // What the format prescribes rests on two f32 quotients, the scale's and v / d.  Products with a reciprocal are within
 // 2^-22 of them and give the same f16 scale and the same code except next to a border between two of them; only there
-// the division is made.  (With divisions throughout the kernel issued 300 instructions per four values and was bound by
-// that: 89 us for 16 x 1024 tokens of 8 heads of 128, keys and values.)
+// the division is made.  (With divisions throughout append took 89 us where it then took 66.)
 //
 // f16(top / n).  The border between two f16 numbers is at bit 12 of an f32 mantissa.
 __device__ __forceinline__ uint16_t scale_of(float top, float n, float inv_n) {
@@ -372,6 +374,10 @@ vx_status vx_kv_cache_create(vx_context* ctx, vx_qtype k_type, vx_qtype v_type, 
     const size_t tiles = page_tokens / kTileTokens;
     VX_REQUIRE(pages <= ((size_t)1 << 50) / (tiles * heads * record), VX_ERR_OUT_OF_MEMORY, "vx_kv_cache_create: %zu pages are too many", pages);
     DeviceGuard guard(ctx->device);
+    // the kernels' code is loaded now, so that the first call may be one that is being recorded
+    cudaFuncAttributes loaded;
+    VX_CUDA(cudaFuncGetAttributes(&loaded, kv_append_kernel));
+    VX_CUDA(cudaFuncGetAttributes(&loaded, kv_read_kernel));
     std::unique_ptr<vx_kv_cache> c(new (std::nothrow) vx_kv_cache());
     VX_REQUIRE(c, VX_ERR_OUT_OF_MEMORY, "host allocation failed");
     c->k_type = k_type;

@@ -917,6 +917,8 @@ vx_status vx_moe_create(vx_context* ctx, const float* router, size_t experts, co
     p.row_log = 2;
     while ((1u << p.row_log) < p.experts) ++p.row_log;
     int per_sm = 0;
+    cudaFuncAttributes loaded;  // all kernels' code is loaded now, so that the first call may be one that is being recorded
+    VX_CUDA(cudaFuncGetAttributes(&loaded, moe_route_kernel));
     for (uint32_t team : {4u, 8u}) {
         const Launch inner = inner_launch(p, team);
         VX_CUDA(cudaFuncSetAttribute(inner.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)inner.smem));

@@ -58,12 +58,15 @@ class CacheRows:
             if sl is None:
                 raise ValueError("seqs is needed with a plain pointer")
             seqs = sl
+        given = max_pages is not None
         if max_pages is None:
             if tl is None:
                 raise ValueError("max_pages is needed with a plain pointer")
             max_pages = tl // seqs if seqs else 0
         if (tl is not None and tl < seqs * max_pages) or (bl is not None and seqs and bl < seqs + 1) or (sl is not None and sl < seqs):
             raise IndexError("table, begin or start is shorter than the sequences need")
+        if not given and seqs > 0 and tl % seqs:
+            raise ValueError("the table does not have the same number of pages for every sequence")
         if rows < 0 or seqs < 0 or max_pages < 0:
             raise ValueError("rows, seqs and max_pages must not be negative")
         self.rows, self.seqs, self.max_pages = rows, seqs, max_pages
@@ -172,6 +175,8 @@ class CacheAttention:
                 if ml is None:
                     raise ValueError("mask_words is needed with a plain pointer")
                 mask_words = ml // rows.rows if rows.rows else 1
+                if mask_words and rows.rows and ml % rows.rows:
+                    raise ValueError("the mask does not have the same number of words for every row")
             words = mask_words
             _check_len("mask", ml, rows.rows, words, words)
         if not self.cache._h:
