@@ -10,7 +10,7 @@ struct vx_kv_attention {
     const vx_context* ctx = nullptr;
     const vx_kv_cache* cache = nullptr;
     size_t heads = 0, max_seqs = 0;
-    uint32_t grid[3] = {};  // thread blocks by groups of eight rows (1, 2)
+    uint32_t grid[3] = {};  // thread blocks by groups of eight rows (1, 2), 0: four rows
     uint8_t* workspace = nullptr;
     size_t ml_offset = 0, counters_offset = 0;
 };
@@ -68,14 +68,14 @@ vx_status vx_kv_attention_create(vx_context* ctx, const vx_kv_cache* cache, size
     a->heads = heads;
     a->max_seqs = max_seqs;
     size_t rows = 0, blocks = 0;
-    for (uint32_t nt = 1; nt <= 2; ++nt) {
+    for (uint32_t nt = 0; nt <= 2; ++nt) {
         int per_sm = 0;
         uint32_t smem = 0;
         const vx_status st = setup(cache, nt, &per_sm, &smem);
         if (st != VX_OK) return st;
         VX_REQUIRE(per_sm > 0, VX_ERR_UNSUPPORTED, "vx_kv_attention_create: the kernel does not fit an SM");
         a->grid[nt] = (uint32_t)(ctx->sm_count * per_sm);
-        rows = std::max(rows, (size_t)2 * a->grid[nt] * 8 * nt);
+        rows = std::max(rows, (size_t)2 * a->grid[nt] * (nt == 0 ? 4 : 8 * nt));
         blocks = std::max(blocks, (size_t)a->grid[nt]);
     }
     a->ml_offset = rows * cache->head_dim * sizeof(float);
@@ -143,7 +143,7 @@ vx_status vx_kv_attention_run(vx_context* ctx, const vx_kv_attention* a, const v
     // two groups of 8 in one block share the conversion of the codes; 32 rows at a time spilled registers (35 against
     // 30 us for 4 x 8 drafted tokens of 32 heads over 4000).
     const uint64_t each = ((uint64_t)p.r.rows + p.r.seqs - 1) / p.r.seqs * group;
-    const uint32_t nt = each <= 8 ? 1 : 2;
+    const uint32_t nt = each <= 4 ? 0 : each <= 8 ? 1 : 2;
     DeviceGuard guard(ctx->device);
     const vx_status ls = launch(a->cache, nt, a->grid[nt], ctx->stream, p);
     if (ls != VX_OK) return ls;

@@ -46,8 +46,8 @@ struct AttnParams {
     float scale_log2;        // scale * log2 e
     const uint32_t* mask;
     uint32_t mask_words;
-    float* part_o;           // [2 * grid][8 NT][D]
-    float2* part_ml;         // [2 * grid][8 NT] maximum (base 2), sum
+    float* part_o;           // [2 * grid][rows of an item][D]
+    float2* part_ml;         // [2 * grid][rows of an item] maximum (base 2), sum
     uint32_t* counters;      // [grid] parts that are done, of what begins in this block; zero between calls
 };
 
@@ -324,11 +324,11 @@ __device__ __forceinline__ void join_parts(const AttnParams& p, const Segment& s
 template <bool K4, bool V4, int NB, int NT, int W>
 struct AttnLayout {  // of W warps
     static constexpr uint32_t k_bytes = kv_part_bytes(K4, NB), v_bytes = kv_part_bytes(V4, NB), record = k_bytes + v_bytes;
-    static constexpr uint32_t rows = 8 * NT, dim = 32 * NB;
+    static constexpr uint32_t rows = NT == 0 ? 4 : 8 * NT, dim = 32 * NB;
     static constexpr uint32_t ring = W * 2 * record;
     static constexpr uint32_t joined = W / 2 * rows * dim * 4;  // outputs of half the warps, after the loop
     static constexpr uint32_t tiles = ring > joined ? ring : joined;
-    static constexpr uint32_t q_bytes = NB * NT * 2 * 512;
+    static constexpr uint32_t q_bytes = NB * (NT == 0 ? 1 : 2 * NT) * 512;
     // the weights' transposition buffer lies over the keys' codes, which have been read by then, where it fits
     static constexpr uint32_t p_warp = rows * 32 * 4;
     static constexpr bool p_over = p_warp <= kv_code_bytes(K4, NB);
@@ -362,6 +362,9 @@ __global__ void __launch_bounds__(AttnShape<K4, V4, NB, NT>::warps * 32, AttnSha
 kv_attention_kernel(AttnParams p) {
     using Shape = AttnShape<K4, V4, NB, NT>;
     constexpr uint32_t R = Shape::rows, W = Shape::warps, kHalf = W / 2, kPerWarp = (R + W - 1) / W;
+    // Groups of eight columns, and rows of a group that a lane has results of: with four rows their two parts are the columns.
+    constexpr bool kParts = NT == 0;
+    constexpr int N = kParts ? 1 : NT, E = kParts ? 1 : 2;
     constexpr float kNone = -INFINITY;
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t* qf = smem + Shape::tiles;
@@ -373,6 +376,7 @@ kv_attention_kernel(AttnParams p) {
     pdl_wait();
     pdl_launch();
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    auto row_of = [&](int n, int e) { return kParts ? t : n * 8 + 2 * t + e; };
 
     Share at(p);
     if (!at.template find<R, W, kTileTokens>(p, shared64)) return;
@@ -387,7 +391,7 @@ kv_attention_kernel(AttnParams p) {
         uint32_t last_tile = tile1;
         if (p.mask == nullptr) last_tile = min(last_tile, (sq.start + (row_first + row_count - 1) / p.group) / kTileTokens + 1);
 
-        // ---- q's rows (2 NT a warp) and the first two tiles of every warp come in together -----------------------------
+        // ---- q's rows and the first two tiles of every warp come in together -----------------------------
         float qv[kPerWarp][NB];
 #pragma unroll
         for (uint32_t x = 0; x < kPerWarp; ++x) {
@@ -437,29 +441,27 @@ kv_attention_kernel(AttnParams p) {
             for (int b = 0; b < NB; ++b) {
                 const float v = qv[x][b] * up;
                 const __half h = __float2half_rn(v), l = __float2half_rn(v - __half2float(h));
-                uint8_t* dst = qf + ((b * NT + r / 8) * 2) * 512 + ((r % 8) * 4 + frag_lane(lane)) * 16 + frag_half(K4, lane) * 2;
+                uint8_t* dst = qf + frag_lane(lane) * 16 + frag_half(K4, lane) * 2 + (kParts ? b * 512 + r * 128 : ((b * N + r / 8) * 2) * 512 + (r % 8) * 64);
                 *reinterpret_cast<__half*>(dst) = h;
-                *reinterpret_cast<__half*>(dst + 512) = l;
+                *reinterpret_cast<__half*>(dst + (kParts ? 64 : 512)) = l;
             }
         }
         __syncthreads();
         const uint32_t qs = smem_addr(qf) + lane * 16;
-        float inv[NT][2];
+        float inv[N][E];
+        float top[N][E], sum[N][E], acc[2 * NB][N][2 * E], unit = 1.0f;  // acc counts 1 / (2 unit)
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            inv[n][0] = inv_lift[n * 8 + 2 * t];
-            inv[n][1] = inv_lift[n * 8 + 2 * t + 1];
-        }
-
-        float top[NT][2], sum[NT][2], acc[2 * NB][NT][4], unit = 1.0f;  // acc counts 1 / (2 unit)
+        for (int n = 0; n < N; ++n) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            top[n][0] = top[n][1] = kNone;
-            sum[n][0] = sum[n][1] = 0.0f;
+            for (int e = 0; e < E; ++e) {
+                inv[n][e] = inv_lift[row_of(n, e)];
+                top[n][e] = kNone;
+                sum[n][e] = 0.0f;
+            }
 #pragma unroll
             for (int d = 0; d < 2 * NB; ++d)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) acc[d][n][c] = 0.0f;
+                for (int c = 0; c < 2 * E; ++c) acc[d][n][c] = 0.0f;
         }
 
         for (uint32_t k = 0; k < mine; ++k) {
@@ -472,16 +474,16 @@ kv_attention_kernel(AttnParams p) {
                 const uint32_t pw = smem_addr(pwf);
                 // ---- which of the tile's tokens each of the thread's rows attends to, if not to all -------------------------
                 const bool masked = base + kTileTokens > sq.start;
-                uint32_t may[NT][2];
+                uint32_t may[N][E];
                 if (masked) {
                     const uint32_t before = base < sq.start ? (1u << (sq.start - base)) - 1u : 0u;  // context
                     const uint32_t there = sq.end - base >= 32 ? 0xffffffffu : (1u << (sq.end - base)) - 1u;
                     const uint32_t j0 = base < sq.start ? 0u : base - sq.start, up = base < sq.start ? sq.start - base : 0u;
 #pragma unroll
-                    for (int n = 0; n < NT; ++n)
+                    for (int n = 0; n < N; ++n)
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const uint32_t rr = row_first + n * 8 + 2 * t + e, i = rr / p.group;
+                        for (int e = 0; e < E; ++e) {
+                            const uint32_t rr = row_first + row_of(n, e), i = rr / p.group;
                             uint32_t bits = 0;  // of the call's tokens j0 ..
                             if (rr < sq.n * p.group) {
                                 if (p.mask == nullptr) {
@@ -496,14 +498,14 @@ kv_attention_kernel(AttnParams p) {
                             may[n][e] = (before | bits << up) & there;
                         }
                 }
-                // ---- scores of 32 tokens: s[m][n] = tokens 16 m + g (c 0, 1) and 16 m + g + 8 (c 2, 3), rows 8 n + 2 t, + 1
-                float s[2][NT][4];
+                // ---- scores of 32 tokens: s[m][n][E h + e] = token 16 m + 8 h + g, row row_of(n, e)
+                float s[2][N][2 * E];
 #pragma unroll
                 for (int m = 0; m < 2; ++m)
 #pragma unroll
-                    for (int n = 0; n < NT; ++n)
+                    for (int n = 0; n < N; ++n)
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) s[m][n][c] = 0.0f;
+                        for (int c = 0; c < 2 * E; ++c) s[m][n][c] = 0.0f;
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
                     uint32_t a[2][2][4];
@@ -523,55 +525,60 @@ kv_attention_kernel(AttnParams p) {
                     const uint2 ds = lds64(rec + kv_code_bytes(K4, NB) + b * 64 + g * 8);
                     const float2 d01 = __half22float2(bits_h2(ds.x)), d23 = __half22float2(bits_h2(ds.y));
                     // steps outside, tiles inside: neighbouring products do not wait for each other
-                    float c[2][NT][4];
-                    uint4 qh[NT], ql[NT];
+                    float c[2][N][4];
+                    uint4 qh[N], ql[N];
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        qh[n] = lds128(qs + ((b * NT + n) * 2) * 512);
-                        ql[n] = lds128(qs + ((b * NT + n) * 2 + 1) * 512);
+                    for (int n = 0; n < N; ++n) {
+                        qh[n] = lds128(qs + (kParts ? b : (b * N + n) * 2) * 512);
+                        if (!kParts) ql[n] = lds128(qs + ((b * N + n) * 2 + 1) * 512);
                     }
                     auto step = [&](auto use) {
 #pragma unroll
-                        for (int n = 0; n < NT; ++n)
+                        for (int n = 0; n < N; ++n)
 #pragma unroll
                             for (int m = 0; m < 2; ++m) use(n, m);
                     };
-                    step([&](int n, int m) { mma_f16_new(c[m][n], a[m][0], ql[n].x, ql[n].y); });
-                    step([&](int n, int m) { mma_f16(c[m][n], a[m][1], ql[n].z, ql[n].w); });
-                    step([&](int n, int m) { mma_f16(c[m][n], a[m][0], qh[n].x, qh[n].y); });
+                    if (kParts) {
+                        step([&](int n, int m) { mma_f16_new(c[m][n], a[m][0], qh[n].x, qh[n].y); });
+                    } else {
+                        step([&](int n, int m) { mma_f16_new(c[m][n], a[m][0], ql[n].x, ql[n].y); });
+                        step([&](int n, int m) { mma_f16(c[m][n], a[m][1], ql[n].z, ql[n].w); });
+                        step([&](int n, int m) { mma_f16(c[m][n], a[m][0], qh[n].x, qh[n].y); });
+                    }
                     step([&](int n, int m) { mma_f16(c[m][n], a[m][1], qh[n].z, qh[n].w); });
                     step([&](int n, int m) {
-                        const float d0 = m == 0 ? d01.x : d23.x, d1 = m == 0 ? d01.y : d23.y;
-                        s[m][n][0] = fmaf(d0, c[m][n][0], s[m][n][0]);
-                        s[m][n][1] = fmaf(d0, c[m][n][1], s[m][n][1]);
-                        s[m][n][2] = fmaf(d1, c[m][n][2], s[m][n][2]);
-                        s[m][n][3] = fmaf(d1, c[m][n][3], s[m][n][3]);
+                        const float d[2] = {m == 0 ? d01.x : d23.x, m == 0 ? d01.y : d23.y};
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+#pragma unroll
+                            for (int e = 0; e < E; ++e)
+                                s[m][n][E * h + e] = fmaf(d[h], kParts ? c[m][n][2 * h] + c[m][n][2 * h + 1] : c[m][n][2 * h + e], s[m][n][E * h + e]);
                     });
                 }
 #pragma unroll
                 for (int m = 0; m < 2; ++m)
 #pragma unroll
-                    for (int n = 0; n < NT; ++n)
+                    for (int n = 0; n < N; ++n)
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) s[m][n][c] *= inv[n][c & 1];
+                        for (int c = 0; c < 2 * E; ++c) s[m][n][c] *= inv[n][c % E];
                 if (masked) {
                     __syncwarp();  // keeps this a branch that other tiles jump over
 #pragma unroll
                     for (int m = 0; m < 2; ++m)
 #pragma unroll
-                        for (int n = 0; n < NT; ++n)
+                        for (int n = 0; n < N; ++n)
 #pragma unroll
-                            for (int c = 0; c < 4; ++c)
-                                if (!(may[n][c & 1] >> (m * 16 + (c >> 1) * 8 + g) & 1)) s[m][n][c] = kNone;
+                            for (int c = 0; c < 2 * E; ++c)
+                                if (!(may[n][c % E] >> (m * 16 + (c / E) * 8 + g) & 1)) s[m][n][c] = kNone;
                 }
                 __syncwarp();  // the keys' codes have been read
                 // ---- running maximum and sum; the weights change sides through shared memory -----------------------------
-                float fall[NT][2];
+                float fall[N][E];
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+                for (int n = 0; n < N; ++n)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float mx = fmaxf(fmaxf(s[0][n][e], s[0][n][e + 2]), fmaxf(s[1][n][e], s[1][n][e + 2]));
+                    for (int e = 0; e < E; ++e) {
+                        float mx = fmaxf(fmaxf(s[0][n][e], s[0][n][e + E]), fmaxf(s[1][n][e], s[1][n][e + E]));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
@@ -583,9 +590,9 @@ kv_attention_kernel(AttnParams p) {
                         for (int m = 0; m < 2; ++m)
 #pragma unroll
                             for (int h = 0; h < 2; ++h) {
-                                const float w = ex2(s[m][n][e + 2 * h] - ref);
+                                const float w = ex2(s[m][n][e + E * h] - ref);
                                 add += w;
-                                const uint32_t row = n * 8 + 2 * t + e, lo = g + 8 * h;  // token lo + 16 m
+                                const uint32_t row = row_of(n, e), lo = g + 8 * h;  // token lo + 16 m
                                 pwf[p_slot(row, (lo & 3) * 2 + m) * 4 + (lo >> 2)] = w;
                             }
                         sum[n][e] = fmaf(sum[n][e], fall[n][e], add);
@@ -606,7 +613,7 @@ kv_attention_kernel(AttnParams p) {
                     most[3] = __hmax2(most[3], __habs2(bits_h2(dv[b].w)));
                 }
                 __half2 back[4];  // 2^(1 - e)
-                float pe[NT][8], largest = 0.0f;
+                float pe[N][8], largest = 0.0f;
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
                     const uint32_t e = h2_bits(most[x]) & 0x7c007c00u;
@@ -616,10 +623,10 @@ kv_attention_kernel(AttnParams p) {
                     pe[0][2 * x + 1] = f.y;
                 }
 #pragma unroll
-                for (int n = NT - 1; n >= 0; --n)
+                for (int n = N - 1; n >= 0; --n)
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        const uint4 f = lds128(pw + p_slot(n * 8 + g, t * 2 + x) * 16);
+                        const uint4 f = lds128(pw + p_slot(kParts ? g / 2 : n * 8 + g, t * 2 + x) * 16);
                         const uint32_t w[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
@@ -633,16 +640,20 @@ kv_attention_kernel(AttnParams p) {
                     const float ratio = now * __uint_as_float(0x7f000000u - __float_as_uint(unit));  // powers of two
                     unit = now;
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        fall[n][0] *= ratio;
-                        fall[n][1] *= ratio;
-                    }
+                    for (int n = 0; n < N; ++n)
+#pragma unroll
+                        for (int e = 0; e < E; ++e) fall[n][e] *= ratio;
                 }
-                uint32_t ph[NT][4], pl[NT][4];  // pairs of tokens
+                uint32_t ph[N][4], pl[N][4];  // pairs of tokens
+                uint32_t minus[N][4];         // what hi is to be taken off for the lane's column: of the parts of four rows, the first has hi itself
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+                for (int n = 0; n < N; ++n)
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) split_f16(pe[n][2 * x] * unit, pe[n][2 * x + 1] * unit, &ph[n][x], &pl[n][x]);
+                    for (int x = 0; x < 4; ++x) {
+                        split_f16(pe[n][2 * x] * unit, pe[n][2 * x + 1] * unit, &ph[n][x], &pl[n][x]);
+                        minus[n][x] = kParts && !(g & 1) ? 0u : ph[n][x];
+                        if (kParts && !(g & 1)) pl[n][x] = 0u;
+                    }
                 // ---- output ------------------------------------------------------------------------------------------
                 auto output = [&](auto some_masked) {
 #pragma unroll
@@ -677,12 +688,12 @@ kv_attention_kernel(AttnParams p) {
                                 a[x][1][3] = f16_of_bytes(w4.w, 0x4342);
                             }
                         }
-                        uint32_t hi_[NT][4], lo_[NT][4];
+                        uint32_t hi_[N][4], lo_[N][4];  // with four rows, the lane's part is in lo_
 #pragma unroll
-                        for (int n = 0; n < NT; ++n)
+                        for (int n = 0; n < N; ++n)
 #pragma unroll
                             for (int x = 0; x < 4; ++x) {
-                                const __half2 h = __hmul2(bits_h2(ph[n][x]), d[x]);
+                                const __half2 h = __hmul2(bits_h2(minus[n][x]), d[x]);
                                 const __half2 l = __hfma2(bits_h2(pl[n][x]), d[x], __hfma2(bits_h2(ph[n][x]), d[x], __hneg2(h)));
                                 hi_[n][x] = h2_bits(h);
                                 lo_[n][x] = h2_bits(l);
@@ -694,20 +705,23 @@ kv_attention_kernel(AttnParams p) {
                             }
                         // The tensor cores cut their f32 sums off instead of rounding them: a tile's sum is taken from
                         // zero and added to the output here, or the loss would grow with the number of tiles.
-                        float o[NT][2][4];
+                        float o[N][2][4];
                         auto step = [&](auto use) {
 #pragma unroll
-                            for (int n = 0; n < NT; ++n)
+                            for (int n = 0; n < N; ++n)
 #pragma unroll
                                 for (int m = 0; m < 2; ++m) use(n, m);
                         };
                         step([&](int n, int m) { mma_f16_new(o[n][m], a[0][m], lo_[n][0], lo_[n][1]); });
                         step([&](int n, int m) { mma_f16(o[n][m], a[1][m], lo_[n][2], lo_[n][3]); });
-                        step([&](int n, int m) { mma_f16(o[n][m], a[0][m], hi_[n][0], hi_[n][1]); });
-                        step([&](int n, int m) { mma_f16(o[n][m], a[1][m], hi_[n][2], hi_[n][3]); });
+                        if (!kParts) {
+                            step([&](int n, int m) { mma_f16(o[n][m], a[0][m], hi_[n][0], hi_[n][1]); });
+                            step([&](int n, int m) { mma_f16(o[n][m], a[1][m], hi_[n][2], hi_[n][3]); });
+                        }
                         step([&](int n, int m) {
 #pragma unroll
-                            for (int c = 0; c < 4; ++c) acc[2 * b + m][n][c] = fmaf(acc[2 * b + m][n][c], fall[n][c & 1], o[n][m][c]);
+                            for (int c = 0; c < 2 * E; ++c)
+                                acc[2 * b + m][n][c] = fmaf(acc[2 * b + m][n][c], fall[n][c % E], kParts ? o[n][m][2 * c] + o[n][m][2 * c + 1] : o[n][m][c]);
                         });
                     }
                 };
@@ -727,44 +741,43 @@ kv_attention_kernel(AttnParams p) {
         // ---- the warps' parts become one -------------------------------------------------------------------------
         const float down = 0.5f / unit;
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < N; ++n)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
+            for (int e = 0; e < E; ++e) {
                 float l = sum[n][e];
                 l += __shfl_xor_sync(0xffffffffu, l, 4);
                 l += __shfl_xor_sync(0xffffffffu, l, 8);
                 l += __shfl_xor_sync(0xffffffffu, l, 16);
-                if (g == 0) ml[warp * R + n * 8 + 2 * t + e] = make_float2(top[n][e], l);
+                if (g == 0) ml[warp * R + row_of(n, e)] = make_float2(top[n][e], l);
             }
         __syncthreads();
         float* joined = reinterpret_cast<float*>(smem);
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < N; ++n)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const uint32_t row = n * 8 + 2 * t + e;
+            for (int e = 0; e < E; ++e) {
                 float m = kNone;
 #pragma unroll
-                for (uint32_t w = 0; w < W; ++w) m = fmaxf(m, ml[w * R + row].x);
+                for (uint32_t w = 0; w < W; ++w) m = fmaxf(m, ml[w * R + row_of(n, e)].x);
                 const float f = top[n][e] == kNone ? 0.0f : ex2(top[n][e] - m) * down;
 #pragma unroll
                 for (int d = 0; d < 2 * NB; ++d) {
                     acc[d][n][e] *= f;
-                    acc[d][n][e + 2] *= f;
+                    acc[d][n][e + E] *= f;
                 }
             }
         auto each = [&](auto use) {  // lane's four neighbouring values of every (row, block)
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+            for (int n = 0; n < N; ++n)
 #pragma unroll
-                for (int e = 0; e < 2; ++e)
+                for (int e = 0; e < E; ++e)
 #pragma unroll
-                    for (int b = 0; b < NB; ++b) use(n, e, b, (n * 8 + 2 * t + e) * Shape::dim + b * 32 + g * 4);
+                    for (int b = 0; b < NB; ++b) use(n, e, b, row_of(n, e) * Shape::dim + b * 32 + g * 4);
         };
         auto store = [&](uint32_t half) {
             each([&](int n, int e, int b, uint32_t at) {
                 *reinterpret_cast<float4*>(joined + half * R * Shape::dim + at) =
-                    make_float4(acc[2 * b][n][e], acc[2 * b][n][e + 2], acc[2 * b + 1][n][e], acc[2 * b + 1][n][e + 2]);
+                    make_float4(acc[2 * b][n][e], acc[2 * b][n][e + E], acc[2 * b + 1][n][e], acc[2 * b + 1][n][e + E]);
             });
         };
         if (warp >= kHalf) store(warp - kHalf);
@@ -773,9 +786,9 @@ kv_attention_kernel(AttnParams p) {
             each([&](int n, int e, int b, uint32_t at) {
                 const float4 f = *reinterpret_cast<const float4*>(joined + warp * R * Shape::dim + at);
                 acc[2 * b][n][e] += f.x;
-                acc[2 * b][n][e + 2] += f.y;
+                acc[2 * b][n][e + E] += f.y;
                 acc[2 * b + 1][n][e] += f.z;
-                acc[2 * b + 1][n][e + 2] += f.w;
+                acc[2 * b + 1][n][e + E] += f.w;
             });
             store(warp);
         }
@@ -825,12 +838,16 @@ bool attn_pick(uint32_t nb, uint32_t nt, F f) {
     using std::integral_constant;
 #define VX_ATTN_CASE(B, N) \
     if (nb == B && nt == N) return go(integral_constant<int, B>{}, integral_constant<int, N>{});
+    VX_ATTN_CASE(2, 0)
     VX_ATTN_CASE(2, 1)
     VX_ATTN_CASE(2, 2)
+    VX_ATTN_CASE(3, 0)
     VX_ATTN_CASE(3, 1)
     VX_ATTN_CASE(3, 2)
+    VX_ATTN_CASE(4, 0)
     VX_ATTN_CASE(4, 1)
     VX_ATTN_CASE(4, 2)
+    VX_ATTN_CASE(8, 0)
     VX_ATTN_CASE(8, 1)
     VX_ATTN_CASE(8, 2)
 #undef VX_ATTN_CASE
