@@ -159,6 +159,28 @@ def test_what_lies_in_masked_places_does_not_matter(backend, vt):
         s.check(got, may)
 
 
+@pytest.mark.parametrize("kt", [vb.Q8_0, vb.Q4_0])
+@pytest.mark.parametrize("vt", [vb.Q8_0, vb.Q4_0])
+@pytest.mark.parametrize("dim", [64, 96, 128, 256])
+@pytest.mark.parametrize("group", [1, 2])
+def test_small_trees_and_what_they_leave_out(backend, kt, vt, dim, group):
+    """Up to four, or eight, rows of a head of keys on average (the products' columns are laid out differently), more in one
+    sequence; NaN in a token that the mask leaves out."""
+    rng = _rng(dim + group)
+    seqs = [(37, 3), (0, 2), (64, 6), (1130, 1), (31, 3)]
+    s = Scene(backend, seqs, 2 * group, 2, dim, 32, kt, vt, seed=dim, pad=1)
+    may, mask = _trees(rng, seqs)
+    mask = np.concatenate([mask, np.zeros((1, 1), np.uint32)])
+    for i in range(6):                                 # token 2 of the third sequence is for nobody
+        may[2][i, 2] = False
+        mask[5 + i, 0] &= ~np.uint32(4)
+    clean = s.run(mask)
+    s.check(clean, may)
+    x = s._b(np.full(2 * dim, np.nan, np.float32))
+    s.cache.append(None, x, x, vb.CacheRows(s._b(s.table[2:3]), s._b(np.array([0, 1], np.int32)), s._b(np.array([66], np.int32)), 1))
+    assert np.array_equal(s.run(mask), clean)
+
+
 def test_nan_in_the_context_and_in_q_reaches_its_own_rows_only(backend):
     s = Scene(backend, [(40, 2), (70, 2)], 4, 2, 64, seed=6)
     clean = s.run()

@@ -3,7 +3,7 @@
 //
 // S^T = K Q^T and O^T = V^T P^T: the codes are the A operand (16 tokens or 16 values of the head high), the query rows are the
 // 8-wide N dimension, so the few rows of a decode step (query heads that share a head of keys, times drafted tokens)
-// fill the tensor cores' tiles.  A thread block has a head of a sequence, up to 8 NT query rows and a run of 32-token
+// fill the tensor cores' tiles.  A thread block has a head of a sequence, 4 (NT 0), 8 or 16 query rows and a run of 32-token
 // tiles; its four or six warps take the tiles in turn, each with its own running maximum, sum and output (one pass over the
 // cache, no synchronisation between tiles), two tiles in flight per warp (cp.async, a record is contiguous).
 //   scores   per block of 32 values: sum of code * (q hi + q lo) on the tensor cores, times the block's scale, in f32
@@ -16,11 +16,11 @@
 // The runs are shares of all tiles of all (sequence, head, group of rows), see Share.  A share that covers the tiles of a
 // (sequence, head, rows) only in part leaves maximum, sum and unnormalised output in the workspace, at most two per block,
 // and the last block to finish a part joins them all, in their order.
-// Measured, 32 heads over 8 of 128 in Q8_0: a token each of 16 sequences of up to 16384 tokens 88 us (392 MB at 4.4 TB/s, 0.67 of
-// the copy rate; some 25 us are the launch, the first tiles' latency and the join); 4 x 8 drafted tokens over 4000 30 us, 2 x 48
-// over 12000 157 us; one token of 16 heads of 64 over 60001 in Q4_0 40 us.  With many rows the tensor products take a
-// fifth of the time: the chain scores -> maximum -> weights -> output binds, at 12 warps per SM (0.5 instructions
-// a cycle and scheduler).
+// Measured (recorded), 32 heads over 8 of 128 in Q8_0: a token each of 16 sequences of up to 16384 tokens 73 us (392 MB at 5.4 TB/s,
+// 0.82 of the copy rate), of one of 500 9.3 us; 4 x 8 drafted tokens over 4000 30 us, 2 x 48 over 12000 156 us; one token
+// of 16 heads of 64 over 60001 in Q4_0 34 us (589 instructions a tile of 32 tokens).  With many rows the products take 0.4
+// of what the tensor cores could do: the chain scores -> maximum -> weights -> output binds, at 12 warps per SM (0.5
+// instructions a cycle and scheduler; 16 warps of 128 registers are no faster).
 #pragma once
 
 #include <type_traits>
