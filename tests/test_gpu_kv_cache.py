@@ -153,6 +153,50 @@ def test_what_is_not_finite_reads_back_as_nan(backend, qt):
         assert np.isnan(got[bad]).all() and np.isfinite(got[~bad]).all()
 
 
+@pytest.mark.parametrize("qt", [vb.Q8_0, vb.Q4_0])
+def test_ties_borders_signs_and_small_scales(backend, qt):
+    """Values of equal magnitude and different signs, values half way between two codes, scales next to a border of f16, f16's
+    small numbers and zeros of both signs: still the host quantiser's codes."""
+    rng = _rng(30)
+    heads, dim, n = 2, 128, 96
+    step, top = (127.0, 127) if qt == vb.Q8_0 else (7.0, 7)
+    x = np.zeros((n, heads * dim // 32, 32), np.float32)
+    for t in range(n):
+        for b in range(x.shape[1]):
+            kind = (t * x.shape[1] + b) % 8
+            v = rng.integers(-top, top + 1, 32).astype(np.float32)
+            if kind == 1:                              # half way: the scale is 1 / 8, exact
+                v = (rng.integers(-top, top, 32) + 0.5).astype(np.float32) / 8
+                v[5] = -top / 8 if t % 2 else top / 8
+            elif kind == 2:                            # next to half way
+                v = np.nextafter((rng.integers(-top, top, 32) + 0.5).astype(np.float32), rng.choice([-np.inf, np.inf], 32).astype(np.float32)) / 16
+                v[3] = top / 16
+            elif kind == 3:                            # the scale half way between two f16 numbers, or next to it
+                s = np.float32((1024 + int(rng.integers(0, 1024)) + 0.5) / 1024)
+                v = rng.standard_normal(32).astype(np.float32)
+                v[7] = np.nextafter(np.float32(s * step), np.float32(rng.choice([0.0, s * step, np.inf])))
+            elif kind == 4:
+                v = (rng.standard_normal(32) * 10.0 ** rng.uniform(-9, -3)).astype(np.float32)
+            elif kind == 5:
+                v = np.where(rng.random(32) < 0.5, np.float32(-0.0), np.float32(0.0)).astype(np.float32)
+            elif kind == 6:
+                v = (rng.standard_normal(32) * 1e-30).astype(np.float32)
+            elif kind == 7:                            # one magnitude, both signs
+                v = np.where(rng.random(32) < 0.5, -1.0, 1.0).astype(np.float32) * np.float32(rng.uniform(0.1, 10))
+            x[t, b] = v
+    flat = x.reshape(n, heads * dim)
+    cache = vb.QuantizedCache(backend, qt, qt, heads, dim, 3, 32)
+    xb = backend.init_buffer(flat.ravel())
+    rows = _rows(backend, [[2, 0, 1]], [0, n], [0], n)
+    cache.append(None, xb, xb, rows)
+    k, v = backend.uninit_buffer(flat.size), backend.uninit_buffer(flat.size)
+    cache.read(None, k, v, rows)
+    want = vb.dequantize_host(qt, vb.quantize(qt, flat), n, heads * dim).astype(np.float32).reshape(-1, 32)
+    for got in (_read(backend, k).reshape(-1, 32), _read(backend, v).reshape(-1, 32)):
+        bad = [i for i in range(len(want)) if not np.array_equal(got[i], want[i])]
+        assert not bad, (len(bad), bad[0] % 8, got[bad[0]], want[bad[0]])
+
+
 def test_many_sequences_and_empty_calls(backend):
     """More sequences than one step of the search sees, most of them without rows."""
     rng = _rng(11)

@@ -81,6 +81,13 @@ def test_units_that_four_warps_share(backend, gt, experts, hidden, inner, top_k,
     assert all(np.array_equal(a, b) for a, b in zip(first, l.run(x)))
 
 
+@pytest.mark.parametrize("hidden,tokens", [(2624, 3), (4128, 5), (9504, 2), (32, 4)])
+def test_output_tiles_share_out_the_columns(backend, hidden, tokens):
+    """Three, two, one and four blocks add up an output tile's columns."""
+    l = Layer(backend, 2, hidden, 192, 2, False, vb.Q8_0, vb.Q4_0, max_tokens=tokens, seed=hidden)
+    l.check(_rng(tokens).standard_normal((tokens, hidden)).astype(np.float32))
+
+
 def test_calls_follow_each_other_and_repeat_bit_for_bit(backend):
     """Different token counts through one layer; the same call again gives the same bits."""
     l = Layer(backend, 16, 512, 256, 4, max_tokens=32, seed=2)
