@@ -142,7 +142,7 @@ vx_status vx_kv_attention_run(vx_context* ctx, const vx_kv_attention* a, const v
     // Rows of a sequence that share a head of keys, as the host can know them (the average), in groups of 4, 8 or 16.  Four
     // rows' two parts fill the eight columns of a product (9.3 us with, 10.7 without for one token of 4 heads to a head of
     // keys over 500; 73 and 80 us for 16 sequences of up to 16384).  Two groups of 8 in one block share the conversion of the
-    // codes (30 us for 4 x 8 drafted tokens of 32 heads over 4000, 156 for 2 x 48 over 12000; one group at a time 34 and
+    // codes (30 us for 4 x 8 drafted tokens of 32 heads over 4000, 149 for 2 x 48 over 12000; one group at a time 34 and
     // 183); 32 rows spilled registers (35).
     const uint64_t each = ((uint64_t)p.r.rows + p.r.seqs - 1) / p.r.seqs * group;
     const uint32_t nt = each <= 4 ? 0 : each <= 8 ? 1 : 2;

@@ -17,10 +17,10 @@
 // (sequence, head, rows) only in part leaves maximum, sum and unnormalised output in the workspace, at most two per block,
 // and the last block to finish a part joins them all, in their order.
 // Measured (recorded), 32 heads over 8 of 128 in Q8_0: a token each of 16 sequences of up to 16384 tokens 73 us (392 MB at 5.4 TB/s,
-// 0.82 of the copy rate), of one of 500 9.3 us; 4 x 8 drafted tokens over 4000 30 us, 2 x 48 over 12000 156 us; one token
-// of 16 heads of 64 over 60001 in Q4_0 34 us (589 instructions a tile of 32 tokens).  With many rows the products take 0.4
-// of what the tensor cores could do: the chain scores -> maximum -> weights -> output binds, at 12 warps per SM (0.5
-// instructions a cycle and scheduler; 16 warps of 128 registers are no faster).
+// 0.82 of the copy rate), of one of 500 9.3 us; 4 x 8 drafted tokens over 4000 30 us, 2 x 48 over 12000 149 us; one token
+// of 16 heads of 64 over 60001 in Q4_0 34 us (589 instructions a tile of 32 tokens; 16 warps of 128 registers are no faster).
+// With many rows the products take 0.4 of what the tensor cores could do: the chain scores -> maximum -> weights ->
+// output binds (0.5 instructions a cycle and scheduler with 8 warps of 255 registers as with 12 of 168).
 #pragma once
 
 #include <type_traits>
@@ -336,11 +336,14 @@ struct AttnLayout {  // of W warps
     static constexpr uint32_t smem = tiles + q_bytes + p_bytes + rows * 4 + W * rows * 8 + 128;
 };
 
-// Twelve warps per SM, as 168 registers allow: three blocks of four where their shared memory fits, else two of six
-// (154 us instead of the 160 of two blocks of four for 48 drafted tokens of 32 heads over 12000); six or four in one block for the largest heads.
+// Twelve warps per SM, as 168 registers allow: three blocks of four where their shared memory fits, else two of six (154 us
+// instead of the 160 of two blocks of four for 48 drafted tokens of 32 heads over 12000, with eight rows to a block).  Sixteen rows
+// need more registers than that: two blocks of four, 255 registers (156 us with six and 168 for those tokens, 149 so; 16
+// tokens over 500: 15.7 and 14.7; heads of 64 over 12000: 95.5 and 98).  The largest heads have one block.
 constexpr bool attn_fits(uint32_t smem, uint32_t blocks) { return blocks * (smem + 1024) <= 228 * 1024; }
 template <bool K4, bool V4, int NB, int NT>
 constexpr int attn_warps() {
+    if (NT == 2 && NB <= 4) return 4;
     if (attn_fits(AttnLayout<K4, V4, NB, NT, 4>::smem, 3)) return 4;
     if (attn_fits(AttnLayout<K4, V4, NB, NT, 6>::smem, 2)) return 6;
     if (attn_fits(AttnLayout<K4, V4, NB, NT, 4>::smem, 2)) return 4;
@@ -349,8 +352,7 @@ constexpr int attn_warps() {
 template <bool K4, bool V4, int NB, int NT>
 struct AttnShape : AttnLayout<K4, V4, NB, NT, attn_warps<K4, V4, NB, NT>()> {
     static constexpr int warps = attn_warps<K4, V4, NB, NT>();
-    // blocks of an SM, for the registers: 168 a thread where heads of up to 128 values take twelve warps
-    static constexpr int blocks = NB > 4 ? 1 : warps == 4 ? 3 : 2;
+    static constexpr int blocks = NB > 4 ? 1 : warps == 4 && NT < 2 ? 3 : 2;  // of an SM, for the registers
 };
 
 // 16-byte slot of the weights' transposition buffer: rows of eight slots, spread so that the writes (one float per
