@@ -18,10 +18,10 @@
 // middle codes): 5e-7 relative to the exact result, 2e-7 with converted codes.  Nibbles left at bits 0..3 lose six more
 // bits: 6e-6.
 // Measured (recorded calls): 8 tokens, 2 of 8 experts of 14336 x 4096, Q4_0 gate and up, Q8_0 down: inner 122 us (3.8 TB/s),
-// down 77 us (5.7 TB/s); 32 tokens, 4 of 32 experts of 1408 x 2048, Q4_0: inner 47 us, down 35 us; one token of 4 such
-// experts: 20 us, of which 5 are the router's.  Reading the weights takes 0.58 of the memory's rate in the inner kernel, which is bound by
-// its instructions (78 per 32 x 32 weights, 28 of them to take the codes apart, at 0.53 a cycle and scheduler: 128
-// registers leave four warps to hide latencies), 0.87 in the down kernel.
+// down 77 us (5.7 TB/s); 32 tokens, 4 of 32 experts of 1408 x 2048, Q4_0: inner 47 us, down 35 us; one token, 8 of 64
+// experts of 1024 x 2048: 20 us, of which the router's launch takes 4.  The inner kernel reads at 0.58 of the copy rate, bound by its
+// instructions (73 per 32 x 32 weights, 28 of them to take the codes apart, at 0.51 a cycle and scheduler: 128
+// registers leave four warps to hide latencies), the down kernel at 0.87.
 #include <algorithm>
 #include <cstddef>
 #include <memory>
