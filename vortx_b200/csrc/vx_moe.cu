@@ -1,5 +1,5 @@
 // A mixture-of-experts layer for a few tokens on block-quantised weights, in three launches:
-//   route   logits = router x, in slices of the columns, and x split into two f16 parts per block of 32
+//   route   logits = router x, in slices of the columns, and x split into two f16 parts, lifted together per chunk of a gate row
 //   inner   silu(gate x) * (up x): four or eight warps per (expert with tokens, 32 inner rows)
 //   down    y = sum weight * (down h): a thread block per (32 output rows, share of all experts' columns)
 // Every block of the last two picks the experts from the logits itself (2.5 us; less than one block doing it for all would
@@ -10,18 +10,14 @@
 // cp.async copies that run ahead over the ends of units and experts; no synchronisation between warps until the
 // sums are added up).  On the tensor cores (m16n8k16) 16 rows of codes are A; B's columns are the two parts of four
 // tokens, or eight tokens, whose parts are then multiplied one after the other into the same sums.
-// A code u (code + 8 or + 128, not negative) is used as the f16 number whose bits it is, u 2^-20 (nibbles moved to bits
-// 4..7) or u 2^-24: a shift and a logic operation, or a byte permutation, per pair and no conversion.  The offset's
-// part of a block's sum, 8 or 128 times the sum of the vector's parts, is taken off with the multiplication that scales
-// the sum.  That makes the partial sums two to three times as large as those of the signed codes, and the tensor cores
-// align products by the exponent field, so the leading zeros of such a number are lost bits (two of 24 for the
-// middle codes): 5e-7 relative to the exact result, 2e-7 with converted codes.  Nibbles left at bits 0..3 lose six more
-// bits: 6e-6.
-// Measured (recorded calls): 8 tokens, 2 of 8 experts of 14336 x 4096, Q4_0 gate and up, Q8_0 down: inner 122 us (3.8 TB/s),
-// down 77 us (5.7 TB/s); 32 tokens, 4 of 32 experts of 1408 x 2048, Q4_0: inner 47 us, down 35 us; one token, 8 of 64
-// experts of 1024 x 2048: 20 us, of which the router's launch takes 4.  The inner kernel reads at 0.58 of the copy rate, bound by its
-// instructions (73 per 32 x 32 weights, 28 of them to take the codes apart, at 0.51 a cycle and scheduler: 128
-// registers leave four warps to hide latencies), the down kernel at 0.87.
+// A code becomes its f16 number before it is multiplied (one logic operation or byte permutation and one f16 operation per
+// pair).  Taking the bits of code + 8 or + 128 as a subnormal f16 number, and 8 or 128 times the vector's sum off afterwards,
+// would save the f16 operation (2 to 7 % of the time below), but its error goes with 128 times the block's largest value, not
+// with the row's own products: 1.5e-5 of sum |w||x| beside values 1000 times the others, and 5e-7 of the largest output
+// on even inputs, where this form has 3e-7.
+// Measured (recorded calls): 8 tokens, 2 of 8 experts of 14336 x 4096, Q4_0 gate and up, Q8_0 down: 209 us; 32 tokens, 4 of 32
+// experts of 1408 x 2048, Q4_0: 83 us; 7 tokens, 3 of 16 experts of 608 x 1120, Q8_0: 18.6 us; one token, 8 of 64 experts of
+// 1024 x 2048, Q4_0: 20.5 us, of which the router's launch takes 4.
 #include <algorithm>
 #include <cstddef>
 #include <memory>
@@ -56,9 +52,9 @@ struct MoeParams {
     Matrix gate, up, down;
     float* logits;       // [slices][tokens][experts]
     uint8_t* xh;         // [tokens][2 parts][hidden / 32][64 bytes], B-operand order
-    float2* xs;          // [tokens][hidden / 32]: what a block's sum is multiplied with, and what is added then
+    float* xs;           // [tokens][chunks of a gate row]: what a chunk's sum is multiplied with
     uint8_t* hh;         // the inner vectors, per slot = token * top_k + place
-    float2* hs;
+    float* hs;           // [slots][inner / 32]: the same for a block's sum
     int32_t* ids_out;
     float* weights_out;
 };
@@ -101,18 +97,17 @@ __device__ __forceinline__ void logits_of(const MoeParams& p, uint32_t expert, u
     }
 }
 
-// One block of 32 values (a lane each) as two parts in B-operand order, and what its sums are to be multiplied with and
-// corrected by.  f16 ends just below 2^16: values from 2^105 on count as infinite.
-__device__ __forceinline__ void split_block(float v, uint32_t lane, bool four, uint8_t* hi, uint8_t* lo, float2* factor) {
-    const float up = fmaxf(lift(warp_max(fabsf(v))), __uint_as_float((127u - 89u) << 23));
+// The power of two that values, `most` the largest magnitude, are split with.  f16 ends just below 2^16: values from 2^105 on
+// count as infinite.
+__device__ __forceinline__ float split_lift(float most) { return fmaxf(lift(most), __uint_as_float((127u - 89u) << 23)); }
+__device__ __forceinline__ float split_factor(float up) { return __uint_as_float(0x7f000000u - __float_as_uint(up)); }  // 1 / up
+// One block of 32 values (a lane each) as two parts in B-operand order.
+__device__ __forceinline__ void split_block(float v, float up, uint32_t lane, bool four, uint8_t* hi, uint8_t* lo) {
     const float x = v * up;
     const __half h = __float2half_rn(x), l = __float2half_rn(x - __half2float(h));
     const uint32_t at = frag_lane(lane) * 16 + frag_half(four, lane) * 2;
     *reinterpret_cast<__half*>(hi + at) = h;
     *reinterpret_cast<__half*>(lo + at) = l;
-    const float sum = warp_add(__half2float(h) + __half2float(l));
-    const float down = __uint_as_float(0x7f000000u - __float_as_uint(up));  // 1 / up, a power of two
-    if (lane == 0) *factor = make_float2((four ? 1048576.0f : 16777216.0f) * down, (four ? -8.0f : -128.0f) * sum * down);
 }
 
 __global__ void __launch_bounds__(kMoeThreads) moe_route_kernel(MoeParams p) {
@@ -129,11 +124,21 @@ __global__ void __launch_bounds__(kMoeThreads) moe_route_kernel(MoeParams p) {
             float v[4];
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i) v[i] = b0 + i < nb ? p.x[(size_t)t * p.x_stride + (b0 + i) * 32 + lane] : 0.0f;
+            // a chunk of gate and up (four blocks in Q4_0, two in Q8_0) has one power of two
+            const uint32_t each = p.gate4 ? 4 : 2, chunks = (nb + each - 1) / each;
+            float m0 = fmaxf(fabsf(v[0]), fabsf(v[1])), m1 = fmaxf(fabsf(v[2]), fabsf(v[3]));
+            if (p.gate4) m0 = m1 = fmaxf(m0, m1);
+            const float up0 = split_lift(warp_max(m0)), up1 = split_lift(warp_max(m1));
+            if (lane == 0) {
+                float* factor = p.xs + (size_t)t * chunks + b0 / each;
+                factor[0] = split_factor(up0);
+                if (!p.gate4 && b0 + 2 < nb) factor[1] = split_factor(up1);
+            }
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i)
                 if (b0 + i < nb) {
                     uint8_t* hi = p.xh + ((size_t)t * 2 * nb + b0 + i) * 64;
-                    split_block(v[i], lane, p.gate4 != 0, hi, hi + (size_t)nb * 64, p.xs + (size_t)t * nb + b0 + i);
+                    split_block(v[i], i < 2 ? up0 : up1, lane, p.gate4 != 0, hi, hi + (size_t)nb * 64);
                 }
         }
     }
@@ -364,93 +369,88 @@ __device__ __forceinline__ uint32_t token_of(uint32_t n, uint32_t t) { return NT
 template <int NT>
 struct Vectors {
     const uint8_t* px[NT];
-    const float2* pf[NT];
+    const float* pf[NT];
+    // nb blocks and nf factors a vector
     template <class Row>
-    __device__ __forceinline__ Vectors(const uint8_t* h, const float2* f, uint32_t nb, const Row* rows, uint32_t count, uint32_t lane) {
+    __device__ __forceinline__ Vectors(const uint8_t* h, const float* f, uint32_t nb, uint32_t nf, const Row* rows, uint32_t count, uint32_t lane) {
         const uint32_t g = lane >> 2, t = lane & 3;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             const uint32_t i = min(NT == 1 ? g / 2 : g, count - 1), k = min(token_of<NT>(n, t), count - 1);
             px[n] = h + (size_t)(rows[i] * 2u + (NT == 1 ? g & 1 : n)) * (nb * 64) + t * 16;
-            pf[n] = f + (size_t)rows[k] * nb;
+            pf[n] = f + (size_t)rows[k] * nf;
         }
     }
-    __device__ __forceinline__ void advance(uint32_t blocks) {
+    __device__ __forceinline__ void advance(uint32_t blocks, uint32_t factors) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             px[n] += (size_t)blocks * 64;
-            pf[n] += blocks;
+            pf[n] += factors;
         }
     }
-    __device__ __forceinline__ void load(int block, uint4* parts, float2* factor) const {
+    __device__ __forceinline__ void load(int block, uint4* parts) const {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            parts[n] = *reinterpret_cast<const uint4*>(px[n] + block * 64);
-            factor[n] = pf[n][block];
-        }
+        for (int n = 0; n < NT; ++n) parts[n] = *reinterpret_cast<const uint4*>(px[n] + block * 64);
+    }
+    __device__ __forceinline__ void load_factor(int at, float* factor) const {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) factor[n] = pf[n][at];
     }
 };
-// Blocks of the vectors that are in registers: a chunk's, four at most.
+// Blocks of the vectors that are in registers: a chunk's, four at most.  Factors: one for a chunk of two matrices (all its blocks are
+// here then), one a block for a chunk of one.
 template <bool FOUR, int MATS>
 struct Ahead {
     static constexpr uint32_t B = Chunk<FOUR, MATS>::blocks;
     template <int NT>
     static constexpr uint32_t group = std::min(B, NT == 1 || MATS == 2 ? 4u : 2u);
     static constexpr uint32_t size = std::max(group<1>, 2 * group<2>);
+    static_assert(MATS == 1 || (group<1> == B && group<2> == B), "a chunk of two matrices is one group");
     uint4 parts[size];
-    float2 factor[size];
+    float factor[MATS == 2 ? 2 : size];
     template <int NT>
     __device__ __forceinline__ void load(const Vectors<NT>& x, int block, uint32_t j) {
-        x.load(block, parts + j * NT, factor + j * NT);
+        x.load(block, parts + j * NT);
+        if (MATS == 1) x.load_factor(block, factor + j * NT);
     }
     // the first blocks of a pass over chunks c0 .. c1 - 1
     template <int NT>
     __device__ __forceinline__ void start(Vectors<NT> x, uint32_t c0, uint32_t c1, uint32_t nb) {
         if (c0 >= c1) return;
-        x.advance(c0 * B);
+        x.advance(c0 * B, MATS == 2 ? c0 : c0 * B);
 #pragma unroll
         for (uint32_t j = 0; j < group<NT>; ++j)
             if (c0 * B + j < nb) load<NT>(x, j, j);
+        if (MATS == 2) x.load_factor(0, factor);
     }
 };
 
-// acc[m][n] += block j of the two 16-row tiles of 32 rows: rows 16 m + g and 16 m + g + 8, token token_of(n, t).  codes: where the
-// lane's row begins, its unit swizzled; a stage begins at a multiple of 128 bytes, so the block's number goes into the address's bits.
-template <bool FOUR, int MATS, int NT, class D>
-__device__ __forceinline__ void multiply(uint32_t codes, uint32_t j, const uint4* parts, const float2* factor, D scale,
-                                         float (&acc)[2][NT][2]) {
+// Products of block j with the two 16-row tiles of 32 rows: use(m, n, h, sum), sum that of row 16 m + 8 h + g, token token_of(n, t).
+// codes: where the lane's row begins, its unit swizzled; a stage begins at a multiple of 128 bytes, so the block's number goes into
+// the address's bits.
+template <bool FOUR, int MATS, int NT, class Use>
+__device__ __forceinline__ void multiply(uint32_t codes, uint32_t j, const uint4* parts, Use use) {
     using C = Chunk<FOUR, MATS>;
     uint32_t a[2][2][4];
     if (FOUR) {
         uint32_t w[4];
         ldmatrix_x4(w, codes ^ j * 16);
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const uint32_t u = w[2 * i + h];
-                a[i][0][h] = (u << 4) & 0x00f000f0u;
-                a[i][0][2 + h] = (u >> 4) & 0x00f000f0u;
-                a[i][1][h] = u & 0x00f000f0u;
-                a[i][1][2 + h] = (u >> 8) & 0x00f000f0u;
-            }
+        for (int i = 0; i < 2; ++i) a_of_nibbles(w[2 * i], w[2 * i + 1], a[i]);
     } else {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             uint32_t w[4];
             ldmatrix_x4(w, (codes ^ j * 32) + i * 16 * C::bytes);
 #pragma unroll
-            for (int h = 0; h < 4; ++h) {
-                const uint32_t u = w[h] ^ 0x80808080u;
-                a[i][h >> 1][h & 1] = __byte_perm(u, 0, 0x4140);
-                a[i][h >> 1][2 + (h & 1)] = __byte_perm(u, 0, 0x4342);
-            }
+            for (int h = 0; h < 4; ++h) w[h] ^= 0x80808080u;  // code + 128
+            a_of_bytes(w, a[i]);
         }
     }
     float s[2][4];
-    auto both = [&](auto use) {  // neighbouring products do not wait for each other
-        use(0);
-        use(1);
+    auto both = [&](auto product) {  // neighbouring products do not wait for each other
+        product(0);
+        product(1);
     };
     if (NT > 1) {
         both([&](int i) { mma_f16_new(s[i], a[i][0], parts[NT - 1].x, parts[NT - 1].y); });
@@ -464,10 +464,7 @@ __device__ __forceinline__ void multiply(uint32_t codes, uint32_t j, const uint4
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const float sum = NT == 1 ? s[i][2 * h] + s[i][2 * h + 1] : s[i][2 * h + n];
-                acc[i][n][h] = fmaf(fmaf(sum, factor[n].x, factor[n].y), scale(2 * i + h), acc[i][n][h]);
-            }
+            for (int h = 0; h < 2; ++h) use(i, n, h, NT == 1 ? s[i][2 * h] + s[i][2 * h + 1] : s[i][2 * h + n]);
     });
 }
 
@@ -482,7 +479,7 @@ __device__ __forceinline__ void dot_chunks(Vectors<NT> x, Ahead<FOUR, MATS>& ahe
     using C = Chunk<FOUR, MATS>;
     // where the lane's row begins for ldmatrix, block 0: a row is a tile's of 32 (Q4_0) or of 16, then its second unit (Q8_0)
     const uint32_t lane_row = FOUR ? lane : lane & 15, lane_at = lane_row * C::bytes + ((FOUR ? 0 : lane >> 4) ^ C::swizzle(lane_row)) * 16;
-    x.advance(c0 * B);
+    x.advance(c0 * B, MATS == 2 ? c0 : c0 * B);
 #pragma unroll
     for (int a = 0; a < MATS; ++a)
 #pragma unroll
@@ -497,19 +494,31 @@ __device__ __forceinline__ void dot_chunks(Vectors<NT> x, Ahead<FOUR, MATS>& ahe
 #pragma unroll
             for (int a = 0; a < MATS; ++a) {
                 const typename S::template Of<G> d(stage + kCodes + a * 32 * S::pitch, j0, lane >> 2, nb);
+                float chunk[2][NT][2];  // of two matrices' chunks, whose blocks share a factor
 #pragma unroll
                 for (uint32_t j = 0; j < G; ++j) {
                     const uint32_t block = c * B + j0 + j;
                     if (WHOLE || block < nb)
-                        multiply<FOUR, MATS, NT>(codes + a * (kCodes / 2), j0 + j, ahead.parts + j * NT, ahead.factor + j * NT,
-                                                 [&](int row) { return d(row, j); }, acc[a]);
+                        multiply<FOUR, MATS, NT>(codes + a * (kCodes / 2), j0 + j, ahead.parts + j * NT, [&](int m, int n, int h, float sum) {
+                            if (MATS == 1) acc[a][m][n][h] = fmaf(sum * ahead.factor[j * NT + n], d(2 * m + h, j), acc[a][m][n][h]);
+                            else chunk[m][n][h] = j == 0 ? sum * d(2 * m + h, j) : fmaf(sum, d(2 * m + h, j), chunk[m][n][h]);
+                        });
                     if (a == MATS - 1) {
                         const uint32_t later = j0 + j + (j0 + G < B ? G : TEAM * B + G - B);
                         if ((j0 + G < B || more) && (WHOLE || c * B + later < nb)) ahead.template load<NT>(x, later, j);
                     }
                 }
+                if (MATS == 2) {
+#pragma unroll
+                    for (int m = 0; m < 2; ++m)
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) acc[a][m][n][h] = fmaf(chunk[m][n][h], ahead.factor[n], acc[a][m][n][h]);
+                }
             }
-        x.advance(TEAM * B);
+        if (MATS == 2 && more) x.load_factor(TEAM, ahead.factor);
+        x.advance(TEAM * B, MATS == 2 ? TEAM : TEAM * B);
         done();
     }
 }
@@ -595,7 +604,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_inner_kernel(MoeParams p) 
     Ahead<FOUR, 2> vectors;
     auto begin = [&](auto groups) {
         constexpr int NT = decltype(groups)::value;
-        return Vectors<NT>(p.xh, p.xs, nb, plan->token + now.at, min(kGroup, now.count(plan)), lane);
+        return Vectors<NT>(p.xh, p.xs, nb, chunks, plan->token + now.at, min(kGroup, now.count(plan)), lane);
     };
     auto begin_ahead = [&]() {
         if (now.unit >= units) return;
@@ -646,7 +655,9 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_inner_kernel(MoeParams p) 
                 const float h = a / (1.0f + expf(-a)) * b;
                 const uint32_t slot = slots[i];
                 uint8_t* hi = p.hh + ((size_t)slot * 2 * nbf + rows32) * 64;
-                split_block(h, lane, p.down4 != 0, hi, hi + (size_t)nbf * 64, p.hs + (size_t)slot * nbf + rows32);
+                const float up = split_lift(warp_max(fabsf(h)));
+                split_block(h, up, lane, p.down4 != 0, hi, hi + (size_t)nbf * 64);
+                if (lane == 0) p.hs[(size_t)slot * nbf + rows32] = split_factor(up);
             }
             if (NT > 1) barrier();
             turn ^= 1;
@@ -765,7 +776,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_down_kernel(MoeParams p) {
     Ahead<FOUR, 1> vectors;
     auto begin = [&](auto groups) {
         constexpr int NT = decltype(groups)::value;
-        return Vectors<NT>(p.hh, p.hs, nb, plan->list + now.at, min(kGroup, plan->begin[now.a + 1] - now.at), lane);
+        return Vectors<NT>(p.hh, p.hs, nb, nb, plan->list + now.at, min(kGroup, plan->begin[now.a + 1] - now.at), lane);
     };
     auto begin_ahead = [&]() {
         if (!now.valid()) return;
@@ -938,8 +949,8 @@ vx_status vx_moe_create(vx_context* ctx, const float* router, size_t experts, co
         at += round_up(bytes, 256);
         return o;
     };
-    const size_t o_logits = take(p.slices * max_tokens * experts * 4), o_xh = take(max_tokens * 2 * nbh * 64), o_xs = take(max_tokens * nbh * 8),
-                 o_hh = take(slots * 2 * nbf * 64), o_hs = take(slots * nbf * 8);
+    const size_t o_logits = take(p.slices * max_tokens * experts * 4), o_xh = take(max_tokens * 2 * nbh * 64), o_xs = take(max_tokens * nbh * 4),
+                 o_hh = take(slots * 2 * nbf * 64), o_hs = take(slots * nbf * 4);
     const cudaError_t e = device_malloc(ctx, reinterpret_cast<void**>(&m->workspace), at);
     if (e != cudaSuccess) {
         (void)cudaGetLastError();
@@ -948,9 +959,9 @@ vx_status vx_moe_create(vx_context* ctx, const float* router, size_t experts, co
     uint8_t* w = m->workspace;
     p.logits = reinterpret_cast<float*>(w + o_logits);
     p.xh = w + o_xh;
-    p.xs = reinterpret_cast<float2*>(w + o_xs);
+    p.xs = reinterpret_cast<float*>(w + o_xs);
     p.hh = w + o_hh;
-    p.hs = reinterpret_cast<float2*>(w + o_hs);
+    p.hs = reinterpret_cast<float*>(w + o_hs);
     *out = m.release();
     return VX_OK;
 }
