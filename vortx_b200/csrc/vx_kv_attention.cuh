@@ -599,6 +599,19 @@ kv_attention_kernel(AttnParams p) {
                             }
                         sum[n][e] = fmaf(sum[n][e], fall[n][e], add);
                     }
+                if (masked) {  // -0 for what a row does not attend to, 0 for a weight that is nothing
+#pragma unroll
+                    for (int n = 0; n < N; ++n)
+#pragma unroll
+                        for (int e = 0; e < E; ++e)
+#pragma unroll
+                            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                                for (int h = 0; h < 2; ++h) {
+                                    const uint32_t lo = g + 8 * h;
+                                    if (!(may[n][e] >> (m * 16 + lo) & 1)) pwf[p_slot(row_of(n, e), (lo & 3) * 2 + m) * 4 + (lo >> 2)] = -0.0f;
+                                }
+                }
                 __syncwarp();
                 // ---- the value blocks' scales: tokens t + 4 i + 16 s of every lane, and the power of two that they allow
                 const uint32_t vrec = rec + Shape::k_bytes, vscales = vrec + kv_code_bytes(V4, NB) + t * 16;
@@ -699,8 +712,8 @@ kv_attention_kernel(AttnParams p) {
                                 const __half2 l = __hfma2(bits_h2(pl[n][x]), d[x], __hfma2(bits_h2(ph[n][x]), d[x], __hneg2(h)));
                                 hi_[n][x] = h2_bits(h);
                                 lo_[n][x] = h2_bits(l);
-                                if (decltype(some_masked)::value) {  // what is no number in a masked place stays there
-                                    const uint32_t on = (ph[n][x] & 0x7fffu ? 0xffffu : 0u) | (ph[n][x] & 0x7fff0000u ? 0xffff0000u : 0u);
+                                if (decltype(some_masked)::value) {  // what is no number in a masked place (weight -0) stays there
+                                    const uint32_t on = ((ph[n][x] & 0xffffu) == 0x8000u ? 0u : 0xffffu) | (ph[n][x] >> 16 == 0x8000u ? 0u : 0xffff0000u);
                                     hi_[n][x] &= on;
                                     lo_[n][x] &= on;
                                 }
