@@ -40,3 +40,17 @@ def test_nan_in_a_value_whose_weight_is_nothing(backend, vt, dim, heads, kv_head
     got[:n, :, 32:64] = 0.0
     want[0][:, :, 32:64] = 0.0
     s.check(got, v=want, k=[quantised(s.kt, k) for k in s.k])
+
+
+@pytest.mark.parametrize("vt", [vb.Q8_0, vb.Q4_0])
+@pytest.mark.parametrize("dim", [64, 96, 128, 256])
+@pytest.mark.parametrize("group", [1, 2, 4])
+def test_rows_that_attend_to_large_and_to_small_values(backend, vt, dim, group):
+    """Four drafted tokens in one tile, two of large values and two whose values are 2^-22 of that; each attends to its own
+    kind.  With 1, 2 and 4 query heads to a head of keys: 4, 8 and 16 rows to a thread block."""
+    s = Scene(backend, [(0, 4), (0, 4)], 2 * group, 2, dim, 32, vb.Q8_0, vt, seed=dim + group)
+    v = [a * np.float32(2.0) ** np.array([16, -6, 16, -6], np.float32)[:, None, None] for a in s.v]
+    may = np.array([[1, 0, 0, 0], [0, 1, 0, 0], [1, 0, 1, 0], [0, 1, 0, 1]], bool)
+    mask = np.tile((may << np.arange(4)).sum(1).astype(np.uint32), 2).reshape(8, 1)
+    want = _with_values(s, v)
+    s.check(s.run(mask), [may, may], v=want)

@@ -9,8 +9,8 @@
 //   scores   per block of 32 values: sum of code * (q hi + q lo) on the tensor cores, times the block's scale, in f32
 //   softmax  base 2 (log2 e is multiplied into q), running maximum per row, weights p <= 1
 //   output   the value blocks' scales d are per token, so they go into the weights.  With 2^e the power of two below a
-//            token's largest |d|, p 2^e is lifted so that the tile's largest lies in [2^12, 2^13) and split into two f16
-//            parts, once per tile; the f16 scales become d 2^(1 - e), in [2, 4) for the largest, exact; and the two parts of
+//            token's largest |d|, p 2^e is lifted so that the row's largest of the tile lies in [2^12, 2^13) and split into
+//            two f16 parts, once per tile; the f16 scales become d 2^(1 - e), in [2, 4) for the largest, exact; and the two parts of
 //            the product, hi = p hi * d and lo = p lo * d + (p hi * d - hi), are three f16 operations per pair of
 //            tokens and block (the difference is exact).  A token of no weight, however large, costs the others nothing
 // The runs are shares of all tiles of all (sequence, head, group of rows), see Share.  A share that covers the tiles of a
@@ -451,7 +451,7 @@ kv_attention_kernel(AttnParams p) {
         __syncthreads();
         const uint32_t qs = smem_addr(qf) + lane * 16;
         float inv[N][E];
-        float top[N][E], sum[N][E], acc[2 * NB][N][2 * E], unit = 1.0f;  // acc counts 1 / (2 unit)
+        float top[N][E], sum[N][E], acc[2 * NB][N][2 * E], unit[N][E];  // acc counts 1 / (2 unit)
 #pragma unroll
         for (int n = 0; n < N; ++n) {
 #pragma unroll
@@ -459,6 +459,7 @@ kv_attention_kernel(AttnParams p) {
                 inv[n][e] = inv_lift[row_of(n, e)];
                 top[n][e] = kNone;
                 sum[n][e] = 0.0f;
+                unit[n][e] = 1.0f;
             }
 #pragma unroll
             for (int d = 0; d < 2 * NB; ++d)
@@ -628,7 +629,7 @@ kv_attention_kernel(AttnParams p) {
                     most[3] = __hmax2(most[3], __habs2(bits_h2(dv[b].w)));
                 }
                 __half2 back[4];  // 2^(1 - e)
-                float pe[N][8], largest = 0.0f;
+                float pe[N][8];
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
                     const uint32_t e = h2_bits(most[x]) & 0x7c007c00u;
@@ -637,8 +638,10 @@ kv_attention_kernel(AttnParams p) {
                     pe[0][2 * x] = f.x;
                     pe[0][2 * x + 1] = f.y;
                 }
+                float largest[N], now[N][E];
 #pragma unroll
-                for (int n = N - 1; n >= 0; --n)
+                for (int n = N - 1; n >= 0; --n) {
+                    largest[n] = 0.0f;
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
                         const uint4 f = lds128(pw + p_slot(kParts ? g / 2 : n * 8 + g, t * 2 + x) * 16);
@@ -646,26 +649,38 @@ kv_attention_kernel(AttnParams p) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             pe[n][4 * x + i] = __uint_as_float(w[i]) * pe[0][4 * x + i];
-                            largest = fmaxf(largest, pe[n][4 * x + i]);
+                            largest[n] = fmaxf(largest[n], pe[n][4 * x + i]);
                         }
                     }
-                largest = warp_max(largest);
-                if (largest > 0.0f) {
-                    const float now = fminf(lift(largest) * 0.25f, __uint_as_float((40u + 127u) << 23));
-                    const float ratio = now * __uint_as_float(0x7f000000u - __float_as_uint(unit));  // powers of two
-                    unit = now;
-#pragma unroll
-                    for (int n = 0; n < N; ++n)
-#pragma unroll
-                        for (int e = 0; e < E; ++e) fall[n][e] *= ratio;
                 }
+                // Each row has its own power of two: found by the four lanes with its weights, given to those with its output.
+#pragma unroll
+                for (int o = 1; o < 4; o *= 2)
+#pragma unroll
+                    for (int n = 0; n < N; ++n) largest[n] = fmaxf(largest[n], __shfl_xor_sync(0xffffffffu, largest[n], o));
+#pragma unroll
+                for (int n = 0; n < N; ++n) {
+                    // 2^12 over the power of two below the largest, 2^40 at most: what a row without weights has here
+                    const float up = __uint_as_float(min(((12u + 2u * 127u) << 23) - (__float_as_uint(largest[n]) & 0x7f800000u), (40u + 127u) << 23));
+#pragma unroll
+                    for (int e = 0; e < E; ++e) now[n][e] = __shfl_sync(0xffffffffu, up, kParts ? 8 * t : 8 * t + 4 * e);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) pe[n][i] *= up;
+                }
+#pragma unroll
+                for (int n = 0; n < N; ++n)
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        fall[n][e] *= now[n][e] * __uint_as_float(0x7f000000u - __float_as_uint(unit[n][e]));  // powers of two
+                        unit[n][e] = now[n][e];
+                    }
                 uint32_t ph[N][4], pl[N][4];  // pairs of tokens
                 uint32_t minus[N][4];         // what hi is to be taken off for the lane's column: of the parts of four rows, the first has hi itself
 #pragma unroll
                 for (int n = 0; n < N; ++n)
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
-                        split_f16(pe[n][2 * x] * unit, pe[n][2 * x + 1] * unit, &ph[n][x], &pl[n][x]);
+                        split_f16(pe[n][2 * x], pe[n][2 * x + 1], &ph[n][x], &pl[n][x]);
                         minus[n][x] = kParts && !(g & 1) ? 0u : ph[n][x];
                         if (kParts && !(g & 1)) pl[n][x] = 0u;
                     }
@@ -754,7 +769,6 @@ kv_attention_kernel(AttnParams p) {
         cp_async_wait<0>();
 
         // ---- the warps' parts become one -------------------------------------------------------------------------
-        const float down = 0.5f / unit;
 #pragma unroll
         for (int n = 0; n < N; ++n)
 #pragma unroll
@@ -774,7 +788,7 @@ kv_attention_kernel(AttnParams p) {
                 float m = kNone;
 #pragma unroll
                 for (uint32_t w = 0; w < W; ++w) m = fmaxf(m, ml[w * R + row_of(n, e)].x);
-                const float f = top[n][e] == kNone ? 0.0f : ex2(top[n][e] - m) * down;
+                const float f = top[n][e] == kNone ? 0.0f : ex2(top[n][e] - m) * __uint_as_float(0x7e800000u - __float_as_uint(unit[n][e]));
 #pragma unroll
                 for (int d = 0; d < 2 * NB; ++d) {
                     acc[d][n][e] *= f;
