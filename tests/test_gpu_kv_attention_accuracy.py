@@ -1,11 +1,17 @@
 """Attention over the quantised cache where values are not numbers or differ by many powers of two: each number of the result is held
-to the tolerance of its own sum, (2 d + 2^-18) sum p |v| over the tokens of its row and its place in the head
-(decode_ref.attention), whatever other rows, tokens or blocks hold."""
+to the tolerance of its own sum, whatever other rows, tokens or blocks hold.
+
+Tolerance.  decode_ref.attention's (2 d + 2^-18) sum p |v|, over the tokens of the number's row and its place j in the head, and
+where tokens' weights in the block of 32 values differ widely, what the two f16 parts of a weight leave: with w_t = p_t |scale_t| of
+that block, at most 2^-21 max(w) |code_tj| for each token.  For the largest w of the block is at least 2^-1 in the units in which it is
+split (a row's largest weight in [2^12, 2^13), times scales of 2^-13 and more; or w itself in [2^14, 2^15)), and in them a
+weight's parts miss at most 2^-25, times a scale below 4, and their product's two roundings 2^-25 each: 2^-22.4 in all, next
+to the 2^-22 of w_t itself that 2^-18 covers."""
 import numpy as np
 import pytest
 
 import vortx_b200 as vb
-from decode_ref import quantised
+from decode_ref import attention, quantised
 from test_gpu_kv_attention import Scene, _rng
 
 pytestmark = pytest.mark.gpu
@@ -19,6 +25,27 @@ def _with_values(s, v):
     kv = [s._b(np.concatenate([a.reshape(len(a), -1) for a in x])) for x in (s.k, s.v)]
     s.cache.append(None, *kv, vb.CacheRows(s._b(s.table), s._b(every), s._b(np.zeros(len(total), np.int32)), int(every[-1])))
     return [quantised(s.vt, a) for a in s.v]
+
+
+def _check(s, got, v, may=None, scale=None):
+    """v: what the values' codes stand for; may[s]: [n, n] among the new tokens, None: those up to a row's own."""
+    scale = s.dim ** -0.5 if scale is None else scale
+    for at, (c, n) in enumerate(s.seqs):
+        k = quantised(s.kt, s.k[at])
+        blocks = np.abs(s.v[at]).reshape(c + n, s.kv_heads, -1, 32).max(-1)
+        d = (blocks / np.float32(127 if s.vt == vb.Q8_0 else 7)).astype(np.float16).astype(np.float64).repeat(32, -1)
+        code = np.divide(np.abs(v[at]), d, out=np.zeros_like(v[at]), where=d > 0)
+        ok = np.concatenate([np.ones((n, c), bool), np.tril(np.ones((n, n), bool)) if may is None else may[at]], 1)
+        for h in range(s.heads):
+            q, hk = s.q[s.begin[at]:s.begin[at] + n, h].astype(np.float64), h // (s.heads // s.kv_heads)
+            want, tol = attention(q, k[:, hk], v[at][:, hk], ok, scale)
+            score = np.where(ok, scale * q @ k[:, hk].T, -np.inf)
+            p = np.exp(score - score.max(1, keepdims=True))
+            p /= p.sum(1, keepdims=True)
+            for i in range(n):
+                tol[i] += 2.0 ** -21 * (p[i][:, None] * d[:, hk]).max(0) * code[ok[i], hk].sum(0)
+            err = np.abs(got[s.begin[at]:s.begin[at] + n, h] - want)
+            assert (err <= tol).all(), (at, h, float((err / tol).max()))
 
 
 @pytest.mark.parametrize("vt", [vb.Q8_0, vb.Q4_0])
@@ -39,7 +66,8 @@ def test_nan_in_a_value_whose_weight_is_nothing(backend, vt, dim, heads, kv_head
     want[0][at] = 0.0
     got[:n, :, 32:64] = 0.0
     want[0][:, :, 32:64] = 0.0
-    s.check(got, v=want, k=[quantised(s.kt, k) for k in s.k])
+    s.v[0][at] = 0.0
+    _check(s, got, want)
 
 
 @pytest.mark.parametrize("vt", [vb.Q8_0, vb.Q4_0])
@@ -53,4 +81,43 @@ def test_rows_that_attend_to_large_and_to_small_values(backend, vt, dim, group):
     may = np.array([[1, 0, 0, 0], [0, 1, 0, 0], [1, 0, 1, 0], [0, 1, 0, 1]], bool)
     mask = np.tile((may << np.arange(4)).sum(1).astype(np.uint32), 2).reshape(8, 1)
     want = _with_values(s, v)
-    s.check(s.run(mask), [may, may], v=want)
+    _check(s, s.run(mask), want, [may, may])
+
+
+@pytest.mark.parametrize("vt", [vb.Q8_0, vb.Q4_0])
+@pytest.mark.parametrize("dim,heads,kv_heads,n", [(64, 2, 2, 1), (96, 4, 2, 3), (128, 8, 2, 3), (256, 4, 2, 1)])
+@pytest.mark.parametrize("down", [10, 14, 15, 16, 18, 22])
+@pytest.mark.parametrize("pattern", ["every token", "in turns"])
+def test_blocks_of_a_token_that_differ(backend, vt, dim, heads, kv_heads, n, down, pattern):
+    """A block of 32 values is 2^-down of the others': the second one of every token, or the first and second of tokens in turn."""
+    s = Scene(backend, [(100, n), (3, n)], heads, kv_heads, dim, 32, vb.Q8_0, vt, seed=dim + down)
+    v = [a * np.float32(2.0 ** 14) for a in s.v]
+    for a in v:
+        small = np.float32(2.0 ** -down)
+        a[:, :, 32:64] *= small
+        if pattern == "in turns":
+            a[::2, :, 32:64] /= small
+            a[::2, :, :32] *= small
+    want = _with_values(s, v)
+    _check(s, s.run(), want)
+
+
+@pytest.mark.parametrize("vt", [vb.Q8_0, vb.Q4_0])
+@pytest.mark.parametrize("dim,heads,kv_heads", [(64, 2, 2), (96, 4, 2), (128, 8, 2), (256, 2, 2)])
+def test_blocks_that_only_tokens_of_little_weight_have(backend, vt, dim, heads, kv_heads):
+    """The heaviest tokens' second block is zeros; what stands there comes from tokens of 2^-24 of their weight.  The last block is
+    zeros in every token."""
+    s = Scene(backend, [(90, 1)], heads, kv_heads, dim, 32, vb.Q8_0, vt, seed=dim)
+    light = np.arange(91) % 3 == 1
+    s.q[:] = 0.0
+    s.q[:, :, 0] = 1.0
+    s.k[0][:, :, 0] = np.where(light, -16.6, 0.0)[:, None]       # 16.6 = 24 ln 2
+    s.k[0][:, :, 1:] *= np.float32(0.01)
+    v = s.v[0].copy()
+    v[~light, :, 32:64] = 0.0
+    if dim > 64:
+        v[:, :, -32:] = 0.0
+    want = _with_values(s, [v])
+    got = s.run(scale=1.0)
+    _check(s, got, want, scale=1.0)
+    assert np.abs(got[:, :, 32:64]).max() > 0 and (dim == 64 or (got[:, :, -32:] == 0).all())

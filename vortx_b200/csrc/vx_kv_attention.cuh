@@ -10,9 +10,12 @@
 //   softmax  base 2 (log2 e is multiplied into q), running maximum per row, weights p <= 1
 //   output   the value blocks' scales d are per token, so they go into the weights.  With 2^e the power of two below a
 //            token's largest |d|, p 2^e is lifted so that the row's largest of the tile lies in [2^12, 2^13) and split into
-//            two f16 parts, once per tile; the f16 scales become d 2^(1 - e), in [2, 4) for the largest, exact; and the two parts of
+//            two f16 parts, once per tile; the f16 scales become d 2^(1 - e), in [2, 4) for the largest; and the two parts of
 //            the product, hi = p hi * d and lo = p lo * d + (p hi * d - hi), are three f16 operations per pair of
-//            tokens and block (the difference is exact).  A token of no weight, however large, costs the others nothing
+//            tokens and block (the difference is exact).  A token of no weight, however large, costs the others nothing.
+//            That holds while a token's scales are within 2^14 of its largest, so that none becomes a small number of
+//            f16; where a token with weight has a smaller one (or zeros in a block where others have more), p d is
+//            taken in f32, lifted per row and block, and split (see `wide`)
 // The runs are shares of all tiles of all (sequence, head, group of rows), see Share.  A share that covers the tiles of a
 // (sequence, head, rows) only in part leaves maximum, sum and unnormalised output in the workspace, at most two per block,
 // and the last block to finish a part joins them all, in their order.
@@ -617,16 +620,18 @@ kv_attention_kernel(AttnParams p) {
                 // ---- the value blocks' scales: tokens t + 4 i + 16 s of every lane, and the power of two that they allow
                 const uint32_t vrec = rec + Shape::k_bytes, vscales = vrec + kv_code_bytes(V4, NB) + t * 16;
                 uint4 dv[NB];
-                __half2 most[4];
+                __half2 most[4], least[4];
 #pragma unroll
                 for (int x = 0; x < 4; ++x) most[x] = bits_h2(0x04000400u);  // 2^-14: smaller scales keep their own size
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
                     dv[b] = lds128(vscales + b * 64);
-                    most[0] = __hmax2(most[0], __habs2(bits_h2(dv[b].x)));  // of NaN and a number, the number
-                    most[1] = __hmax2(most[1], __habs2(bits_h2(dv[b].y)));
-                    most[2] = __hmax2(most[2], __habs2(bits_h2(dv[b].z)));
-                    most[3] = __hmax2(most[3], __habs2(bits_h2(dv[b].w)));
+                    const uint32_t d[4] = {dv[b].x, dv[b].y, dv[b].z, dv[b].w};
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {  // of NaN and a number, the number
+                        most[x] = __hmax2(most[x], __habs2(bits_h2(d[x])));
+                        least[x] = b == 0 ? __habs2(bits_h2(d[x])) : __hmin2(least[x], __habs2(bits_h2(d[x])));
+                    }
                 }
                 __half2 back[4];  // 2^(1 - e)
                 float pe[N][8];
@@ -638,6 +643,13 @@ kv_attention_kernel(AttnParams p) {
                     pe[0][2 * x] = f.x;
                     pe[0][2 * x + 1] = f.y;
                 }
+                // whether a token may have a scale too far below its largest
+                auto small_of = [&](const __half2 (&d)[4]) {
+                    const __half2 low = __hmin2(__hmin2(__hmul2(d[0], back[0]), __hmul2(d[1], back[1])),
+                                                __hmin2(__hmul2(d[2], back[2]), __hmul2(d[3], back[3])));
+                    return !__hbge2(low, bits_h2(0x08000800u));  // 2^-13
+                };
+                const bool small_here = small_of(least);
                 float largest[N], now[N][E];
 #pragma unroll
                 for (int n = N - 1; n >= 0; --n) {
@@ -685,7 +697,18 @@ kv_attention_kernel(AttnParams p) {
                         if (kParts && !(g & 1)) pl[n][x] = 0u;
                     }
                 // ---- output ------------------------------------------------------------------------------------------
-                auto output = [&](auto some_masked) {
+                auto weights = [&](int n, float (&w)[8]) {  // of the lane's row and tokens, once more
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const uint4 f = lds128(pw + p_slot(kParts ? g / 2 : n * 8 + g, t * 2 + x) * 16);
+                        w[4 * x] = __uint_as_float(f.x);
+                        w[4 * x + 1] = __uint_as_float(f.y);
+                        w[4 * x + 2] = __uint_as_float(f.z);
+                        w[4 * x + 3] = __uint_as_float(f.w);
+                    }
+                };
+                auto output = [&](auto some_masked, auto in_f32) {
+                    constexpr bool kMasked = decltype(some_masked)::value, kWide = decltype(in_f32)::value;
 #pragma unroll
                     for (int b = 0; b < NB; ++b) {
                         const __half2 d[4] = {__hmul2(bits_h2(dv[b].x), back[0]), __hmul2(bits_h2(dv[b].y), back[1]),
@@ -719,20 +742,47 @@ kv_attention_kernel(AttnParams p) {
                             }
                         }
                         uint32_t hi_[N][4], lo_[N][4];  // with four rows, the lane's part is in lo_
+                        float back_to[N][E];            // what the block's sums count in the output's unit
+                        if constexpr (!kWide) {
 #pragma unroll
-                        for (int n = 0; n < N; ++n)
+                            for (int n = 0; n < N; ++n)
 #pragma unroll
-                            for (int x = 0; x < 4; ++x) {
-                                const __half2 h = __hmul2(bits_h2(minus[n][x]), d[x]);
-                                const __half2 l = __hfma2(bits_h2(pl[n][x]), d[x], __hfma2(bits_h2(ph[n][x]), d[x], __hneg2(h)));
-                                hi_[n][x] = h2_bits(h);
-                                lo_[n][x] = h2_bits(l);
-                                if (decltype(some_masked)::value) {  // what is no number in a masked place (weight -0) stays there
-                                    const uint32_t on = ((ph[n][x] & 0xffffu) == 0x8000u ? 0u : 0xffffu) | (ph[n][x] >> 16 == 0x8000u ? 0u : 0xffff0000u);
-                                    hi_[n][x] &= on;
-                                    lo_[n][x] &= on;
+                                for (int x = 0; x < 4; ++x) {
+                                    const __half2 h = __hmul2(bits_h2(minus[n][x]), d[x]);
+                                    const __half2 l = __hfma2(bits_h2(pl[n][x]), d[x], __hfma2(bits_h2(ph[n][x]), d[x], __hneg2(h)));
+                                    hi_[n][x] = h2_bits(h);
+                                    lo_[n][x] = h2_bits(l);
+                                    if (kMasked) {  // what is no number in a masked place (weight -0) stays there
+                                        const uint32_t on = ((ph[n][x] & 0xffffu) == 0x8000u ? 0u : 0xffffu) | (ph[n][x] >> 16 == 0x8000u ? 0u : 0xffff0000u);
+                                        hi_[n][x] &= on;
+                                        lo_[n][x] &= on;
+                                    }
+                                }
+                        } else {
+                            const uint32_t own[4] = {dv[b].x, dv[b].y, dv[b].z, dv[b].w};
+#pragma unroll
+                            for (int n = 0; n < N; ++n) {
+                                float w[8], most_ = 0.0f;
+                                weights(n, w);
+#pragma unroll
+                                for (int x = 0; x < 4; ++x) {
+                                    const float2 f = __half22float2(bits_h2(own[x]));
+                                    w[2 * x] = __float_as_uint(w[2 * x]) == 0x80000000u ? 0.0f : w[2 * x] * f.x;
+                                    w[2 * x + 1] = __float_as_uint(w[2 * x + 1]) == 0x80000000u ? 0.0f : w[2 * x + 1] * f.y;
+                                    most_ = fmaxf(most_, fmaxf(fabsf(w[2 * x]), fabsf(w[2 * x + 1])));
+                                }
+                                most_ = fmaxf(most_, __shfl_xor_sync(0xffffffffu, most_, 1));
+                                most_ = fmaxf(most_, __shfl_xor_sync(0xffffffffu, most_, 2));
+                                const float up = lift(most_), inverse = __uint_as_float(0x7f000000u - __float_as_uint(up));
+#pragma unroll
+                                for (int e = 0; e < E; ++e) back_to[n][e] = 2.0f * unit[n][e] * __shfl_sync(0xffffffffu, inverse, kParts ? 8 * t : 8 * t + 4 * e);
+#pragma unroll
+                                for (int x = 0; x < 4; ++x) {
+                                    split_f16(w[2 * x] * up, w[2 * x + 1] * up, &hi_[n][x], &lo_[n][x]);
+                                    if (kParts && !(g & 1)) lo_[n][x] = hi_[n][x];
                                 }
                             }
+                        }
                         // The tensor cores cut their f32 sums off instead of rounding them: a tile's sum is taken from
                         // zero and added to the output here, or the loss would grow with the number of tiles.
                         float o[N][2][4];
@@ -750,16 +800,45 @@ kv_attention_kernel(AttnParams p) {
                         }
                         step([&](int n, int m) {
 #pragma unroll
-                            for (int c = 0; c < 2 * E; ++c)
-                                acc[2 * b + m][n][c] = fmaf(acc[2 * b + m][n][c], fall[n][c % E], kParts ? o[n][m][2 * c] + o[n][m][2 * c + 1] : o[n][m][c]);
+                            for (int c = 0; c < 2 * E; ++c) {
+                                const float sum_ = kParts ? o[n][m][2 * c] + o[n][m][2 * c + 1] : o[n][m][c];
+                                acc[2 * b + m][n][c] = fmaf(acc[2 * b + m][n][c], fall[n][c % E], kWide ? sum_ * back_to[n][c % E] : sum_);
+                            }
                         });
                     }
                 };
-                if (masked) {
+                bool wide = __any_sync(0xffffffffu, small_here);
+                if (wide) {  // most often the zeros behind a sequence's end: only tokens that a row gives weight count
+                    uint32_t weighted[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+                    for (int n = 0; n < N; ++n) {
+                        float w[8];
+                        weights(n, w);
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) weighted[x] |= (w[2 * x] > 0.0f ? 0xffffu : 0u) | (w[2 * x + 1] > 0.0f ? 0xffff0000u : 0u);
+                    }
+                    auto closer = [&](auto but_empty) {  // but_empty: not the blocks in which no token of the tile has anything
+                        __half2 low[4] = {bits_h2(0x7bff7bffu), bits_h2(0x7bff7bffu), bits_h2(0x7bff7bffu), bits_h2(0x7bff7bffu)};
+#pragma unroll
+                        for (int b = 0; b < NB; ++b) {
+                            const uint32_t d[4] = {dv[b].x, dv[b].y, dv[b].z, dv[b].w};
+                            if (decltype(but_empty)::value && !__any_sync(0xffffffffu, ((d[0] | d[1] | d[2] | d[3]) & 0x7fff7fffu) != 0)) continue;
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) low[x] = __hmin2(low[x], __habs2(bits_h2(d[x])));
+                        }
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) low[x] = bits_h2((h2_bits(low[x]) & weighted[x]) | (0x7bff7bffu & ~weighted[x]));
+                        return (bool)__any_sync(0xffffffffu, small_of(low));
+                    };
+                    wide = closer(std::false_type()) && closer(std::true_type());
+                }
+                if (wide) {
+                    output(std::false_type(), std::true_type());
+                } else if (masked) {
                     __syncwarp();
-                    output(std::true_type());
+                    output(std::true_type(), std::false_type());
                 } else {
-                    output(std::false_type());
+                    output(std::false_type(), std::false_type());
                 }
             }
             __syncwarp();  // the tile and the weights have been read
