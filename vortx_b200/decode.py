@@ -28,9 +28,10 @@ def _check_len(what: str, length: Optional[int], rows: int, stride: int, width: 
 
 def _typed(what: str, t, dtypes) -> tuple:
     """Device pointer and length of t.  Where the element type is known it must be one of dtypes; the last dimension of a
-    view must be dense (the others' strides are the call's stride arguments)."""
+    view must be dense (the others' strides are the call's stride arguments).  A buffer must not have been freed: its
+    address is zero then, which would mean an argument that is not given, and a view's is one near it."""
     if type(t) is GpuBuffer:                                # these calls cost as much on the host as on the device
-        if t.dtype in dtypes:
+        if t.dtype in dtypes and t.ptr:
             return t.ptr, t._len
         buf = t
     elif hasattr(t, "as_tensor_ref"):
@@ -42,7 +43,20 @@ def _typed(what: str, t, dtypes) -> tuple:
         return _ptr_len(t)
     if buf.dtype not in dtypes:
         raise TypeError(f"{what} must hold {dtypes[0].name} elements, not {buf.dtype.name}")
+    if not buf.ptr and buf._len:
+        raise ValueError(f"{what} has been freed")
     return _ptr_len(t)
+
+
+class _Pointer:
+    """In place of a buffer where a plain pointer was given: nobody knows whether it is still good."""
+
+    ptr = 1
+
+
+def _buffer_of(t):
+    buf = t if type(t) is GpuBuffer else t.as_tensor_ref().raw_buffer() if hasattr(t, "as_tensor_ref") else _Pointer
+    return buf if buf.ptr else _Pointer                     # of no elements
 
 
 class CacheRows:
@@ -50,7 +64,7 @@ class CacheRows:
     p lies in page table[s, p // page_tokens].  The arrays are int32 on the device (table [seqs, max_pages], begin
     [seqs + 1], start [seqs]) and are read when the call runs; `rows` is how many rows the call's tensors have.
     `seqs` and `max_pages` follow from the lengths unless plain pointers are given.  Pointers are captured at
-    construction."""
+    construction; calls after one of the buffers has been freed are refused."""
 
     def __init__(self, table, begin, start, rows: int, seqs: Optional[int] = None, max_pages: Optional[int] = None):
         (tp, tl), (bp, bl), (sp, sl) = (_typed(n, t, _WORDS) for n, t in (("table", table), ("begin", begin), ("start", start)))
@@ -71,8 +85,16 @@ class CacheRows:
             raise ValueError("rows, seqs and max_pages must not be negative")
         self.rows, self.seqs, self.max_pages = rows, seqs, max_pages
         self._keep = (table, begin, start)
+        self._buffers = _buffer_of(table), _buffer_of(begin), _buffer_of(start)
         self._c = _lib.VxKvRows(tp or None, max_pages, bp or None, sp or None, seqs, rows)
-        self._ref = C.byref(self._c)
+        self._pointer = C.byref(self._c)
+
+    @property
+    def _ref(self):
+        table, begin, start = self._buffers
+        if not (table.ptr and begin.ptr and start.ptr):
+            raise ValueError("the rows' table, begin or start has been freed")
+        return self._pointer
 
 
 class QuantizedCache:
