@@ -1,4 +1,4 @@
-"""What the decode-step operators' Python layer refuses of buffers that have been freed (no GPU)."""
+"""What the decode-step operators' Python layer refuses of buffers that have been freed and of views with gaps (no GPU)."""
 import ctypes as C
 
 import numpy as np
@@ -111,3 +111,58 @@ def test_empty_tensors_need_no_address():
     cache, _, _ = _objects()
     with pytest.raises(vb.VortxError):
         cache.append(None, empty, empty, rows)
+
+
+def _view(shape, stride, dtype=np.float32, offset=0, size=1 << 16):
+    return TensorRef(TensorLayout.contiguous([size]).view(offset, shape, stride), _buf(size, dtype))
+
+
+@pytest.mark.parametrize("what,shape,stride,dtype", [("table", [3, 4], [9, 1], np.int32), ("begin", [4], [2], np.int32), ("start", [3, 1], [5, 1], np.int32)])
+def test_rows_of_arrays_with_gaps_are_refused(what, shape, stride, dtype):
+    """Four columns of a page table of nine: the kernels take the pages of all sequences one after the other."""
+    arrays = {"table": _i32(12), "begin": _i32(4), "start": _i32(3)}
+    arrays[what] = _view(shape, stride, dtype)
+    with pytest.raises(ValueError, match="dense|stride 1"):
+        vb.CacheRows(**arrays, rows=3, seqs=3, max_pages=4)
+    arrays[what] = _view(shape, [int(np.prod(shape[i + 1:])) for i in range(len(shape))], dtype)
+    vb.CacheRows(**arrays, rows=3, seqs=3, max_pages=4)
+
+
+def test_views_with_gaps_need_the_stride_argument():
+    """Rows of a wider matrix (q, k and v of one projection) without saying how far apart they are; heads that are not next to each
+    other; a mask, ids or weights with gaps, which have no stride argument."""
+    rows = vb.CacheRows(_i32(1), _i32(2), _i32(1), 3)
+    gaps = dict(k=_view([3, 128], [384, 1]), q=_view([3, 256], [512, 1]), x=_view([3, 64], [96, 1]))
+    for name, call in _calls(rows, **gaps).items():
+        with pytest.raises(ValueError, match="dense"):
+            call()
+    for kw in ({"mask": _view([3, 1], [2, 1], np.uint32)}, {"ids": _view([3, 2], [4, 1], np.int32)}, {"weights": _view([3, 2], [4, 1])}):
+        for name, call in _calls(rows, **kw).items():
+            if name.startswith("attention" if "mask" in kw else "layer"):
+                with pytest.raises(ValueError, match="dense"):
+                    call()
+    cache, att, layer = _objects()
+    b = _NoBackend()
+    # with the stride they reach the library, which has no object here
+    for call in (lambda: cache.append(None, gaps["k"], gaps["k"], rows, k_stride=384, v_stride=384), lambda: cache.read(None, gaps["k"], None, rows, k_stride=384),
+                 lambda: att.dispatch(b, None, _buf(768), gaps["q"], rows, q_stride=512), lambda: att.dispatch(b, None, gaps["q"], _buf(768), rows, out_stride=512),
+                 lambda: layer.dispatch(b, None, _buf(192), gaps["x"], 3, x_stride=96), lambda: layer.dispatch(b, None, gaps["x"], _buf(192), 3, y_stride=96)):
+        with pytest.raises(vb.VortxError):
+            call()
+    apart = _view([3, 2, 64], [64, 192, 1])             # [heads, rows, 64] seen as [rows, heads, 64]
+    with pytest.raises(ValueError, match="dense"):
+        cache.append(None, apart, _buf(384), rows, k_stride=64)
+    # dense views and single rows of a wider matrix need no stride
+    one = vb.CacheRows(_i32(1), _i32(2), _i32(1), 1)
+    for call in (lambda: cache.append(None, _view([3, 2, 64], [128, 64, 1]), _view([3, 128], [128, 1], offset=512), rows),
+                 lambda: cache.append(None, _view([1, 128], [384, 1]), _view([128], [1], offset=256), one)):
+        with pytest.raises(vb.VortxError):
+            call()
+
+
+def test_a_router_with_gaps_is_refused():
+    w = vb.QuantizedMatrix.__new__(vb.QuantizedMatrix)
+    w._h, w.backend, w.rows, w.cols = None, _NoBackend(), 128, 64
+    for router, error in ((_view([4, 64], [80, 1]), ValueError), (_view([4, 64], [64, 1]), vb.VortxError)):
+        with pytest.raises(error):
+            vb.MoeLayer(_NoBackend(), router, w, w, w, 4, 2)

@@ -1,7 +1,8 @@
 """What a decode step does besides its projections, on block-quantised data: a cache of keys and values that is
 quantised as it is written (vx_kv_*), attention of new or drafted tokens over it (vx_kv_attention), and a
 mixture-of-experts layer (vx_moe).  vortx has no counterpart; the calls take the shape of Gemv.dispatch
-(backend, pass, outputs, inputs).  Tensors, views, buffers and plain device pointers are accepted alike.
+(backend, pass, outputs, inputs).  Tensors, views, buffers and plain device pointers are accepted alike; a view with
+gaps between its rows needs the call's stride argument, where it has one.
 """
 from __future__ import annotations
 
@@ -26,9 +27,21 @@ def _check_len(what: str, length: Optional[int], rows: int, stride: int, width: 
         raise IndexError(f"{what} is shorter than {rows} rows")
 
 
-def _typed(what: str, t, dtypes) -> tuple:
-    """Device pointer and length of t.  Where the element type is known it must be one of dtypes; the last dimension of a
-    view must be dense (the others' strides are the call's stride arguments).  A buffer must not have been freed: its
+def _dense(view, width: Optional[int]) -> bool:
+    """Whether a view's elements are next to each other: all of them, or those of each row of `width` elements."""
+    below = 1
+    for i in range(view.rank() - 1, -1, -1):
+        if width is not None and below >= width:
+            break
+        if view.size(i) > 1 and view.stride(i) != below:
+            return False
+        below *= view.size(i)
+    return True
+
+
+def _typed(what: str, t, dtypes, width: Optional[int] = None) -> tuple:
+    """Device pointer and length of t.  Where the element type is known it must be one of dtypes.  A view must be dense; if the
+    call says how far apart its rows of `width` elements are, only these.  A buffer must not have been freed: its
     address is zero then, which would mean an argument that is not given, and a view's is one near it."""
     if type(t) is GpuBuffer:                                # these calls cost as much on the host as on the device
         if t.dtype in dtypes and t.ptr:
@@ -36,9 +49,9 @@ def _typed(what: str, t, dtypes) -> tuple:
         buf = t
     elif hasattr(t, "as_tensor_ref"):
         view = t.as_tensor_ref()
-        buf, rank = view.raw_buffer(), view.rank()
-        if rank and view.size(rank - 1) > 1 and view.stride(rank - 1) != 1:
-            raise ValueError(f"{what}: the last dimension of the view must have stride 1")
+        buf = view.raw_buffer()
+        if not _dense(view, width):
+            raise ValueError(f"{what}: the {'rows' if width else 'elements'} of the view must be dense")
     else:
         return _ptr_len(t)
     if buf.dtype not in dtypes:
@@ -117,10 +130,10 @@ class QuantizedCache:
         return int(n.value)
 
     def _rows_of(self, what: str, t, rows: CacheRows, stride: Optional[int]):
-        stride = self.width if stride is None else stride
+        apart, stride = stride is not None, self.width if stride is None else stride
         if t is None:
             return None, stride
-        p, n = _typed(what, t, (_F32,))
+        p, n = _typed(what, t, (_F32,), self.width if apart else None)
         _check_len(what, n, rows.rows, stride, self.width)
         return p, stride
 
@@ -186,8 +199,8 @@ class CacheAttention:
         scale defaults to 1 / sqrt(head_dim).  out may be q, with q's stride."""
         qs = self.width if q_stride is None else q_stride
         os = self.width if out_stride is None else out_stride
-        qp, ql = _typed("q", q, (_F32,))
-        op, ol = _typed("out", out, (_F32,))
+        qp, ql = _typed("q", q, (_F32,), None if q_stride is None else self.width)
+        op, ol = _typed("out", out, (_F32,), None if out_stride is None else self.width)
         _check_len("q", ql, rows.rows, qs, self.width)
         _check_len("out", ol, rows.rows, os, self.width)
         mp, words = None, 0
@@ -249,8 +262,8 @@ class MoeLayer:
             raise ValueError("the layer's weights have been freed")
         xs = self.hidden if x_stride is None else x_stride
         ys = self.hidden if y_stride is None else y_stride
-        xp, xl = _typed("x", x, (_F32,))
-        yp, yl = _typed("y", y, (_F32,))
+        xp, xl = _typed("x", x, (_F32,), None if x_stride is None else self.hidden)
+        yp, yl = _typed("y", y, (_F32,), None if y_stride is None else self.hidden)
         _check_len("x", xl, tokens, xs, self.hidden)
         _check_len("y", yl, tokens, ys, self.hidden)
         ip = wp = None
