@@ -121,3 +121,28 @@ def test_blocks_that_only_tokens_of_little_weight_have(backend, vt, dim, heads, 
     got = s.run(scale=1.0)
     _check(s, got, want, scale=1.0)
     assert np.abs(got[:, :, 32:64]).max() > 0 and (dim == 64 or (got[:, :, -32:] == 0).all())
+
+
+@pytest.mark.parametrize("kt", [vb.Q8_0, vb.Q4_0])
+@pytest.mark.parametrize("dim,heads,kv_heads,n", [(64, 2, 2, 1), (96, 4, 2, 2), (128, 8, 2, 3), (256, 4, 2, 4)])
+@pytest.mark.parametrize("up", [16, 18, 20, 24])
+def test_query_rows_of_a_wide_range(backend, kt, dim, heads, kv_heads, n, up):
+    """An element of q is 2^up times the others, where the keys are zero.  The two f16 parts of the others miss at most 2^-39 of the
+    largest (and 2^-23 of themselves): a score moves by that times scale sum |k|, and the result by twice as much of sum p |v|."""
+    s = Scene(backend, [(60, n), (9, n)], heads, kv_heads, dim, 32, kt, vb.Q8_0, seed=dim + up)
+    s.q[:, :, 5] = np.float32(2.0 ** up)
+    for k in s.k:
+        k[:, :, 5] = 0.0
+    _with_values(s, s.v)
+    got, group, scale = s.run(), heads // kv_heads, dim ** -0.5
+    for at, (c, m) in enumerate(s.seqs):
+        k, v = quantised(s.kt, s.k[at]), quantised(s.vt, s.v[at])
+        ok = np.concatenate([np.ones((m, c), bool), np.tril(np.ones((m, m), bool))], 1)
+        for h in range(heads):
+            q, kh, vh = s.q[s.begin[at]:s.begin[at] + m, h].astype(np.float64), k[:, h // group], v[:, h // group]
+            want, tol = attention(q, kh, vh, ok, scale)
+            score = np.where(ok, scale * q @ kh.T, -np.inf)
+            p = np.exp(score - score.max(1, keepdims=True))
+            p /= p.sum(1, keepdims=True)
+            tol += 2 * scale * 2.0 ** (up - 39) * np.abs(kh).sum(1).max() * (p @ np.abs(vh))
+            assert (np.abs(got[s.begin[at]:s.begin[at] + m, h] - want) <= tol).all()

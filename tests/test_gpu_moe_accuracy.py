@@ -2,8 +2,8 @@
 |weight| |input| of its own row, not against the largest input or output of the call.
 
 Tolerance.  That of decode_ref.moe, 2 * 2^-20 of sum |w||x| for a product, covers them: x is split into two f16 parts with the
-largest of a block (or of a few together) below 2^15, so every x keeps 22 bits down to 2^-17 of that and an absolute 2^-40 of it
-below; with a gain of up to 2^10, as here, that is 2^-30 of an ordinary x.  Codes are exact, products are exact, and sums of
+largest of a block (or of a few together) in [2^14, 2^15), so every x keeps 22 bits down to 2^-16 of that and misses at most 2^-39
+of it below; with a gain of up to 2^10, as here, an ordinary x keeps them.  Codes are exact, products are exact, and sums of
 products rise no higher than sum |w||x| of the row."""
 import numpy as np
 import pytest

@@ -1,12 +1,14 @@
 // Device pieces shared by the decode-step kernels (quantised cache, attention over it, expert layer).
 //
 // Products of block-quantised codes with f32 vectors on the tensor cores, to f32 accuracy.  A code (-127..127 or
-// -8..7) is exact in f16.  An f32 value x is scaled by a power of two that brings the largest of its group (a block,
-// a row) to [2^14, 2^15) and split into two f16 parts, hi = f16(x), lo = f16(x - hi): 22 significant bits for values
-// down to 2^-29 of the group's largest, an absolute error of 2^-25 (2^-40 of the largest) below that.  Products of a
-// code and a part are exact in the f32 accumulator; the two parts' sums are added in f32.  One rounding to fewer bits
-// than f32 is therefore made: 22 bits instead of 24 of x, half a step 2^-23 relative, next to sums whose own f32
-// rounding is of that order.
+// -8..7) is exact in f16.  An f32 value x is scaled by a power of two that brings the largest of its group (a row of q, a few
+// blocks of an expert layer's input) to [2^14, 2^15) and split into two f16 parts, hi = f16(x), lo = f16(x - hi).  From 2^-2 on
+// that keeps 22 significant bits, half a step 2^-23 relative: values down to 2^-16 of the group's largest.  Below, lo is one
+// of f16's small numbers and the error an absolute 2^-25: at most 2^-39 of the largest, so 2^-21 relative for a value 2^-18 of
+// the largest, 2^-15 for one of 2^-24.  Products of a code and a part are exact in the f32 accumulator; the two parts'
+// sums are added in f32.  One rounding to fewer bits than f32 is therefore made, 22 bits instead of 24 of x, next to sums
+// whose own f32 rounding is of that order; of a value so small that it is more, the group's largest is in the same sum (unless its
+// code is zero).
 #pragma once
 
 #include <cuda_fp16.h>
