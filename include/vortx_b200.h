@@ -181,7 +181,8 @@ VX_API vx_status vx_gemv_q_multi(vx_context* ctx, const vx_qweights* const* ws, 
  * infinity, or whose scale passes f16, reads back as NaN throughout (its scale is NaN).
  * The cache is `pages` pages of `page_tokens` tokens (a multiple of 32); which page holds which tokens of a sequence
  * is the caller's page table.  The device form is tiles of 32 tokens of one head in the order in which the
- * attention kernel reads them.  Zero at creation.  Any context of the cache's device may use it. */
+ * attention kernel reads them.  Zero at creation.  Any context of the cache's device may use it.  head_dim is any multiple of 32
+ * up to 512; vx_kv_attention takes 64, 96, 128 and 256 of them. */
 typedef struct vx_kv_cache vx_kv_cache;
 VX_API vx_status vx_kv_cache_create(vx_context* ctx, vx_qtype k_type, vx_qtype v_type, size_t heads, size_t head_dim,
                                     size_t pages, size_t page_tokens, vx_kv_cache** out);
@@ -194,8 +195,12 @@ VX_API vx_status vx_kv_cache_info(const vx_kv_cache* cache, int32_t* k_type, int
  * `rows` is the number of rows that the call's tensors have.  Whatever the arrays hold, nothing outside the tensors
  * and the cache is touched: tokens behind the page table's end and tokens whose page number is negative or too large
  * have no place (they are not written, read back as zeros, and are not attended to); a sequence whose start is
- * negative has no rows; rows that no sequence names take no part (nothing is written to or for them).  The places of two rows of a call must differ: sequences that share
- * a page may both read it, and what is kept of a block that two rows write at once is not defined. */
+ * negative has no rows; rows that no sequence names take no part (nothing is written to or for them).  The places of two
+ * rows of a call must differ: sequences that share a page may both read it, and what is kept of a block that two rows
+ * write at once is not defined.
+ * The host knows rows and sequences, not who has how many: vx_kv_attention_run groups rows by their average, in which
+ * sequences without rows count.  One sequence of 64 rows over 16000 tokens takes 53 us, with 15 empty ones beside it 85 (8
+ * heads of 128, one query head each); 15 of one row and one of 256 take what two calls would (216 and 211 us). */
 typedef struct {
     const int32_t* table; /* [seqs][max_pages] */
     size_t max_pages;
@@ -218,12 +223,14 @@ VX_API vx_status vx_kv_read(vx_context* ctx, const vx_kv_cache* cache, const vx_
  *   out[r, h, :] = sum_p softmax_p(scale * q[r, h, :] . k[p, h / group, :]) v[p, h / group, :],   group = heads / cache heads
  * q and out are rows of heads * head_dim floats, q_stride / out_stride apart; a row that attends to nothing is zeros; rows
  * of no sequence are left as they were.  out may be q, with q's stride; it must not overlap q otherwise.  Scores, softmax
- * and sums are f32; q and the weights of the softmax enter the tensor cores as two f16 parts (22 bits,
- * csrc/vx_decode.cuh).  head_dim is 64, 96, 128 or 256 (VX_ERR_UNSUPPORTED otherwise).  What lies in masked places, NaN
+ * and sums are f32.  q and the weights of the softmax times the values' scales enter the tensor cores as two f16 parts (22
+ * bits, csrc/vx_decode.cuh): an element of q is off by 2^-23 of itself or 2^-39 of its row's largest, whichever is more, and
+ * a token's weight times scale by 2^-22 of itself or 2^-21 of the largest that its row has in that block of 32 values within
+ * the token's tile.  head_dim is 64, 96, 128 or 256 (VX_ERR_UNSUPPORTED otherwise).  What lies in masked places, NaN
  * included, does not reach the result.  One launch.
  * A vx_kv_attention is the workspace of such calls (partial results of sequences that are split over the GPU's SMs),
- * made once for up to max_seqs sequences of a cache, which must outlive it; calls with it follow each other on its
- * context's stream.  A recorded call keeps using it: graphs that may run at the same time need a vx_kv_attention each. */
+ * made once for a cache, which must outlive it; calls with it follow each other on its context's stream.  max_seqs is the
+ * number of sequences that a call may have; the workspace's size does not depend on it.  A recorded call keeps using it: graphs that may run at the same time need a vx_kv_attention each. */
 typedef struct vx_kv_attention vx_kv_attention;
 VX_API vx_status vx_kv_attention_create(vx_context* ctx, const vx_kv_cache* cache, size_t heads, size_t max_seqs,
                                         vx_kv_attention** out);
@@ -242,12 +249,13 @@ VX_API vx_status vx_kv_attention_run(vx_context* ctx, const vx_kv_attention* att
  * its own type): the order of a weight file's three-dimensional expert tensors.  The handles are kept, not copied, and
  * must outlive the layer.
  * Only the weights of experts that get a token are read, each once per 8 of its tokens.  Three launches.
- * Sums are f32; x and the inner vector enter the tensor cores as two f16 parts per block (csrc/vx_decode.cuh).
+ * Sums are f32; x and the inner vector enter the tensor cores as two f16 parts (csrc/vx_decode.cuh): a value is off by 2^-23 of
+ * itself or 2^-39 of the largest of its 128 (gate and up in Q4_0), 64 (Q8_0) or, of the inner vector, 32 neighbours.
  * experts <= 256, top_k <= 16 and <= experts, max_tokens <= 64.  The layer owns the workspace of its calls, with the same rule
  * as vx_kv_attention for calls that overlap.
  * run: x is `tokens` rows of `hidden` floats, x_stride apart; y likewise.  ids / weights (device, [tokens][top_k], may be
- * NULL) receive the chosen experts, best first, and their weights.  y may be x or overlap it.  Inputs whose magnitude
- * is 2^105 or more count as infinite. */
+ * NULL) receive the chosen experts, best first, and their weights.  y may be x or overlap it.  Inputs and inner
+ * values whose magnitude is 2^105 or more count as infinite. */
 typedef struct vx_moe vx_moe;
 VX_API vx_status vx_moe_create(vx_context* ctx, const float* router, size_t experts, const vx_qweights* gate,
                                const vx_qweights* up, const vx_qweights* down, size_t top_k, int32_t normalise,

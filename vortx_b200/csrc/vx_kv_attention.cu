@@ -131,7 +131,6 @@ vx_status vx_kv_attention_run(vx_context* ctx, const vx_kv_attention* a, const v
     p.out = out;
     p.q_stride = q_stride;
     p.out_stride = out_stride;
-    p.heads = (uint32_t)a->heads;
     p.group = group;
     p.scale_log2 = scale * 1.4426950408889634f;
     p.mask = mask;

@@ -45,7 +45,7 @@ struct AttnParams {
     const float* q;
     float* out;
     size_t q_stride, out_stride;
-    uint32_t heads, group;   // query heads, of one head of keys
+    uint32_t group;          // query heads of one head of keys
     float scale_log2;        // scale * log2 e
     const uint32_t* mask;
     uint32_t mask_words;

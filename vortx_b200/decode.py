@@ -178,7 +178,7 @@ def tree_mask(parents: Sequence[int]) -> np.ndarray:
 
 
 class CacheAttention:
-    """Attention over a QuantizedCache (vx_kv_attention); holds the workspace of its calls, for up to `max_seqs` sequences.
+    """Attention over a QuantizedCache (vx_kv_attention); holds the workspace of its calls, of up to `max_seqs` sequences each.
     `heads` query heads share the cache's heads evenly."""
 
     def __init__(self, backend: Backend, cache: QuantizedCache, heads: int, max_seqs: int):
