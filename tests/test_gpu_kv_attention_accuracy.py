@@ -146,3 +146,19 @@ def test_query_rows_of_a_wide_range(backend, kt, dim, heads, kv_heads, n, up):
             p /= p.sum(1, keepdims=True)
             tol += 2 * scale * 2.0 ** (up - 39) * np.abs(kh).sum(1).max() * (p @ np.abs(vh))
             assert (np.abs(got[s.begin[at]:s.begin[at] + m, h] - want) <= tol).all()
+
+
+@pytest.mark.parametrize("vt", [vb.Q8_0, vb.Q4_0])
+@pytest.mark.parametrize("dim,heads,kv_heads", [(64, 2, 2), (96, 4, 2), (128, 16, 2), (256, 2, 2)])
+def test_tiles_that_only_have_tokens_of_little_weight(backend, vt, dim, heads, kv_heads):
+    """Small values of the last two of eight tiles, of 2^-44 of the earlier tokens' weight, are all that stands in the second block."""
+    s = Scene(backend, [(254, 1)], heads, kv_heads, dim, 64, vb.Q8_0, vt, seed=dim + heads)
+    light = np.arange(255) >= 192
+    s.q[:] = 0.0
+    s.q[:, :, 0] = 1.0
+    s.k[0][:, :, 0] = np.where(light, -30.5, 0.0)[:, None]       # 44 ln 2
+    s.k[0][:, :, 1:] *= np.float32(0.01)
+    v = s.v[0] * np.float32(2.0 ** (-8 if vt == vb.Q8_0 else -12))
+    v[~light, :, 32:64] = 0.0
+    want = _with_values(s, [v])
+    _check(s, s.run(scale=1.0), want, scale=1.0)

@@ -672,8 +672,8 @@ kv_attention_kernel(AttnParams p) {
                     for (int n = 0; n < N; ++n) largest[n] = fmaxf(largest[n], __shfl_xor_sync(0xffffffffu, largest[n], o));
 #pragma unroll
                 for (int n = 0; n < N; ++n) {
-                    // 2^12 over the power of two below the largest, 2^40 at most: what a row without weights has here
-                    const float up = __uint_as_float(min(((12u + 2u * 127u) << 23) - (__float_as_uint(largest[n]) & 0x7f800000u), (40u + 127u) << 23));
+                    // 2^12 over the power of two below the largest; 2^64 at most, which a row without weights has (its output stays below 2^120)
+                    const float up = __uint_as_float(min(((12u + 2u * 127u) << 23) - (__float_as_uint(largest[n]) & 0x7f800000u), (64u + 127u) << 23));
 #pragma unroll
                     for (int e = 0; e < E; ++e) now[n][e] = __shfl_sync(0xffffffffu, up, kParts ? 8 * t : 8 * t + 4 * e);
 #pragma unroll
