@@ -79,21 +79,25 @@ __device__ __forceinline__ uint4 lds128(uint32_t a) {
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 __device__ __forceinline__ __half2 bits_h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
 
-// Codes to f16 pairs.  0x6400 | u is the f16 number 1024 + u for u < 1024, so a byte or nibble put into the low bits of
-// 0x6400 becomes a number with one logic operation, and one exact f16 operation takes the offset away.
+// Codes to f16 pairs.  A byte or nibble u (code + 128 or + 8) alone in the low bits of a half is the f16 number u 2^-24, or 16 u
+// 2^-24 at bits 4..7: one byte permutation or logic operation.  One exact f16 multiply-add makes it code 2^-9, a normal number
+// (the tensor cores align products by the exponent field, so the leading zeros of a small one would be lost bits).
+// Putting u under the exponent of 1024 needs a mask and an exponent, two constants, and took a quarter more instructions
+// (8 experts of 14336 x 4096: 209 us, so 197).
+constexpr float kCodeUnits = 512.0f;  // of 2^-9 in 1
+__device__ __forceinline__ uint32_t fma_h2(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t d;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    return d;
+}
 // bytes (two of `w`, picked by `sel`, e.g. 0x4140 = bytes 0 and 1) that hold code + 128
 __device__ __forceinline__ uint32_t f16_of_bytes(uint32_t w, uint32_t sel) {
-    const uint32_t u = __byte_perm(w, 0x64646464u, sel);
-    return h2_bits(__hsub2(bits_h2(u), bits_h2(0x64806480u)));  // 1152
+    return fma_h2(__byte_perm(w, 0, sel), 0x78007800u, 0xb400b400u);  // 2^15, -128 2^-9
 }
 // nibbles at bits 0..3 and 16..19 that hold code + 8
-__device__ __forceinline__ uint32_t f16_of_low_nibbles(uint32_t w) {
-    return h2_bits(__hsub2(bits_h2((w & 0x000f000fu) | 0x64006400u), bits_h2(0x64086408u)));  // 1032
-}
-// nibbles at bits 4..7 and 20..23: 1024 + 16 n; times 1/16 minus 72
-__device__ __forceinline__ uint32_t f16_of_high_nibbles(uint32_t w) {
-    return h2_bits(__hfma2(bits_h2((w & 0x00f000f0u) | 0x64006400u), bits_h2(0x2c002c00u), bits_h2(0xd480d480u)));
-}
+__device__ __forceinline__ uint32_t f16_of_low_nibbles(uint32_t w) { return fma_h2(w & 0x000f000fu, 0x78007800u, 0xa400a400u); }  // 2^15, -8 2^-9
+// nibbles at bits 4..7 and 20..23
+__device__ __forceinline__ uint32_t f16_of_high_nibbles(uint32_t w) { return fma_h2(w & 0x00f000f0u, 0x68006800u, 0xa400a400u); }  // 2^11
 
 // Splits a and b: hi = their f16 parts as a pair (a low), lo = what those miss.
 __device__ __forceinline__ void split_f16(float a, float b, uint32_t* hi, uint32_t* lo) {

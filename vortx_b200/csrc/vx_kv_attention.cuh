@@ -441,7 +441,7 @@ kv_attention_kernel(AttnParams p) {
             }
             const float up = lift(warp_max(most));
             if (r >= R) break;
-            if (lane == 0) inv_lift[r] = 1.0f / up;
+            if (lane == 0) inv_lift[r] = kCodeUnits / up;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 const float v = qv[x][b] * up;
@@ -454,7 +454,7 @@ kv_attention_kernel(AttnParams p) {
         __syncthreads();
         const uint32_t qs = smem_addr(qf) + lane * 16;
         float inv[N][E];
-        float top[N][E], sum[N][E], acc[2 * NB][N][2 * E], unit[N][E];  // acc counts 1 / (2 unit)
+        float top[N][E], sum[N][E], acc[2 * NB][N][2 * E], unit[N][E];  // acc counts kCodeUnits / (2 unit)
 #pragma unroll
         for (int n = 0; n < N; ++n) {
 #pragma unroll
@@ -867,7 +867,7 @@ kv_attention_kernel(AttnParams p) {
                 float m = kNone;
 #pragma unroll
                 for (uint32_t w = 0; w < W; ++w) m = fmaxf(m, ml[w * R + row_of(n, e)].x);
-                const float f = top[n][e] == kNone ? 0.0f : ex2(top[n][e] - m) * __uint_as_float(0x7e800000u - __float_as_uint(unit[n][e]));
+                const float f = top[n][e] == kNone ? 0.0f : ex2(top[n][e] - m) * (0.5f * kCodeUnits * __uint_as_float(0x7f000000u - __float_as_uint(unit[n][e])));
 #pragma unroll
                 for (int d = 0; d < 2 * NB; ++d) {
                     acc[d][n][e] *= f;

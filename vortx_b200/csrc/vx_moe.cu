@@ -100,7 +100,7 @@ __device__ __forceinline__ void logits_of(const MoeParams& p, uint32_t expert, u
 // The power of two that values, `most` the largest magnitude, are split with.  f16 ends just below 2^16: values from 2^105 on
 // count as infinite.
 __device__ __forceinline__ float split_lift(float most) { return fmaxf(lift(most), __uint_as_float((127u - 89u) << 23)); }
-__device__ __forceinline__ float split_factor(float up) { return __uint_as_float(0x7f000000u - __float_as_uint(up)); }  // 1 / up
+__device__ __forceinline__ float split_factor(float up) { return kCodeUnits * __uint_as_float(0x7f000000u - __float_as_uint(up)); }  // over up
 // One block of 32 values (a lane each) as two parts in B-operand order.
 __device__ __forceinline__ void split_block(float v, float up, uint32_t lane, bool four, uint8_t* hi, uint8_t* lo) {
     const float x = v * up;
