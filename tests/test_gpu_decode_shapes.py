@@ -38,6 +38,13 @@ def test_units_of_whole_chunks(backend, gt, experts, hidden, inner, top_k, token
     assert all(np.array_equal(a, b) for a, b in zip(first, l.run(x)))
 
 
+@pytest.mark.parametrize("gt,dt", [(vb.Q8_0, vb.Q4_0), (vb.Q4_0, vb.Q8_0)])
+@pytest.mark.parametrize("experts,hidden,inner,top_k,tokens", [(256, 64, 64, 16, 64), (256, 96, 32, 1, 64), (129, 128, 96, 7, 63), (2, 8224, 64, 2, 64)])
+def test_the_most_experts_and_tokens(backend, gt, dt, experts, hidden, inner, top_k, tokens):
+    l = Layer(backend, experts, hidden, inner, top_k, tokens % 2 == 0, gt, dt, max_tokens=tokens, seed=experts + top_k)
+    l.check(_rng(tokens).standard_normal((tokens, hidden)).astype(np.float32))
+
+
 def _repeat(s, *args):
     first = s.run(*args)
     assert np.array_equal(first, s.run(*args))
@@ -74,3 +81,43 @@ def test_drafts_of_two_sequences_dealt_out_evenly(backend):
             at = slice(s.begin[i], s.begin[i + 1])
             want, tol = attention(s.q[at, h], kq[:, h // group], vq[:, h // group], ok, 0.125)
             assert (np.abs(got[at, h] - want) <= 2 * tol).all()
+
+
+@pytest.mark.parametrize("seqs,heads,kv_heads,dim,kt,vt", [
+    ([(0, 300)], 4, 2, 64, vb.Q8_0, vb.Q8_0), ([(513, 257)], 8, 2, 128, vb.Q8_0, vb.Q4_0), ([(31, 1), (700, 190), (0, 0), (5, 64)], 6, 2, 96, vb.Q4_0, vb.Q8_0),
+    ([(1000, 1)] * 9 + [(200, 180)], 4, 4, 64, vb.Q4_0, vb.Q4_0), ([(40, 140)], 2, 1, 256, vb.Q8_0, vb.Q8_0)])
+def test_pieces_of_prompts(backend, seqs, heads, kv_heads, dim, kt, vt):
+    """Hundreds of rows of a sequence, each attending to the tokens up to itself, alone and next to sequences of one row or none."""
+    s = Scene(backend, seqs, heads, kv_heads, dim, 64, kt, vt, seed=len(seqs) + dim, pad=3)
+    s.check(_repeat(s))
+
+
+def test_pages_behind_four_gigabytes(backend):
+    """A cache of 5.9 GB whose sequences lie in its first and last pages: byte offsets of more than 32 bits."""
+    rng = _rng(40)
+    heads, kv, dim, page, pages, context = 8, 4, 256, 64, 42000, 200
+    cache = vb.QuantizedCache(backend, vb.Q8_0, vb.Q8_0, kv, dim, pages, page)
+    assert cache.device_bytes() > 5 << 30
+    dev = lambda a: backend.init_buffer(np.ascontiguousarray(a).ravel())  # noqa: E731
+    i32 = lambda a: dev(np.asarray(a, np.int32))  # noqa: E731
+    table = i32([[pages - 1, 0, pages - 7, 31000], [1, pages - 2, 30900, 2]])
+    k, v = (rng.standard_normal((2, context, kv, dim)).astype(np.float32) for _ in range(2))
+    q = rng.standard_normal((2, heads, dim)).astype(np.float32)
+    cache.append(None, dev(k), dev(v), vb.CacheRows(table, i32([0, context, 2 * context]), i32([0, 0]), 2 * context))
+    back = backend.uninit_buffer(v.size)
+    cache.read(None, None, back, vb.CacheRows(table, i32([0, context, 2 * context]), i32([0, 0]), 2 * context))
+    got = np.empty(v.size, np.float32)
+    backend.slow_read_buffer(back, got)
+    assert np.array_equal(got.reshape(v.shape), quantised(vb.Q8_0, v).astype(np.float32))
+    att = vb.CacheAttention(backend, cache, heads, 2)
+    out = backend.uninit_buffer(q.size)
+    att.dispatch(backend, None, out, dev(q), vb.CacheRows(table, i32([0, 1, 2]), i32([context - 1] * 2), 2))
+    got = np.empty(q.size, np.float32)
+    backend.slow_read_buffer(out, got)
+    kq, vq = quantised(vb.Q8_0, k), quantised(vb.Q8_0, v)
+    for s in range(2):
+        for h in range(heads):
+            want, tol = attention(q[s, h:h + 1], kq[s, :, h // 2], vq[s, :, h // 2], np.ones((1, context), bool), dim ** -0.5)
+            assert (np.abs(got.reshape(q.shape)[s, h] - want[0]) <= tol[0]).all()
+    att.free()
+    cache.free()
