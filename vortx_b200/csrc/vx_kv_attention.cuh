@@ -20,10 +20,12 @@
 // (sequence, head, rows) only in part leaves maximum, sum and unnormalised output in the workspace, at most two per block,
 // and the last block to finish a part joins them all, in their order.
 // Measured (recorded), 32 heads over 8 of 128 in Q8_0: a token each of 16 sequences of up to 16384 tokens 73 us (392 MB at 5.4 TB/s,
-// 0.82 of the copy rate), of one of 500 9.3 us; 4 x 8 drafted tokens over 4000 30 us, 2 x 48 over 12000 149 us; one token
-// of 16 heads of 64 over 60001 in Q4_0 34 us (589 instructions a tile of 32 tokens; 16 warps of 128 registers are no faster).
+// 0.82 of the copy rate), of one of 500 9.2 us; 4 x 8 drafted tokens over 4000 30 us, 2 x 48 over 12000 149 us; one token
+// of 16 heads of 64 over 60001 in Q4_0 30 us (537 instructions a tile of 32 tokens; 16 warps of 128 registers were no faster).
 // With many rows the products take 0.4 of what the tensor cores could do: the chain scores -> maximum -> weights ->
 // output binds (0.5 instructions a cycle and scheduler with 8 warps of 255 registers as with 12 of 168).
+// Looking for scales that f16 cannot hold costs 0 to 2 %, and 3 % where most tiles are a sequence's last; having them in every tile
+// 10 to 45 %.
 #pragma once
 
 #include <type_traits>
@@ -343,6 +345,7 @@ struct AttnLayout {  // of W warps
 // instead of the 160 of two blocks of four for 48 drafted tokens of 32 heads over 12000, with eight rows to a block).  Sixteen rows
 // need more registers than that: two blocks of four, 255 registers (156 us with six and 168 for those tokens, 149 so; 16
 // tokens over 500: 15.7 and 14.7; heads of 64 over 12000: 95.5 and 98).  The largest heads have one block.
+// With eight or sixteen rows of 128 or 256 values some registers spill: up to 48 bytes, 256 for sixteen rows of 256.
 constexpr bool attn_fits(uint32_t smem, uint32_t blocks) { return blocks * (smem + 1024) <= 228 * 1024; }
 template <bool K4, bool V4, int NB, int NT>
 constexpr int attn_warps() {

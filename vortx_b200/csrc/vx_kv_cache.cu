@@ -6,8 +6,9 @@
 // written as whole 64-byte pieces, four loads per lane under way.  A tile that the call covers completely is put
 // together in shared memory and goes out as 16-byte vectors; the others' codes are stored where they belong.
 // The floor is the f32 side of the copy: 4 bytes a value next to 1.06 (Q8_0) or 0.56 (Q4_0).  Measured, 16 x 1024 tokens of
-// 8 heads of 128 in Q4_0 (134 MB of f32, 19 MB of codes): append 47 us (3.3 TB/s), bound by its instructions (29 lane operations
-// per value, a fifth of which find out where things are); read 32 us (4.8 TB/s).  Eight lanes to a block took 66 and 36 us. One
+// 8 heads of 128 in Q4_0 (134 MB of f32, 19 MB of codes): append 47 us (3.3 TB/s; 29 lane operations
+// per value, a fifth of which find out where things are, at 0.64 a cycle and scheduler: it waits for its loads and at the two
+// barriers a head around the block's image); read 32 us (4.8 TB/s).  Eight lanes to a block took 66 and 36 us. One
 // token: 4.6 us for both calls, recorded.
 #include <algorithm>
 #include <memory>

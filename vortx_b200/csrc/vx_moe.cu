@@ -12,12 +12,15 @@
 // tokens, or eight tokens, whose parts are then multiplied one after the other into the same sums.
 // A code becomes its f16 number before it is multiplied (one logic operation or byte permutation and one f16 operation per
 // pair).  Taking the bits of code + 8 or + 128 as a subnormal f16 number, and 8 or 128 times the vector's sum off afterwards,
-// would save the f16 operation (2 to 7 % of the time below), but its error goes with 128 times the block's largest value, not
-// with the row's own products: 1.5e-5 of sum |w||x| beside values 1000 times the others, and 5e-7 of the largest output
-// on even inputs, where this form has 3e-7.
-// Measured (recorded calls): 8 tokens, 2 of 8 experts of 14336 x 4096, Q4_0 gate and up, Q8_0 down: 209 us; 32 tokens, 4 of 32
-// experts of 1408 x 2048, Q4_0: 83 us; 7 tokens, 3 of 16 experts of 608 x 1120, Q8_0: 18.6 us; one token, 8 of 64 experts of
-// 1024 x 2048, Q4_0: 20.5 us, of which the router's launch takes 4.
+// would save the f16 operation, but its error goes with 128 times the block's largest value, not with the row's own
+// products: 1.5e-5 of sum |w||x| beside values 1000 times the others, and 5e-7 of the largest output on even inputs,
+// where this form has 3e-7.
+// Measured (recorded calls): 8 tokens, 2 of 8 experts of 14336 x 4096, Q4_0 gate and up, Q8_0 down: 197 us (alone: inner 117, 4.0
+// TB/s, down 77, 5.7 TB/s); 32 tokens, 4 of 32 experts of 1408 x 2048, Q4_0: 76 us; 7 tokens, 3 of 16 experts of 608 x 1120,
+// Q8_0: 18.1 us; one token, 8 of 64 experts of 1024 x 2048, Q4_0: 19.4 us.  The inner kernel reads at 0.61 of the copy rate with 76
+// instructions per 32 x 32 weights (36 of them to take the codes apart) at 0.57 a cycle and scheduler: neither issue slots nor
+// memory are full.  What it waits for most are the vectors' parts, which each warp reads from the L2 into its registers;
+// 128 registers leave four warps a scheduler to hide that, and its Q4_0 forms spill 12 to 60 bytes.
 #include <algorithm>
 #include <cstddef>
 #include <memory>
