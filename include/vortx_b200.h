@@ -199,8 +199,8 @@ VX_API vx_status vx_kv_cache_info(const vx_kv_cache* cache, int32_t* k_type, int
  * rows of a call must differ: sequences that share a page may both read it, and what is kept of a block that two rows
  * write at once is not defined.
  * The host knows rows and sequences, not who has how many: vx_kv_attention_run groups rows by their average, in which
- * sequences without rows count.  One sequence of 64 rows over 16000 tokens takes 53 us, with 15 empty ones beside it 85 (8
- * heads of 128, one query head each); 15 of one row and one of 256 take what two calls would (216 and 211 us). */
+ * sequences without rows count.  One sequence of 64 rows over 16000 tokens takes 53 us, with 15 empty ones beside it 78 (8
+ * heads of 128, one query head each); 15 of one row and one of 256 take what two calls would (212 and 206 us). */
 typedef struct {
     const int32_t* table; /* [seqs][max_pages] */
     size_t max_pages;
